@@ -1,0 +1,218 @@
+// The KV-cache codec's entry points: checks, the kernels' parameters and their launch.
+#include <cstring>
+
+#include "gpu_kv_codec_api.h"
+#include "host_common.h"
+#include "kv_codec.cuh"
+
+namespace kv = confkv::kv;
+using namespace confkv::host;
+
+static_assert(LMCACHE_GPU_KV_INT8 == kv::kInt8 && LMCACHE_GPU_KV_FP8 == kv::kFp8 && LMCACHE_GPU_KV_MXFP4 == kv::kMxFp4);
+static_assert(LMCACHE_GPU_KV_BF16 == kv::kBf16 && LMCACHE_GPU_KV_FP16 == kv::kFp16 && LMCACHE_GPU_KV_FP32 == kv::kFp32);
+
+namespace {
+
+constexpr uint64_t kMaxTiles = 1u << 30;   // of a launch
+
+bool layout_ok(const lmcache_gpu_kv_layout* l)
+{
+    return l != nullptr && l->format >= kv::kInt8 && l->format <= kv::kMxFp4 && l->dtype >= kv::kBf16 &&
+           l->dtype <= kv::kFp32 && l->planes >= 1 && l->planes <= 2 && l->layers >= 1 && l->layers <= 65535 &&
+           l->heads >= 1 && l->heads <= 65535 && l->head_dim >= 1 && l->head_dim <= 65535;
+}
+
+// Vectors of an object; above kMaxVectors where it has too many.
+uint64_t object_vectors(const lmcache_gpu_kv_layout& l, uint32_t tokens)
+{
+    const uint64_t rows = uint64_t{l.planes} * l.layers * l.heads;   // < 2^34
+    return tokens != 0 && rows > kv::kMaxVectors / tokens ? uint64_t{kv::kMaxVectors} + 1 : rows * tokens;
+}
+
+bool aligned(const void* p, uint64_t to)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
+}
+
+bool pages_ok(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages& p)
+{
+    const uint32_t bases = l.planes * l.layers;
+    if (p.bases == nullptr || bases > kv::kMaxBases || p.block_size == 0 || p.blocks > kv::kMaxVectors ||
+        p.blocks * p.block_size > kv::kMaxVectors || p.block_stride < 0 || p.row_stride < 0 || p.head_stride < 0) {
+        return false;
+    }
+    for (uint32_t k = 0; k < bases; ++k) {
+        if ((p.bases[k] == nullptr && p.blocks != 0) || !aligned(p.bases[k], kv::element_bytes(l.dtype))) {
+            return false;
+        }
+    }
+    return true;
+}
+
+bool run_ok(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages* pages, const lmcache_gpu_kv_run& r)
+{
+    if (r.count == 0) {
+        return true;
+    }
+    const uint64_t vectors = object_vectors(l, r.tokens);
+    if (vectors > kv::kMaxVectors) {
+        return false;
+    }
+    const uint64_t size = kv::record_layout(l.format, l.head_dim, vectors).size;
+    if (r.record == nullptr || !aligned(r.record, 16) || r.record_bytes < size || !aligned(r.ok, 4)) {
+        return false;
+    }
+    if (r.count > 1 && (r.record_stride < 0 || static_cast<uint64_t>(r.record_stride) < size || r.record_stride % 16 != 0)) {
+        return false;
+    }
+    if (vectors == 0) {
+        return true;
+    }
+    if (pages != nullptr) {
+        return r.slots != nullptr && aligned(r.slots, 8) && r.slots_stride >= 0;
+    }
+    return r.object != nullptr && aligned(r.object, kv::element_bytes(l.dtype)) && r.object_stride >= 0 &&
+           r.plane_stride >= 0 && r.layer_stride >= 0 && r.token_stride >= 0 && r.head_stride >= 0;
+}
+
+using Kernel = void (*)(const kv::Args);
+
+template <int FMT, class T>
+Kernel warp_kernel(bool quantise)
+{
+    return quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>;
+}
+
+template <int FMT>
+Kernel kernel_for(int dtype, bool quantise)
+{
+    return dtype == kv::kBf16   ? warp_kernel<FMT, __nv_bfloat16>(quantise)
+           : dtype == kv::kFp16 ? warp_kernel<FMT, __half>(quantise)
+                                : warp_kernel<FMT, float>(quantise);
+}
+
+int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, const lmcache_gpu_kv_run* runs,
+           size_t count, int device, void* stream_ptr, bool quantise)
+{
+    if (!layout_ok(layout) || device < 0 || (runs == nullptr && count != 0)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    const lmcache_gpu_kv_layout& l = *layout;
+    if (pages != nullptr && !pages_ok(l, *pages)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    for (size_t i = 0; i < count; ++i) {
+        if (!run_ok(l, pages, runs[i])) {
+            return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+        }
+    }
+    if (count == 0) {
+        return LMCACHE_GPU_AESGCM_OK;
+    }
+    DeviceGuard guard(device);
+    if (!guard.ok()) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_ptr);
+    const int64_t element = kv::element_bytes(l.dtype);
+
+    kv::Args a;
+    a.by_layers = kv::make_fast_div(l.layers);
+    a.by_heads = kv::make_fast_div(l.heads);
+    a.by_block = kv::make_fast_div(pages != nullptr ? pages->block_size : 1);
+    a.head_dim = l.head_dim;
+    a.layers = l.layers;
+    a.paged = pages != nullptr ? 1 : 0;
+    a.slots = 0;
+    a.block_stride = a.row_stride = a.page_head_stride = 0;
+    if (pages != nullptr) {
+        a.slots = static_cast<uint32_t>(pages->blocks * pages->block_size);
+        a.block_stride = pages->block_stride * element;
+        a.row_stride = pages->row_stride * element;
+        a.page_head_stride = pages->head_stride * element;
+        std::memcpy(a.bases, pages->bases, sizeof(void*) * l.planes * l.layers);
+    }
+    const Kernel kernel = l.format == kv::kInt8  ? kernel_for<kv::kInt8>(l.dtype, quantise)
+                          : l.format == kv::kFp8 ? kernel_for<kv::kFp8>(l.dtype, quantise)
+                                                 : kernel_for<kv::kMxFp4>(l.dtype, quantise);
+    a.runs = 0;
+    uint64_t tiles = 0;
+    auto flush = [&]() -> cudaError_t {
+        if (a.runs == 0) {
+            return cudaSuccess;
+        }
+        const cudaError_t e = launch_pdl(kernel, static_cast<uint32_t>(tiles), kv::kThreads, 0, s, a);
+        a.runs = 0;
+        tiles = 0;
+        return e;
+    };
+    for (size_t i = 0; i < count; ++i) {
+        const lmcache_gpu_kv_run& r = runs[i];
+        const uint64_t vectors = object_vectors(l, r.tokens);
+        const kv::RecordLayout rec = kv::record_layout(l.format, l.head_dim, vectors);
+        const uint32_t units = vectors == 0 ? 1 : static_cast<uint32_t>(vectors);
+        // as many objects at once as FastDiv can tell apart
+        const uint32_t most = kv::kMaxVectors / units;
+        for (uint32_t first = 0; first < r.count;) {
+            const uint32_t n = r.count - first < most ? r.count - first : most;
+            const uint64_t more = (uint64_t{n} * units + kv::kWarps - 1) / kv::kWarps;
+            if (a.runs == kv::kMaxRuns || (a.runs != 0 && tiles + more > kMaxTiles)) {
+                if (flush() != cudaSuccess) {
+                    return LMCACHE_GPU_AESGCM_ERR_CUDA;
+                }
+            }
+            kv::Run& d = a.run[a.runs++];
+            d.object = static_cast<char*>(r.object) + first * r.object_stride * element;
+            d.object_stride = r.object_stride * element;
+            d.plane_stride = r.plane_stride * element;
+            d.layer_stride = r.layer_stride * element;
+            d.token_stride = r.token_stride * element;
+            d.head_stride = r.head_stride * element;
+            d.slots = r.slots + first * r.slots_stride;
+            d.slots_stride = r.slots_stride;
+            d.record = static_cast<char*>(r.record) + first * r.record_stride;
+            d.record_stride = r.record_stride;
+            d.ok = r.ok != nullptr ? r.ok + first : nullptr;
+            d.codes_end = rec.codes_end;
+            d.scales_at = rec.scales_at;
+            d.scales_end = rec.scales_end;
+            d.record_bytes = rec.size;
+            d.by_object = kv::make_fast_div(units);
+            d.by_tokens = kv::make_fast_div(r.tokens == 0 ? 1 : r.tokens);
+            d.vectors = n * units;
+            d.empty = vectors == 0 ? 1 : 0;
+            d.tile_start = static_cast<uint32_t>(tiles);
+            d.header[0] = kv::kMagic;
+            d.header[1] = r.tokens;
+            d.header[2] = l.layers | l.heads << 16;
+            d.header[3] = l.head_dim | static_cast<uint32_t>(l.format) << 16 | static_cast<uint32_t>(l.dtype) << 20 |
+                          l.planes << 24;
+            tiles += more;
+            first += n;
+        }
+    }
+    return cuda_rc(flush());
+}
+
+}  // namespace
+
+extern "C" size_t lmcache_gpu_kv_record_size(const lmcache_gpu_kv_layout* layout, uint32_t tokens)
+{
+    if (!layout_ok(layout)) {
+        return 0;
+    }
+    const uint64_t vectors = object_vectors(*layout, tokens);
+    return vectors > kv::kMaxVectors ? 0 : kv::record_layout(layout->format, layout->head_dim, vectors).size;
+}
+
+extern "C" int lmcache_gpu_kv_quantise_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages,
+                                             const lmcache_gpu_kv_run* runs, size_t count, int device, void* stream)
+{
+    return launch(layout, pages, runs, count, device, stream, true);
+}
+
+extern "C" int lmcache_gpu_kv_dequantise_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages,
+                                               const lmcache_gpu_kv_run* runs, size_t count, int device, void* stream)
+{
+    return launch(layout, pages, runs, count, device, stream, false);
+}

@@ -1,0 +1,131 @@
+// The KV codec's arithmetic up to the rounding to a code; the CPU tests compile it too and check it against
+// whole numbers.
+#pragma once
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "kv_layout.h"
+
+namespace confkv {
+namespace kv {
+
+KV_HD uint32_t float_bits(float f)
+{
+#ifdef __CUDA_ARCH__
+    return __float_as_uint(f);
+#else
+    uint32_t u;
+    std::memcpy(&u, &f, 4);
+    return u;
+#endif
+}
+
+KV_HD float bits_float(uint32_t u)
+{
+#ifdef __CUDA_ARCH__
+    return __uint_as_float(u);
+#else
+    float f;
+    std::memcpy(&f, &u, 4);
+    return f;
+#endif
+}
+
+KV_HD float fused(float a, float b, float c) { return fmaf(a, b, c); }
+KV_HD double fused(double a, double b, double c) { return fma(a, b, c); }
+
+constexpr uint32_t kInfinity = 0x7f800000u;
+constexpr uint32_t kNan = 0x7fffffffu;
+
+// The codes of INT8 and FP8 are roundings of the exact quotient top x / A (top = 127 or 448), and the
+// quotient that is computed must not cross a border between two codes. With 2^-E a power of two near
+// 1 / A, t = x (top 2^-E) is exact (11 + 7 bits at most for 16-bit caches; where t underflows the code is 0
+// anyway), b = A 2^-E is exact, and with y = 1 / b rounded, q0 = t y is within 2^-23 of t / b, of its
+// size. The residual t - b q0 is then added back, q = q0 + (t - b q0) y, which leaves one rounding of q and
+// some 2^-46. A quotient that is a border itself has few bits, so the residual and then q are
+// exact, and the tie goes to even. Any other is at least 2^-19 of its size away from every border: t
+// is a whole number T < 2^18 and b a whole number B < 2^11, times powers of two, a border a whole number
+// M < 2^8 times one, and T 2^i and M B (or T and M B 2^i) differ by a whole number. float32 caches (T < 2^31,
+// B < 2^24, so 2^-32) do the same in double.
+template <class F>
+struct Divider {
+    F c, b, y;
+    KV_HD F quotient(float x) const
+    {
+        const F t = static_cast<F>(x) * c;
+        const F q0 = t * y;
+        const F r = fused(-b, q0, t);
+        return fused(r, y, q0);
+    }
+};
+
+// For A = amax, finite. A = 0 gives quotients of 0 for the zeros that it comes from.
+template <class F>
+KV_HD Divider<F> make_divider(float amax, float top)
+{
+    Divider<F> d;
+    if (amax == 0.0f) {
+        d.c = 0;
+        d.b = 1;
+        d.y = 1;
+        return d;
+    }
+    // E is kept where 2^-E and top 2^-E are normal floats (bfloat16's least A, 2^-133, leaves b = 2^-14)
+    int e = static_cast<int>(float_bits(amax) >> 23) - 127;
+    e = e < -119 ? -119 : (e > 126 ? 126 : e);
+    const float p = bits_float(static_cast<uint32_t>(127 - e) << 23);
+    d.c = static_cast<F>(top) * static_cast<F>(p);
+    d.b = static_cast<F>(amax) * static_cast<F>(p);
+    d.y = static_cast<F>(1) / d.b;
+    return d;
+}
+
+template <int FMT>
+constexpr float kTop = FMT == kInt8 ? 127.0f : 448.0f;
+
+// FLT_MAX / 127 and FLT_MAX / 448, rounded down: no code times a scale overflows.
+template <int FMT>
+constexpr float kMostScale = FMT == kInt8 ? 0x1.020406p+121f : 0x1.249248p+119f;
+
+// A vector's scale; one rounding, to float, which the values read back carry as 2^-24 of their size.
+template <int FMT>
+KV_HD float scale_of(float amax)
+{
+    return fminf(amax / kTop<FMT>, kMostScale<FMT>);
+}
+
+// A double as the float towards zero, its last bit set where something was lost: a later rounding to
+// few bits then goes the way that the double itself would.
+KV_HD float round_to_odd(double q)
+{
+#ifdef __CUDA_ARCH__
+    const float f = __double2float_rz(q);
+#else
+    float f = static_cast<float>(q);
+    if (std::fabs(static_cast<double>(f)) > std::fabs(q)) {
+        f = bits_float(float_bits(f) - 1u);
+    }
+#endif
+    return static_cast<double>(f) == q ? f : bits_float(float_bits(f) | 1u);
+}
+
+KV_HD float for_rounding(float q) { return q; }
+KV_HD float for_rounding(double q) { return round_to_odd(q); }
+
+// An MXFP4 block's scale byte e + 127 from the bits of its largest |x|; 255: a value is not finite.
+KV_HD uint32_t mx_scale_byte(uint32_t bits)
+{
+    if (bits >= kInfinity) {
+        return 255u;
+    }
+    const uint32_t biased = bits >> 23;           // floor(log2 A) + 127 of a normal A
+    return biased > 2u ? biased - 2u : 0u;
+}
+
+// 2^-e of a scale byte below 254; x 2^-e is exact, or so small that its code is 0.
+KV_HD float mx_inverse(uint32_t byte) { return bits_float((254u - byte) << 23); }
+
+}  // namespace kv
+}  // namespace confkv

@@ -1,0 +1,300 @@
+"""KV-cache codec: 8- and 4-bit records of KV objects, on the GPU.
+
+Wraps lmcache_gpu_kv_{quantise,dequantise}_async (include/gpu_kv_codec_api.h, which states the
+formats and the record layout; an extension, ConfKV has no counterpart). A record is what is sealed in the
+place of the object, so that frames, host copies and storage shrink to a half (int8, fp8) or a quarter
+(mxfp4) of a 16-bit cache.
+
+    codec = KvCodec(lib, "int8", torch.bfloat16, planes=2, layers=32, heads=8, head_dim=128, device=0)
+    records = torch.empty(n, codec.record_bytes(256), dtype=torch.uint8, device="cuda:0")
+    codec.quantise(objects, records)                  # objects [n, 2, 32, 256, 8, 128]
+    codec.dequantise(records, restored, ok=ok)        # ok: int32 [n], 1 where the record was this codec's
+
+    cache = PagedKvCache(codec, layers)               # one [2, blocks, block_size, 8, 128] tensor a layer
+    codec.quantise_paged(cache, slots, records)       # slots [n, 256] int64: tokens that become n objects
+    codec.dequantise_paged(records, cache, slots, ok=ok)
+
+Every call enqueues on `stream` (default: the device's current one) and returns; as with seal_async the
+caller keeps the buffers alive and synchronises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from .gpu_aesgcm import GpuAesGcmLibrary
+
+FORMATS = ("int8", "fp8", "mxfp4")
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+HEADER_BYTES = 32
+MX_BLOCK = 32
+RECORD_ALIGN = 16
+MAX_BASES = 512
+
+
+class KvLayout(ctypes.Structure):
+    """lmcache_gpu_kv_layout."""
+
+    _fields_ = [("format", ctypes.c_int32), ("dtype", ctypes.c_int32), ("planes", ctypes.c_uint32),
+                ("layers", ctypes.c_uint32), ("heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
+
+
+class KvPages(ctypes.Structure):
+    """lmcache_gpu_kv_pages."""
+
+    _fields_ = [("bases", ctypes.c_void_p), ("blocks", ctypes.c_uint64), ("block_size", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32), ("block_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+# lmcache_gpu_kv_run: object and its five strides, slots and their stride, record, record_stride,
+# record_bytes, ok, tokens, count
+RUN = struct.Struct("<Q5qQqQqQQII")
+
+assert ctypes.sizeof(KvLayout) == 24 and ctypes.sizeof(KvPages) == 48 and RUN.size == 104
+
+CODEC_SYMBOLS = (
+    "lmcache_gpu_kv_record_size",
+    "lmcache_gpu_kv_quantise_async",
+    "lmcache_gpu_kv_dequantise_async",
+)
+
+
+def _declare(lib) -> None:
+    vp = ctypes.c_void_p
+    lib.lmcache_gpu_kv_record_size.argtypes = [vp, ctypes.c_uint32]
+    lib.lmcache_gpu_kv_record_size.restype = ctypes.c_size_t
+    for name in ("lmcache_gpu_kv_quantise_async", "lmcache_gpu_kv_dequantise_async"):
+        fn = getattr(lib, name)
+        fn.argtypes = [vp, vp, ctypes.c_char_p, ctypes.c_size_t, ctypes.c_int, vp]
+        fn.restype = ctypes.c_int
+
+
+def _as_list(x):
+    return [x] if isinstance(x, torch.Tensor) else list(x)
+
+
+def _overlaps(shape, strides) -> bool:
+    """Whether two indices of a tensor may share memory: in the order of the strides, each has to pass
+    over all that the smaller ones reach."""
+    reach = 0
+    for stride, size in sorted((s, n) for n, s in zip(shape, strides) if n > 1):
+        if stride <= reach:
+            return True
+        reach += stride * (size - 1)
+    return False
+
+
+class KvCodec:
+    """A format for the objects of one cache: [planes, layers, tokens, heads, head_dim] of `dtype`."""
+
+    def __init__(self, library: GpuAesGcmLibrary, format: str, dtype: torch.dtype, *, planes: int, layers: int,
+                 heads: int, head_dim: int, device: int | torch.device = 0):
+        if format not in FORMATS:
+            raise ValueError(f"kv codec: format must be one of {', '.join(FORMATS)}")
+        if dtype not in DTYPES:
+            raise ValueError("kv codec: dtype must be bfloat16, float16 or float32")
+        self.library = library
+        self.format, self.dtype = format, dtype
+        self.planes, self.layers, self.heads, self.head_dim = int(planes), int(layers), int(heads), int(head_dim)
+        if not (1 <= self.planes <= 2 and all(1 <= n <= 65535 for n in (self.layers, self.heads, self.head_dim))):
+            raise ValueError("kv codec: planes must be 1 or 2; layers, heads and head_dim 1 to 65535")
+        self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if self.device.type != "cuda" or self.device.index is None:
+            raise ValueError("kv codec: device must be a CUDA device with its index")
+        _declare(library.lib)
+        self._layout = KvLayout(FORMATS.index(format), DTYPES.index(dtype), self.planes, self.layers, self.heads,
+                                self.head_dim)
+        self._layout_ptr = ctypes.addressof(self._layout)
+        self._sizes: dict[int, int] = {}
+
+    # ---- records
+    def record_bytes(self, tokens: int) -> int:
+        """Bytes of the record of an object of `tokens` tokens."""
+        size = self._sizes.get(tokens)
+        if size is None:
+            if not 0 <= tokens < 1 << 32:
+                raise ValueError("kv codec: bad number of tokens")
+            size = int(self.library.lib.lmcache_gpu_kv_record_size(self._layout_ptr, tokens))
+            if size == 0:
+                raise ValueError("kv codec: an object has to have fewer than 2^31 vectors")
+            if len(self._sizes) < 4096:
+                self._sizes[tokens] = size
+        return size
+
+    def split(self, record: torch.Tensor, tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Views of a record's (or of [n, R] records') codes and scales: codes [..., planes, layers, tokens,
+        heads, head_dim] int8 or float8_e4m3fn (mxfp4: uint8, two values a byte), scales [..., planes, layers, tokens,
+        heads] float32 (mxfp4: uint8, one a block of 32 values as their last dimension)."""
+        vectors = self.planes * self.layers * tokens * self.heads
+        mx = self.format == "mxfp4"
+        size = (self.head_dim + 1) // 2 if mx else self.head_dim
+        at = HEADER_BYTES + (vectors * size + 15) // 16 * 16
+        per = -(-self.head_dim // MX_BLOCK)
+        lead, index = record.shape[:-1], (self.planes, self.layers, tokens, self.heads)
+        codes = record[..., HEADER_BYTES:HEADER_BYTES + vectors * size]
+        scales = record[..., at:at + vectors * (per if mx else 4)]
+        if mx:
+            return codes.reshape(*lead, *index, size), scales.reshape(*lead, *index, per)
+        codes = codes.view(torch.int8 if self.format == "int8" else torch.float8_e4m3fn)
+        return codes.view(*lead, *index, size), scales.view(torch.float32).view(*lead, *index)
+
+    # ---- arguments
+    def _run(self, record, tokens, count, object_args, slots_args, ok) -> bytes:
+        size = self.record_bytes(tokens)
+        if record.dtype != torch.uint8 or record.device != self.device:
+            raise ValueError(f"kv codec: records are uint8 tensors on {self.device}")
+        if record.dim() == 1 and count == 1:
+            stride, room = 0, record.shape[0]
+        elif record.dim() == 2 and record.shape[0] == count:
+            stride, room = record.stride(0), record.shape[1]
+        else:
+            raise ValueError("kv codec: one record, or a row of records, for every object")
+        if room < size:
+            raise ValueError(f"kv codec: a record of {tokens} tokens takes {size} bytes")
+        ptr = record.data_ptr()
+        if record.stride(-1) != 1 and room > 1 or ptr % RECORD_ALIGN or count > 1 and (stride % RECORD_ALIGN or stride < size):
+            raise ValueError("kv codec: records are contiguous, at multiples of 16 bytes, and do not overlap")
+        ok_ptr = 0
+        if ok is not None:
+            if ok.dtype != torch.int32 or ok.device != self.device or ok.numel() != count or not ok.is_contiguous():
+                raise ValueError(f"kv codec: ok is an int32 tensor of one value an object on {self.device}")
+            ok_ptr = ok.data_ptr()
+        return RUN.pack(*object_args, *slots_args, ptr, stride, size, ok_ptr, tokens, count)
+
+    def _object_run(self, obj, record, ok, writes) -> bytes:
+        if obj.dtype != self.dtype or obj.device != self.device:
+            raise ValueError(f"kv codec: objects are {self.dtype} tensors on {self.device}")
+        shape, strides = obj.shape, obj.stride()
+        if obj.dim() == 5:
+            count, stride = 1, 0
+        elif obj.dim() == 6:
+            count, stride = shape[0], strides[0]
+        else:
+            raise ValueError("kv codec: objects are [planes, layers, tokens, heads, head_dim], or a row of them")
+        planes, layers, tokens, heads, dim = shape[-5:]
+        if (planes, layers, heads, dim) != (self.planes, self.layers, self.heads, self.head_dim):
+            raise ValueError(f"kv codec: an object of shape {tuple(shape)} is not one of this codec's")
+        if strides[-1] != 1 and dim > 1:
+            raise ValueError("kv codec: the values of a vector have to follow one another")
+        if writes and _overlaps(shape, strides):
+            raise ValueError("kv codec: an object that is written to may not overlap itself")
+        return self._run(record, tokens, count, (obj.data_ptr(), stride, *strides[-5:-1]), (0, 0), ok)
+
+    def _slots_run(self, slots, record, ok) -> bytes:
+        if slots.dtype != torch.int64 or slots.device != self.device:
+            raise ValueError(f"kv codec: slots are int64 tensors on {self.device}")
+        if slots.dim() == 1:
+            count, stride = 1, 0
+        elif slots.dim() == 2:
+            count, stride = slots.shape[0], slots.stride(0)
+        else:
+            raise ValueError("kv codec: slots are [tokens], or a row of them")
+        tokens = slots.shape[-1]
+        if slots.stride(-1) != 1 and tokens > 1:
+            raise ValueError("kv codec: the slots of an object have to follow one another")
+        return self._run(record, tokens, count, (0,) * 6, (slots.data_ptr(), stride), ok)
+
+    def _runs(self, sources, records, ok, make) -> tuple[bytes, int]:
+        sources, records = _as_list(sources), _as_list(records)
+        oks = [None] * len(sources) if ok is None else _as_list(ok)
+        if not len(sources) == len(records) == len(oks):
+            raise ValueError("kv codec: one tensor of records (and of verdicts) for every tensor of objects or slots")
+        return b"".join([make(s, r, k) for s, r, k in zip(sources, records, oks)]), len(sources)
+
+    def _call(self, name, runs, cache, stream) -> None:
+        raw, count = runs
+        if stream is None:
+            handle = torch._C._cuda_getCurrentRawStream(self.device.index)
+        else:
+            if stream.device != self.device:
+                raise ValueError(f"kv codec: the stream is not one of {self.device}")
+            handle = stream.cuda_stream
+        rc = getattr(self.library.lib, name)(self._layout_ptr, cache._pages_ptr if cache is not None else None, raw, count,
+                                             self.device.index, handle)
+        self.library.check(rc, name.removeprefix("lmcache_gpu_").removesuffix("_async"))
+
+    def _cache(self, cache) -> "PagedKvCache":
+        if cache.signature != self.signature:
+            raise ValueError("kv codec: the paged cache is not one of this codec's shape, type or device")
+        return cache
+
+    @property
+    def signature(self):
+        return self.dtype, self.planes, self.layers, self.heads, self.head_dim, self.device
+
+    # ---- calls
+    def quantise(self, objects, records, stream: torch.cuda.Stream | None = None) -> None:
+        """Write the records of objects. `objects`: a [planes, layers, tokens, heads, head_dim] tensor of any
+        strides with contiguous vectors, a row of them [n, ...], or a sequence of either; `records`: for each a uint8
+        tensor [>= R], or [n, >= R]."""
+        self._call("lmcache_gpu_kv_quantise_async",
+                   self._runs(objects, records, None, lambda o, r, k: self._object_run(o, r, k, False)), None, stream)
+
+    def dequantise(self, records, objects, ok=None, stream: torch.cuda.Stream | None = None) -> None:
+        """Read records back into objects. `ok`: for each tensor of objects an int32 tensor of one verdict an object:
+        1, or 0 where the record is not one of this codec's for so many tokens; such an object is zero-filled."""
+        self._call("lmcache_gpu_kv_dequantise_async",
+                   self._runs(objects, records, ok, lambda o, r, k: self._object_run(o, r, k, True)), None, stream)
+
+    def quantise_paged(self, cache: "PagedKvCache", slots, records, stream: torch.cuda.Stream | None = None) -> None:
+        """Write the records of tokens of a paged cache. `slots`: an int64 tensor [tokens] on the device, a row of
+        them [n, tokens], or a sequence of either; a slot below 0 or outside the cache is a token of zeros."""
+        self._call("lmcache_gpu_kv_quantise_async", self._runs(slots, records, None, self._slots_run),
+                   self._cache(cache), stream)
+
+    def dequantise_paged(self, records, cache: "PagedKvCache", slots, ok=None,
+                         stream: torch.cuda.Stream | None = None) -> None:
+        """Read records back into slots of a paged cache, and write to no other slot. Slots below 0 or outside the
+        cache are passed over; the others have to differ from one another."""
+        self._call("lmcache_gpu_kv_dequantise_async", self._runs(slots, records, ok, self._slots_run),
+                   self._cache(cache).writable(), stream)
+
+
+class PagedKvCache:
+    """The layers of a paged cache as a codec's calls take them: for each layer a tensor [planes, blocks, block_size,
+    heads, head_dim] (any strides with contiguous vectors, equal in all layers: pages that hold each head's tokens
+    together are a transposed view), or a (keys, values) pair of [blocks, block_size, heads, head_dim]. Slot s is row
+    s % block_size of block s // block_size. Keeps the tensors alive."""
+
+    def __init__(self, codec: KvCodec, layers):
+        self.signature = codec.signature
+        self.layers = list(layers)
+        if len(self.layers) != codec.layers or codec.layers * codec.planes > MAX_BASES:
+            raise ValueError(f"kv codec: a paged cache has the codec's {codec.layers} layers, and {MAX_BASES} planes at most")
+        planes = [[], []]
+        for layer in self.layers:
+            parts = list(layer.unbind(0)) if isinstance(layer, torch.Tensor) and layer.dim() == 5 else \
+                [layer] if isinstance(layer, torch.Tensor) else list(layer)
+            if len(parts) != codec.planes:
+                raise ValueError(f"kv codec: a layer has {codec.planes} planes")
+            for plane, t in zip(planes, parts):
+                plane.append(t)
+        every = planes[0] + planes[1]
+        first = every[0]
+        if first.dim() != 4:
+            raise ValueError("kv codec: a plane is [blocks, block_size, heads, head_dim]")
+        for t in every:
+            if t.dtype != codec.dtype or t.device != codec.device:
+                raise ValueError(f"kv codec: the layers are {codec.dtype} tensors on {codec.device}")
+            if t.shape != first.shape or t.stride() != first.stride():
+                raise ValueError("kv codec: all planes have the same shape and strides")
+        blocks, size, heads, dim = first.shape
+        if (heads, dim) != (codec.heads, codec.head_dim) or size < 1 or blocks * size >= 1 << 31:
+            raise ValueError(f"kv codec: a plane of shape {tuple(first.shape)} is not one of this codec's")
+        if first.stride(-1) != 1 and dim > 1:
+            raise ValueError("kv codec: the values of a vector have to follow one another")
+        self.blocks, self.block_size = blocks, size
+        self._overlap = _overlaps(first.shape, first.stride())
+        self._bases = (ctypes.c_void_p * len(every))(*[t.data_ptr() for t in every])
+        self._pages = KvPages(ctypes.addressof(self._bases), blocks, size, 0, first.stride(0), first.stride(1),
+                              first.stride(2))
+        self._pages_ptr = ctypes.addressof(self._pages)
+
+    def writable(self) -> "PagedKvCache":
+        if self._overlap:
+            raise ValueError("kv codec: a cache that is written to may not overlap itself")
+        return self
