@@ -77,18 +77,113 @@ bool run_ok(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages* pages, c
 
 using Kernel = void (*)(const kv::Args);
 
-template <int FMT, class T>
-Kernel warp_kernel(bool quantise)
+// How a launch cuts its work: `parts` units a vector; the warp kernels have `groups` vectors a tile, the chunk kernels
+// `groups` units of 2^lg_group lanes, `step` of which a group takes at once.
+struct Plan {
+    Kernel kernel;
+    uint32_t parts, lg_group, groups, step;
+};
+
+uint32_t log2_up(uint32_t n)
 {
-    return quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>;
+    uint32_t l = 0;
+    while ((1u << l) < n) {
+        ++l;
+    }
+    return l;
+}
+
+template <int FMT, class T>
+Plan warp_plan(bool quantise)
+{
+    return Plan{quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>, 1, 5, kv::kWarps, 1};
+}
+
+template <int FMT, class T, bool WIDE>
+Plan chunk_plan(uint32_t head_dim, bool quantise)
+{
+    constexpr int few = sizeof(T) == 4 ? 1 : 2;
+    const uint32_t chunks = (head_dim + kv::kChunk - 1) / kv::kChunk;
+    if (!quantise) {
+        return Plan{kv::dequantise_chunk_kernel<FMT, T, WIDE, 2>, chunks, 0, kv::kThreads, 2};
+    }
+    if constexpr (FMT == kv::kMxFp4) {
+        return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 1, few>, (chunks + 1) / 2, 1, kv::kThreads / 2, few};
+    } else {
+        // one chunk a lane, or three where that leaves fewer lanes idle (96 values: 2 lanes of 3 instead of 8 of which 6 work)
+        const uint32_t one = log2_up(chunks), three = log2_up((chunks + 2) / 3);
+        if (one <= 5 && (1u << one) <= (3u << three)) {
+            return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 1, few>, 1, one, kv::kThreads >> one, few};
+        }
+        return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 3, 1>, 1, three, kv::kThreads >> three, 1};
+    }
+}
+
+template <int FMT, class T>
+Plan plan_of(uint32_t head_dim, uint64_t alignment, bool quantise)
+{
+    // a group has 32 lanes of three chunks at most
+    if (head_dim <= 96 * kv::kChunk) {
+        if (head_dim % 16 == 0 && alignment >= 32) {
+            return chunk_plan<FMT, T, true>(head_dim, quantise);
+        }
+        if (head_dim % 8 == 0 && alignment >= 16) {
+            return chunk_plan<FMT, T, false>(head_dim, quantise);
+        }
+    }
+    return warp_plan<FMT, T>(quantise);
 }
 
 template <int FMT>
-Kernel kernel_for(int dtype, bool quantise)
+Plan plan_of(const lmcache_gpu_kv_layout& l, uint64_t alignment, bool quantise)
 {
-    return dtype == kv::kBf16   ? warp_kernel<FMT, __nv_bfloat16>(quantise)
-           : dtype == kv::kFp16 ? warp_kernel<FMT, __half>(quantise)
-                                : warp_kernel<FMT, float>(quantise);
+    return l.dtype == kv::kBf16   ? plan_of<FMT, __nv_bfloat16>(l.head_dim, alignment, quantise)
+           : l.dtype == kv::kFp16 ? plan_of<FMT, __half>(l.head_dim, alignment, quantise)
+                                  : plan_of<FMT, float>(l.head_dim, alignment, quantise);
+}
+
+Plan plan_of(const lmcache_gpu_kv_layout& l, uint64_t alignment, bool quantise)
+{
+    return l.format == kv::kInt8  ? plan_of<kv::kInt8>(l, alignment, quantise)
+           : l.format == kv::kFp8 ? plan_of<kv::kFp8>(l, alignment, quantise)
+                                  : plan_of<kv::kMxFp4>(l, alignment, quantise);
+}
+
+// The largest power of two up to 32 that divides the addresses of all vectors: `bits` gathers the pointers and
+// the strides in bytes of the dimensions that are longer than one.
+uint64_t alignment_of(uint64_t bits)
+{
+    return bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 1);
+}
+
+// How many steps a group takes: 
+uint32_t steps_of(uint64_t units, const Plan& p, int sms)
+{
+    (void)units; (void)p; (void)sms;
+    return 1;
+}
+
+uint64_t strides_of_pages(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages& p, int64_t element)
+{
+    uint64_t bits = 0;
+    for (uint32_t k = 0; k < l.planes * l.layers; ++k) {
+        bits |= reinterpret_cast<uintptr_t>(p.bases[k]);
+    }
+    bits |= p.blocks > 1 ? p.block_stride * element : 0;
+    bits |= p.block_size > 1 ? p.row_stride * element : 0;
+    bits |= l.heads > 1 ? p.head_stride * element : 0;
+    return bits;
+}
+
+uint64_t strides_of_run(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_run& r, int64_t element)
+{
+    uint64_t bits = reinterpret_cast<uintptr_t>(r.object);
+    bits |= r.count > 1 ? r.object_stride * element : 0;
+    bits |= l.planes > 1 ? r.plane_stride * element : 0;
+    bits |= l.layers > 1 ? r.layer_stride * element : 0;
+    bits |= r.tokens > 1 ? r.token_stride * element : 0;
+    bits |= l.heads > 1 ? r.head_stride * element : 0;
+    return bits;
 }
 
 int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, const lmcache_gpu_kv_run* runs,
@@ -113,6 +208,10 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
     if (!guard.ok()) {
         return LMCACHE_GPU_AESGCM_ERR_CUDA;
     }
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_ptr);
     const int64_t element = kv::element_bytes(l.dtype);
 
@@ -132,16 +231,15 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
         a.page_head_stride = pages->head_stride * element;
         std::memcpy(a.bases, pages->bases, sizeof(void*) * l.planes * l.layers);
     }
-    const Kernel kernel = l.format == kv::kInt8  ? kernel_for<kv::kInt8>(l.dtype, quantise)
-                          : l.format == kv::kFp8 ? kernel_for<kv::kFp8>(l.dtype, quantise)
-                                                 : kernel_for<kv::kMxFp4>(l.dtype, quantise);
-    a.runs = 0;
+    const uint64_t page_bits = pages != nullptr ? strides_of_pages(l, *pages, element) : 0;
+    Plan plan{};
     uint64_t tiles = 0;
+    a.runs = 0;
     auto flush = [&]() -> cudaError_t {
         if (a.runs == 0) {
             return cudaSuccess;
         }
-        const cudaError_t e = launch_pdl(kernel, static_cast<uint32_t>(tiles), kv::kThreads, 0, s, a);
+        const cudaError_t e = launch_pdl(plan.kernel, static_cast<uint32_t>(tiles), kv::kThreads, 0, s, a);
         a.runs = 0;
         tiles = 0;
         return e;
@@ -150,17 +248,29 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
         const lmcache_gpu_kv_run& r = runs[i];
         const uint64_t vectors = object_vectors(l, r.tokens);
         const kv::RecordLayout rec = kv::record_layout(l.format, l.head_dim, vectors);
-        const uint32_t units = vectors == 0 ? 1 : static_cast<uint32_t>(vectors);
+        const uint64_t alignment = alignment_of(pages != nullptr ? page_bits : strides_of_run(l, r, element));
+        Plan mine = plan_of(l, vectors == 0 ? 32 : alignment, quantise);
+        const uint32_t per_object = vectors == 0 ? 1 : static_cast<uint32_t>(vectors);
+        if (uint64_t{per_object} * mine.parts > kv::kMaxVectors) {
+            mine = plan_of(l, 1, quantise);     // the warp kernels number vectors only
+        }
+        const uint32_t units = per_object * mine.parts;
         // as many objects at once as FastDiv can tell apart
         const uint32_t most = kv::kMaxVectors / units;
         for (uint32_t first = 0; first < r.count;) {
             const uint32_t n = r.count - first < most ? r.count - first : most;
-            const uint64_t more = (uint64_t{n} * units + kv::kWarps - 1) / kv::kWarps;
-            if (a.runs == kv::kMaxRuns || (a.runs != 0 && tiles + more > kMaxTiles)) {
+            const uint32_t passes = mine.step * steps_of(uint64_t{n} * units, mine, sms);
+            const uint64_t tile = uint64_t{mine.groups} * passes;
+            const uint64_t more = (uint64_t{n} * units + tile - 1) / tile;
+            if (a.runs == kv::kMaxRuns ||
+                (a.runs != 0 && (tiles + more > kMaxTiles || mine.kernel != plan.kernel))) {
                 if (flush() != cudaSuccess) {
                     return LMCACHE_GPU_AESGCM_ERR_CUDA;
                 }
             }
+            plan = mine;
+            a.by_parts = kv::make_fast_div(mine.parts);
+            a.lg_group = mine.lg_group;
             kv::Run& d = a.run[a.runs++];
             d.object = static_cast<char*>(r.object) + first * r.object_stride * element;
             d.object_stride = r.object_stride * element;
@@ -177,10 +287,11 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
             d.scales_at = rec.scales_at;
             d.scales_end = rec.scales_end;
             d.record_bytes = rec.size;
-            d.by_object = kv::make_fast_div(units);
+            d.by_object = kv::make_fast_div(per_object);
             d.by_tokens = kv::make_fast_div(r.tokens == 0 ? 1 : r.tokens);
-            d.vectors = n * units;
+            d.units = n * units;
             d.empty = vectors == 0 ? 1 : 0;
+            d.passes = passes;
             d.tile_start = static_cast<uint32_t>(tiles);
             d.header[0] = kv::kMagic;
             d.header[1] = r.tokens;
