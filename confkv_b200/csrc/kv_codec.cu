@@ -1,4 +1,5 @@
 // The KV-cache codec's entry points: checks, the kernels' parameters and their launch.
+#include <algorithm>
 #include <cstring>
 
 #include "gpu_kv_codec_api.h"
@@ -77,11 +78,10 @@ bool run_ok(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages* pages, c
 
 using Kernel = void (*)(const kv::Args);
 
-// How a launch cuts its work: `parts` units a vector; the warp kernels have `groups` vectors a tile, the chunk kernels
-// `groups` units of 2^lg_group lanes, `step` of which a group takes at once.
+// How a launch cuts its work: 2^lg_group lanes share a vector.
 struct Plan {
     Kernel kernel;
-    uint32_t parts, lg_group, groups, step;
+    uint32_t lg_group;
 };
 
 uint32_t log2_up(uint32_t n)
@@ -93,45 +93,74 @@ uint32_t log2_up(uint32_t n)
     return l;
 }
 
+// The plan for vectors cut into granules of E values, in groups of at least `least` lanes (2^least): of the R in the
+// list the one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int... R>
+Plan granule_plan(uint32_t head_dim, uint32_t least)
+{
+    const uint32_t granules = (head_dim + E - 1) / E;
+    if (FMT == kv::kMxFp4) {
+        least = std::max(least, log2_up(kv::kMxBlock / E));    // a block has its granules in neighbouring lanes
+    }
+    Plan best{nullptr, 0};
+    uint32_t held = ~0u;
+    (
+        [&] {
+            const uint32_t lg = std::max(log2_up((granules + R - 1) / R), least);
+            if (lg <= 5 && (uint32_t{R} << lg) < held) {
+                held = uint32_t{R} << lg;
+                if constexpr (QUANTISE) {
+                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT>, lg};
+                } else {
+                    best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT>, lg};
+                }
+            }
+        }(),
+        ...);
+    return best;
+}
+
 template <int FMT, class T>
 Plan warp_plan(bool quantise)
 {
-    return Plan{quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>, 1, 5, kv::kWarps, 1};
+    return Plan{quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>, 5};
 }
 
-template <int FMT, class T, bool WIDE>
-Plan chunk_plan(uint32_t head_dim, bool quantise)
+// `alignment`: a power of two that divides all vectors' addresses.
+template <bool QUANTISE, int FMT, class T>
+Plan granule_plan(uint32_t head_dim, uint64_t alignment)
 {
-    constexpr int few = sizeof(T) == 4 ? 1 : 2;
-    const uint32_t chunks = (head_dim + kv::kChunk - 1) / kv::kChunk;
-    if (!quantise) {
-        return Plan{kv::dequantise_chunk_kernel<FMT, T, WIDE, 2>, chunks, 0, kv::kThreads, 2};
+    if (head_dim % 16 == 0 && alignment >= 32) {
+        if constexpr (sizeof(T) == 4) {
+            return granule_plan<QUANTISE, FMT, T, 16, false, 2, 3, 1>(head_dim, 0);
+        } else {
+            return granule_plan<QUANTISE, FMT, T, 16, false, 4, 3, 5, 2, 1>(head_dim, 0);
+        }
+    }
+    if (head_dim % 8 == 0 && alignment >= 8 * sizeof(T)) {
+        if constexpr (QUANTISE) {
+            return granule_plan<QUANTISE, FMT, T, 8, false, 8, 6, 5, 4, 3>(head_dim, 1);
+        } else {
+            return granule_plan<QUANTISE, FMT, T, 8, false, 4, 3>(head_dim, 0);
+        }
+    }
+    if (head_dim % 4 == 0 && alignment >= 4 * sizeof(T)) {
+        return granule_plan<QUANTISE, FMT, T, 4, false, 8, 5, 4>(head_dim, 1);
     }
     if constexpr (FMT == kv::kMxFp4) {
-        return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 1, few>, (chunks + 1) / 2, 1, kv::kThreads / 2, few};
+        return head_dim % 2 == 0 && alignment >= 2 * sizeof(T) ? granule_plan<QUANTISE, FMT, T, 2, false, 4, 8, 16>(head_dim, 0)
+                                                               : granule_plan<QUANTISE, FMT, T, 2, true, 4, 8, 16>(head_dim, 0);
     } else {
-        // one chunk a lane, or three where that leaves fewer lanes idle (96 values: 2 lanes of 3 instead of 8 of which 6 work)
-        const uint32_t one = log2_up(chunks), three = log2_up((chunks + 2) / 3);
-        if (one <= 5 && (1u << one) <= (3u << three)) {
-            return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 1, few>, 1, one, kv::kThreads >> one, few};
-        }
-        return Plan{kv::quantise_chunk_kernel<FMT, T, WIDE, 3, 1>, 1, three, kv::kThreads >> three, 1};
+        return head_dim % 2 == 0 && alignment >= 2 * sizeof(T) ? granule_plan<QUANTISE, FMT, T, 2, false, 8, 10, 14>(head_dim, 2)
+                                                               : granule_plan<QUANTISE, FMT, T, 1, false, 10, 16>(head_dim, 2);
     }
 }
 
 template <int FMT, class T>
 Plan plan_of(uint32_t head_dim, uint64_t alignment, bool quantise)
 {
-    // a group has 32 lanes of three chunks at most
-    if (head_dim <= 96 * kv::kChunk) {
-        if (head_dim % 16 == 0 && alignment >= 32) {
-            return chunk_plan<FMT, T, true>(head_dim, quantise);
-        }
-        if (head_dim % 8 == 0 && alignment >= 16) {
-            return chunk_plan<FMT, T, false>(head_dim, quantise);
-        }
-    }
-    return warp_plan<FMT, T>(quantise);
+    const Plan p = quantise ? granule_plan<true, FMT, T>(head_dim, alignment) : granule_plan<false, FMT, T>(head_dim, alignment);
+    return p.kernel != nullptr ? p : warp_plan<FMT, T>(quantise);
 }
 
 template <int FMT>
@@ -153,14 +182,8 @@ Plan plan_of(const lmcache_gpu_kv_layout& l, uint64_t alignment, bool quantise)
 // the strides in bytes of the dimensions that are longer than one.
 uint64_t alignment_of(uint64_t bits)
 {
-    return bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 1);
-}
-
-// How many steps a group takes: 
-uint32_t steps_of(uint64_t units, const Plan& p, int sms)
-{
-    (void)units; (void)p; (void)sms;
-    return 1;
+    bits |= 32;
+    return bits & (~bits + 1);
 }
 
 uint64_t strides_of_pages(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages& p, int64_t element)
@@ -208,10 +231,6 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
     if (!guard.ok()) {
         return LMCACHE_GPU_AESGCM_ERR_CUDA;
     }
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-        return LMCACHE_GPU_AESGCM_ERR_CUDA;
-    }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream_ptr);
     const int64_t element = kv::element_bytes(l.dtype);
 
@@ -249,18 +268,13 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
         const uint64_t vectors = object_vectors(l, r.tokens);
         const kv::RecordLayout rec = kv::record_layout(l.format, l.head_dim, vectors);
         const uint64_t alignment = alignment_of(pages != nullptr ? page_bits : strides_of_run(l, r, element));
-        Plan mine = plan_of(l, vectors == 0 ? 32 : alignment, quantise);
-        const uint32_t per_object = vectors == 0 ? 1 : static_cast<uint32_t>(vectors);
-        if (uint64_t{per_object} * mine.parts > kv::kMaxVectors) {
-            mine = plan_of(l, 1, quantise);     // the warp kernels number vectors only
-        }
-        const uint32_t units = per_object * mine.parts;
+        const Plan mine = plan_of(l, vectors == 0 ? 32 : alignment, quantise);
+        const uint32_t units = vectors == 0 ? 1 : static_cast<uint32_t>(vectors);
         // as many objects at once as FastDiv can tell apart
         const uint32_t most = kv::kMaxVectors / units;
         for (uint32_t first = 0; first < r.count;) {
             const uint32_t n = r.count - first < most ? r.count - first : most;
-            const uint32_t passes = mine.step * steps_of(uint64_t{n} * units, mine, sms);
-            const uint64_t tile = uint64_t{mine.groups} * passes;
+            const uint64_t tile = kv::kThreads >> mine.lg_group;
             const uint64_t more = (uint64_t{n} * units + tile - 1) / tile;
             if (a.runs == kv::kMaxRuns ||
                 (a.runs != 0 && (tiles + more > kMaxTiles || mine.kernel != plan.kernel))) {
@@ -269,7 +283,6 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
                 }
             }
             plan = mine;
-            a.by_parts = kv::make_fast_div(mine.parts);
             a.lg_group = mine.lg_group;
             kv::Run& d = a.run[a.runs++];
             d.object = static_cast<char*>(r.object) + first * r.object_stride * element;
@@ -287,11 +300,10 @@ int launch(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* page
             d.scales_at = rec.scales_at;
             d.scales_end = rec.scales_end;
             d.record_bytes = rec.size;
-            d.by_object = kv::make_fast_div(per_object);
+            d.by_object = kv::make_fast_div(units);
             d.by_tokens = kv::make_fast_div(r.tokens == 0 ? 1 : r.tokens);
             d.units = n * units;
             d.empty = vectors == 0 ? 1 : 0;
-            d.passes = passes;
             d.tile_start = static_cast<uint32_t>(tiles);
             d.header[0] = kv::kMagic;
             d.header[1] = r.tokens;

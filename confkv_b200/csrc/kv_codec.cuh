@@ -19,7 +19,7 @@ namespace kv {
 
 constexpr uint32_t kMaxRuns = 16;      // runs a launch carries in its parameters
 constexpr uint32_t kMaxBases = 512;    // planes * layers of a paged cache
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 128;
 constexpr uint32_t kWarps = kThreads / 32;
 
 // Equal objects at equal distances, strides in bytes.
@@ -32,19 +32,17 @@ struct Run {
     int64_t record_stride;
     int32_t* ok;
     uint64_t codes_end, scales_at, scales_end, record_bytes;
-    FastDiv by_object, by_tokens;       // vectors an object (1 where it has none), tokens
-    uint32_t units;                     // of all objects: vectors (one where an object has none) times parts
+    FastDiv by_object, by_tokens;       // vectors of an object (1 where it has none), its tokens (or 1)
+    uint32_t units;                     // vectors of all objects, one for an object that has none
     uint32_t empty;                     // objects without vectors
-    uint32_t passes;                    // units that a group of a tile handles one after another (chunk kernels)
     uint32_t tile_start;                // the run's first tile in the grid
     uint32_t header[4];
 };
 
 struct Args {
     FastDiv by_layers, by_heads, by_block;
-    FastDiv by_parts;                   // parts that a vector is handled in (chunk kernels)
     uint32_t runs, head_dim, layers, paged;
-    uint32_t lg_group;                  // log2 of the lanes a unit has (chunk kernels)
+    uint32_t lg_group;                  // log2 of the lanes that share a vector
     uint32_t slots;                     // of the paged cache
     int64_t block_stride, row_stride, page_head_stride;   // bytes
     Run run[kMaxRuns];
@@ -272,16 +270,16 @@ __global__ void __launch_bounds__(kThreads) dequantise_warp_kernel(const __grid_
     }
 }
 
-// ------------------------------------------------------- chunks of 16 values
+// ------------------------------------------------------- granules of E values
 //
-// A lane holds chunks of 16 consecutive values: one 32-byte load of a 16-bit cache (two of float32) and one 16- or
-// 8-byte store of codes. WIDE: every vector starts at a multiple of 32 bytes and has whole chunks;
-// else every vector starts at a multiple of 16 bytes and has whole halves of 8 values.
+// A group of 2^lg_group lanes shares a vector. It is cut into granules of E consecutive values, and lane i of the
+// group holds granules i, i + 2^lg_group, ..., R of them: one load each, of 32 bytes where the layout allows it, and one
+// store of E codes. E divides head_dim, and every granule starts at a multiple of min(32, E * sizeof(T)) bytes, so
+// that a granule is there as a whole or not at all. SPLIT (MXFP4 alone, E = 2): values are loaded one by one and the last
+// granule may lack its second value, for odd head_dim and for vectors at odd addresses.
 
-constexpr uint32_t kChunk = 16;
-
-template <class T>
-constexpr uint32_t kChunkWords = kChunk * sizeof(T) / 4;
+template <class T, int E>
+constexpr int kGranuleWords = (E * sizeof(T) + 3) / 4;
 
 __device__ __forceinline__ void load32(uint32_t* w, const void* p)
 {
@@ -297,62 +295,91 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w)
                  : "memory");
 }
 
-__device__ __forceinline__ void load16(uint32_t* w, const void* p)
+// BYTES bytes, a power of two, at a multiple of min(32, BYTES); the upper half of the one word of 2 bytes is 0.
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(uint32_t* w, const void* p)
 {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-}
-
-__device__ __forceinline__ void store16(void* p, const uint32_t* w)
-{
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// The words of a chunk; `second`: it has its last 8 values (else zeros stand for them).
-template <class T, bool WIDE>
-__device__ __forceinline__ void load_chunk(uint32_t* w, const char* p, bool second)
-{
-    constexpr uint32_t n = kChunkWords<T>;
-    if constexpr (WIDE) {
+    if constexpr (BYTES >= 32) {
 #pragma unroll
-        for (uint32_t i = 0; i < n; i += 8) {
-            load32(w + i, p + 4 * i);
+        for (int i = 0; i < BYTES / 32; ++i) {
+            load32(w + 8 * i, static_cast<const char*>(p) + 32 * i);
+        }
+    } else if constexpr (BYTES == 16) {
+        const uint4 v = *static_cast<const uint4*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    } else if constexpr (BYTES == 8) {
+        const uint2 v = *static_cast<const uint2*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+    } else if constexpr (BYTES == 4) {
+        w[0] = *static_cast<const uint32_t*>(p);
+    } else if constexpr (BYTES == 2) {
+        w[0] = *static_cast<const uint16_t*>(p);
+    } else {
+        w[0] = *static_cast<const uint8_t*>(p);
+    }
+}
+
+template <int BYTES>
+__device__ __forceinline__ void store_bytes(void* p, const uint32_t* w)
+{
+    if constexpr (BYTES >= 32) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 32; ++i) {
+            store32(static_cast<char*>(p) + 32 * i, w + 8 * i);
+        }
+    } else if constexpr (BYTES == 16) {
+        *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if constexpr (BYTES == 8) {
+        *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (BYTES == 4) {
+        *static_cast<uint32_t*>(p) = w[0];
+    } else if constexpr (BYTES == 2) {
+        *static_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+    } else {
+        *static_cast<uint8_t*>(p) = static_cast<uint8_t>(w[0]);
+    }
+}
+
+// The words of a granule; `second`: SPLIT, its second value is there.
+template <class T, int E, bool SPLIT>
+__device__ __forceinline__ void load_granule(uint32_t* w, const T* p, bool second)
+{
+    if constexpr (!SPLIT) {
+        load_bytes<E * sizeof(T)>(w, p);
+    } else if constexpr (sizeof(T) == 4) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        w[1] = second ? *reinterpret_cast<const uint32_t*>(p + 1) : 0u;
+    } else {
+        w[0] = *reinterpret_cast<const uint16_t*>(p);
+        w[0] |= second ? static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p + 1)) << 16 : 0u;
+    }
+}
+
+template <class T, int E, bool SPLIT>
+__device__ __forceinline__ void store_granule(T* p, const uint32_t* w, bool second)
+{
+    if constexpr (!SPLIT) {
+        store_bytes<E * sizeof(T)>(p, w);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint32_t*>(p) = w[0];
+        if (second) {
+            *reinterpret_cast<uint32_t*>(p + 1) = w[1];
         }
     } else {
-#pragma unroll
-        for (uint32_t i = 0; i < n; i += 4) {
-            if (i < n / 2 || second) {
-                load16(w + i, p + 4 * i);
-            }
+        *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+        if (second) {
+            *reinterpret_cast<uint16_t*>(p + 1) = static_cast<uint16_t>(w[0] >> 16);
         }
     }
 }
 
-template <class T, bool WIDE>
-__device__ __forceinline__ void store_chunk(char* p, const uint32_t* w, bool second)
-{
-    constexpr uint32_t n = kChunkWords<T>;
-    if constexpr (WIDE) {
-#pragma unroll
-        for (uint32_t i = 0; i < n; i += 8) {
-            store32(p + 4 * i, w + i);
-        }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < n; i += 4) {
-            if (i < n / 2 || second) {
-                store16(p + 4 * i, w + i);
-            }
-        }
-    }
-}
-
-// Values 2i and 2i + 1 of a chunk.
+// Values 2i and 2i + 1 of a granule's words.
 template <class T>
-__device__ __forceinline__ float2 chunk_pair(const uint32_t* w, uint32_t i)
+__device__ __forceinline__ float2 pair_of(const uint32_t* w, int i)
 {
     if constexpr (std::is_same_v<T, float>) {
         return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
@@ -363,28 +390,31 @@ __device__ __forceinline__ float2 chunk_pair(const uint32_t* w, uint32_t i)
     }
 }
 
-// The largest |x| of a chunk as the bits of T without the sign (their order is the values', infinity and NaN above).
-template <class T>
-__device__ __forceinline__ uint32_t chunk_max(const uint32_t* w)
+// The larger of m and the largest |x| of some words, as the bits of T without the sign, whose order is that of the
+// values with infinity and NaN above all. 16-bit types: one maximum for each half of the word; see halves_max.
+template <class T, int WORDS>
+__device__ __forceinline__ uint32_t max_of(uint32_t m, const uint32_t* w)
 {
-    uint32_t m = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kChunkWords<T>; ++i) {
-        if constexpr (std::is_same_v<T, float>) {
+    for (int i = 0; i < WORDS; ++i) {
+        if constexpr (sizeof(T) == 4) {
             m = max(m, w[i] & 0x7fffffffu);
         } else {
             asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
         }
     }
-    if constexpr (!std::is_same_v<T, float>) {
-        m = max(m & 0xffffu, m >> 16);
-    }
     return m;
 }
 
-// The bits as a float's.
 template <class T>
-__device__ __forceinline__ uint32_t max_as_float_bits(uint32_t m)
+__device__ __forceinline__ uint32_t halves_max(uint32_t m)
+{
+    return sizeof(T) == 4 ? m : max(m & 0xffffu, m >> 16);
+}
+
+// Those bits as a float's.
+template <class T>
+__device__ __forceinline__ uint32_t as_float_bits(uint32_t m)
 {
     if constexpr (std::is_same_v<T, float>) {
         return m;
@@ -403,40 +433,65 @@ __device__ __forceinline__ uint32_t int8_bits(double q)
     return static_cast<uint32_t>(__double2loint(q + 6755399441055744.0));
 }
 
+// The codes of two values, in the low two bytes (of INT8, above them something else).
 template <int FMT, class F>
-__device__ __forceinline__ uint32_t codes4(const Divider<F>& d, float2 a, float2 b)
+__device__ __forceinline__ uint32_t codes2(const Divider<F>& d, float2 v)
 {
-    const F q0 = d.quotient(a.x), q1 = d.quotient(a.y), q2 = d.quotient(b.x), q3 = d.quotient(b.y);
+    const F q0 = d.quotient(v.x), q1 = d.quotient(v.y);
     if constexpr (FMT == kInt8) {
-        const uint32_t lo = __byte_perm(int8_bits(q0), int8_bits(q1), 0x0040);
-        const uint32_t hi = __byte_perm(int8_bits(q2), int8_bits(q3), 0x0040);
-        return __byte_perm(lo, hi, 0x5410);
+        return __byte_perm(int8_bits(q0), int8_bits(q1), 0x0040);
     } else {
-        return e4m3x2(for_rounding(q0), for_rounding(q1)) | e4m3x2(for_rounding(q2), for_rounding(q3)) << 16;
+        return e4m3x2(for_rounding(q0), for_rounding(q1));
     }
 }
 
-// Eight e2m1 codes of x * inverse.
-template <class T>
-__device__ __forceinline__ uint32_t e2m1_codes8(const uint32_t* w, uint32_t pair, float inverse)
+// The E codes of a granule, INT8 and FP8.
+template <int FMT, class T, int E, class F>
+__device__ __forceinline__ void codes_of(uint32_t* c, const uint32_t* w, const Divider<F>& d)
 {
-    float2 v[4];
+    if constexpr (E >= 4) {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        v[i] = chunk_pair<T>(w, pair + i);
-        v[i].x *= inverse;
-        v[i].y *= inverse;
+        for (int i = 0; i < E / 4; ++i) {
+            c[i] = __byte_perm(codes2<FMT>(d, pair_of<T>(w, 2 * i)), codes2<FMT>(d, pair_of<T>(w, 2 * i + 1)), 0x5410);
+        }
+    } else if constexpr (E == 2) {
+        c[0] = codes2<FMT>(d, pair_of<T>(w, 0));
+    } else {
+        float x;
+        if constexpr (sizeof(T) == 4) {
+            x = __uint_as_float(w[0]);
+        } else {
+            x = pair_of<T>(w, 0).x;
+        }
+        const F q = d.quotient(x);
+        if constexpr (FMT == kInt8) {
+            c[0] = int8_bits(q);
+        } else {
+            c[0] = e4m3x2(for_rounding(q), 0.0f);
+        }
     }
-    uint32_t r;
-    asm("{ .reg .b8 a, b, c, d;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-        "mov.b32 %0, {a, b, c, d}; }"
-        : "=r"(r)
-        : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
-    return r;
+}
+
+// The E codes of a granule, MXFP4, of x * inverse.
+template <class T, int E>
+__device__ __forceinline__ void mx_codes_of(uint32_t* c, const uint32_t* w, float inverse)
+{
+#pragma unroll
+    for (int i = 0; i < (E + 7) / 8; ++i) {
+        uint32_t byte[4];
+#pragma unroll
+        for (int k = 0; k < 4 && 8 * i + 2 * k < E; ++k) {
+            const float2 v = pair_of<T>(w, 4 * i + k);
+            byte[k] = e2m1x2(v.x * inverse, v.y * inverse);
+        }
+        if constexpr (E >= 8) {
+            c[i] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040), 0x5410);
+        } else if constexpr (E == 4) {
+            c[i] = __byte_perm(byte[0], byte[1], 0x0040);
+        } else {
+            c[i] = byte[0];
+        }
+    }
 }
 
 // The header and the zero bytes behind codes and scales, by one thread.
@@ -452,128 +507,109 @@ __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record
     }
 }
 
-// A unit is a vector that a group of 2^lg_group lanes holds in R chunks each (INT8, FP8), or a block of 32 values
-// that two lanes hold (MXFP4). U units are loaded before the first is worked on.
-template <int FMT, class T, bool WIDE, int R, int U>
-__global__ void __launch_bounds__(kThreads) quantise_chunk_kernel(const __grid_constant__ Args a)
+template <int FMT, class T, int E, int R, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constant__ Args a)
 {
     using F = std::conditional_t<std::is_same_v<T, float>, double, float>;
-    constexpr uint32_t words = kChunkWords<T>;
+    constexpr int words = kGranuleWords<T, E>;
     dev::pdl_release();
     dev::pdl_wait();
     const Run& r = run_of_tile(a, blockIdx.x);
     const uint32_t lg = a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
     const uint32_t groups = kThreads >> lg;
     const uint32_t d = a.head_dim;
-    uint32_t unit = (blockIdx.x - r.tile_start) * groups * r.passes + (threadIdx.x >> lg);
-    for (uint32_t pass = 0; pass < r.passes; pass += U, unit += U * groups) {
-        uint32_t w[U][R][words];
-        uint32_t in_object[U], part[U], object[U];
+    const uint32_t v = (blockIdx.x - r.tile_start) * groups + (threadIdx.x >> lg);
+    const bool mine = v < r.units;
+    const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
+    const T* src = mine && r.empty == 0 ? reinterpret_cast<const T*>(vector_address(a, r, x)) : nullptr;
+    uint32_t w[R][words];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t id = unit + u * groups;
-            const uint32_t v = FMT == kMxFp4 ? quotient(a.by_parts, id) : id;
-            part[u] = FMT == kMxFp4 ? id - v * a.by_parts.d : 0;
-            const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
-            in_object[u] = x.in_object;
-            object[u] = x.object;
-            const char* src = id < r.units && r.empty == 0 ? vector_address(a, r, x) : nullptr;
+    for (int j = 0; j < R; ++j) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
+        for (int i = 0; i < words; ++i) {
+            w[j][i] = 0;
+        }
+        const uint32_t at = ((j << lg) + lane) * E;
+        if (src != nullptr && at < d) {
+            load_granule<T, E, SPLIT>(w[j], src + at, at + 1 < d);
+        }
+    }
+    char* record = r.record + x.object * r.record_stride;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(record) + kHeaderBytes + uint64_t{x.in_object} * code_bytes(FMT, d);
+    if (mine && x.in_object == 0 && lane == 0) {
+        write_frame_of_record(r, record);
+    }
+    const bool write = mine && r.empty == 0;
+    if constexpr (FMT == kMxFp4) {
+        const uint32_t blocks = scale_bytes(FMT, d);
+        uint8_t* scales = reinterpret_cast<uint8_t*>(record) + r.scales_at + uint64_t{x.in_object} * blocks;
 #pragma unroll
-                for (uint32_t i = 0; i < words; ++i) {
-                    w[u][j][i] = 0;
+        for (int j = 0; j < R; ++j) {
+            if ((static_cast<uint32_t>(j) << lg) * E >= d) {
+                break;                          // of all lanes alike
+            }
+            // a block's granules lie in neighbouring lanes; lg_group is large enough for that
+            uint32_t m = halves_max<T>(max_of<T, words>(0, w[j]));
+#pragma unroll
+            for (uint32_t o = 1; o < kMxBlock / E; o <<= 1) {
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            }
+            const uint32_t byte = mx_scale_byte(as_float_bits<T>(m));
+            const uint32_t keep = byte == 255u ? 0u : ~0u;      // codes 0 beside an infinity or a NaN
+            const float inverse = mx_inverse(byte);
+            const uint32_t at = ((j << lg) + lane) * E;
+            if (write && at < d) {
+                uint32_t c[(E + 7) / 8];
+                mx_codes_of<T, E>(c, w[j], inverse);
+#pragma unroll
+                for (int i = 0; i < (E + 7) / 8; ++i) {
+                    c[i] &= keep;
                 }
-                const uint32_t at = (part[u] * 2 + (j << lg) + lane) * kChunk;
-                if (src != nullptr && at < d) {
-                    load_chunk<T, WIDE>(w[u][j], src + at * sizeof(T), at + kChunk / 2 < d);
+                store_bytes<E / 2>(codes + at / 2, c);
+                if (at % kMxBlock == 0) {
+                    scales[at / kMxBlock] = static_cast<uint8_t>(byte);
                 }
             }
         }
+    } else {
+        uint32_t m = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            uint32_t m = 0;
+        for (int j = 0; j < R; ++j) {
+            m = max_of<T, words>(m, w[j]);
+        }
+        m = halves_max<T>(m);
+        for (uint32_t o = 1; o < 1u << lg; o <<= 1) {
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        if (!write) {
+            return;
+        }
+        const uint32_t bits = as_float_bits<T>(m);
+        const bool finite = bits < kInfinity;
+        const uint32_t keep = finite ? ~0u : 0u;    // codes 0 beside an infinity or a NaN
+        const float amax = finite ? __uint_as_float(bits) : 0.0f;
+        const Divider<F> div = make_divider<F>(amax, kTop<FMT>);
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                m = max(m, chunk_max<T>(w[u][j]));
-            }
-            for (uint32_t o = 1; o < 1u << lg; o <<= 1) {
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            }
-            const uint32_t bits = max_as_float_bits<T>(m);
-            if (bits >= kInfinity) {
+        for (int j = 0; j < R; ++j) {
+            const uint32_t at = ((j << lg) + lane) * E;
+            if (at < d) {
+                uint32_t c[(E + 3) / 4];
+                codes_of<FMT, T, E>(c, w[j], div);
 #pragma unroll
-                for (int j = 0; j < R; ++j) {
-#pragma unroll
-                    for (uint32_t i = 0; i < words; ++i) {
-                        w[u][j][i] = 0;
-                    }
+                for (int i = 0; i < (E + 3) / 4; ++i) {
+                    c[i] &= keep;
                 }
+                store_bytes<E>(codes + at, c);
             }
-            if (unit + u * groups >= r.units) {
-                continue;                       // no shuffles below
-            }
-            char* record = r.record + object[u] * r.record_stride;
-            if (in_object[u] == 0 && part[u] == 0 && lane == 0) {
-                write_frame_of_record(r, record);
-            }
-            if (r.empty != 0) {
-                continue;
-            }
-            char* codes = record + kHeaderBytes + uint64_t{in_object[u]} * code_bytes(FMT, d);
-            if constexpr (FMT == kMxFp4) {
-                const uint32_t byte = mx_scale_byte(bits);
-                const float inverse = byte == 255u ? 0.0f : mx_inverse(byte);
-                const uint32_t at = (part[u] * 2 + lane) * kChunk;
-                const uint32_t lo = e2m1_codes8<T>(w[u][0], 0, inverse), hi = e2m1_codes8<T>(w[u][0], 4, inverse);
-                if (WIDE) {
-                    if (at < d) {
-                        *reinterpret_cast<uint2*>(codes + at / 2) = make_uint2(lo, hi);
-                    }
-                } else {
-                    if (at < d) {
-                        *reinterpret_cast<uint32_t*>(codes + at / 2) = lo;
-                    }
-                    if (at + kChunk / 2 < d) {
-                        *reinterpret_cast<uint32_t*>(codes + at / 2 + 4) = hi;
-                    }
-                }
-                if (lane == 0) {
-                    record[r.scales_at + uint64_t{in_object[u]} * a.by_parts.d + part[u]] = static_cast<char>(byte);
-                }
-            } else {
-                const bool finite = bits < kInfinity;
-                const float amax = finite ? __uint_as_float(bits) : 0.0f;
-                const Divider<F> div = make_divider<F>(amax, kTop<FMT>);
-#pragma unroll
-                for (int j = 0; j < R; ++j) {
-                    const uint32_t at = ((j << lg) + lane) * kChunk;
-                    uint32_t c[4];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        c[i] = codes4<FMT>(div, chunk_pair<T>(w[u][j], 2 * i), chunk_pair<T>(w[u][j], 2 * i + 1));
-                    }
-                    if (at < d) {
-                        if (WIDE) {
-                            store16(codes + at, c);
-                        } else {
-                            *reinterpret_cast<uint2*>(codes + at) = make_uint2(c[0], c[1]);
-                            if (at + kChunk / 2 < d) {
-                                *reinterpret_cast<uint2*>(codes + at + 8) = make_uint2(c[2], c[3]);
-                            }
-                        }
-                    }
-                }
-                if (lane == 0) {
-                    reinterpret_cast<float*>(record + r.scales_at)[in_object[u]] =
-                        finite ? scale_of<FMT>(amax) : bits_float(kNan);
-                }
-            }
+        }
+        if (lane == 0) {
+            reinterpret_cast<float*>(record + r.scales_at)[x.in_object] =
+                finite ? scale_of<FMT>(amax) : bits_float(kNan);
         }
     }
 }
 
-// Four values of the codes in a word (INT8, FP8), before the scale.
+// The values of the codes in a word (INT8, FP8), before the scale.
 template <int FMT>
 __device__ __forceinline__ void values4(float* f, uint32_t word)
 {
@@ -600,8 +636,8 @@ __device__ __forceinline__ void values4(float* f, uint32_t word)
     }
 }
 
-// Eight values of the e2m1 codes in a word.
-__device__ __forceinline__ void e2m1_values8(float* f, uint32_t word)
+// The eight values of the e2m1 codes in a word.
+__device__ __forceinline__ void mx_values8(float* f, uint32_t word)
 {
     uint32_t h[4];
     asm("{ .reg .b8 a, b, c, d;\n\t"
@@ -632,107 +668,85 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     }
 }
 
-// A unit is a chunk; a thread loads the codes of U before it writes the values of the first.
-template <int FMT, class T, bool WIDE, int U>
-__global__ void __launch_bounds__(kThreads) dequantise_chunk_kernel(const __grid_constant__ Args a)
+template <int FMT, class T, int E, int R, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_constant__ Args a)
 {
-    constexpr uint32_t words = kChunkWords<T>;
+    constexpr int words = kGranuleWords<T, E>;
+    constexpr int codes_bytes = FMT == kMxFp4 ? E / 2 : E;
     dev::pdl_release();
     dev::pdl_wait();
     const Run& r = run_of_tile(a, blockIdx.x);
+    const uint32_t lg = a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
+    const uint32_t groups = kThreads >> lg;
     const uint32_t d = a.head_dim;
-    uint32_t unit = (blockIdx.x - r.tile_start) * kThreads * r.passes + threadIdx.x;
-    for (uint32_t pass = 0; pass < r.passes; pass += U, unit += U * kThreads) {
-        uint32_t c[U][4];
-        float scale[U];
-        char* dst[U];
-        bool second[U];
+    const uint32_t v = (blockIdx.x - r.tile_start) * groups + (threadIdx.x >> lg);
+    if (v >= r.units) {
+        return;
+    }
+    const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
+    const char* record = r.record + x.object * r.record_stride;
+    // the codes are loaded whatever the header says, so that no load waits for another
+    const uint8_t* codes =
+        reinterpret_cast<const uint8_t*>(record) + kHeaderBytes + uint64_t{x.in_object} * code_bytes(FMT, d);
+    uint32_t c[R][(codes_bytes + 3) / 4];
+    uint32_t scale[FMT == kMxFp4 ? R : 1];
+    if constexpr (FMT != kMxFp4) {
+        scale[0] = r.empty == 0 ? reinterpret_cast<const uint32_t*>(record + r.scales_at)[x.in_object] : 0u;
+    }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t id = unit + u * kThreads;
-            dst[u] = nullptr;
-            c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0;
-            scale[u] = 0.0f;
-            second[u] = false;
-            if (id >= r.units) {
-                continue;
-            }
-            const uint32_t v = quotient(a.by_parts, id), part = id - v * a.by_parts.d;
-            const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
-            const char* record = r.record + x.object * r.record_stride;
-            const bool good = header_matches(r, record);
-            if (x.in_object == 0 && part == 0 && r.ok != nullptr) {
-                r.ok[x.object] = good ? 1 : 0;
-            }
-            if (r.empty != 0) {
-                continue;
-            }
-            char* at = vector_address(a, r, x);
-            if (at == nullptr) {
-                continue;
-            }
-            dst[u] = at + part * kChunk * sizeof(T);
-            second[u] = part * kChunk + kChunk / 2 < d;
-            if (!good) {
-                continue;                       // codes and scale 0
-            }
-            const char* codes = record + kHeaderBytes + uint64_t{x.in_object} * code_bytes(FMT, d);
+    for (int j = 0; j < R; ++j) {
+        const uint32_t at = ((j << lg) + lane) * E;
+        if (FMT == kMxFp4) {
+            scale[j] = 0;
+        }
+        if (at < d && r.empty == 0) {
+            load_bytes<codes_bytes>(c[j], codes + (FMT == kMxFp4 ? at / 2 : at));
             if constexpr (FMT == kMxFp4) {
-                codes += part * (kChunk / 2);
-                if constexpr (WIDE) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(codes);
-                    c[u][0] = q.x;
-                    c[u][1] = q.y;
-                } else {
-                    c[u][0] = *reinterpret_cast<const uint32_t*>(codes);
-                    c[u][1] = second[u] ? *reinterpret_cast<const uint32_t*>(codes + 4) : 0u;
-                }
-                scale[u] = mx_scale(static_cast<uint8_t>(
-                    record[r.scales_at + uint64_t{x.in_object} * scale_bytes(FMT, d) + part / 2]));
-            } else {
-                codes += part * kChunk;
-                if constexpr (WIDE) {
-                    load16(c[u], codes);
-                } else {
-                    const uint2 lo = *reinterpret_cast<const uint2*>(codes);
-                    c[u][0] = lo.x;
-                    c[u][1] = lo.y;
-                    if (second[u]) {
-                        const uint2 hi = *reinterpret_cast<const uint2*>(codes + 8);
-                        c[u][2] = hi.x;
-                        c[u][3] = hi.y;
-                    }
-                }
-                scale[u] = reinterpret_cast<const float*>(record + r.scales_at)[x.in_object];
+                scale[j] = static_cast<uint8_t>(
+                    record[r.scales_at + uint64_t{x.in_object} * scale_bytes(FMT, d) + at / kMxBlock]);
             }
         }
+    }
+    T* dst = r.empty == 0 ? reinterpret_cast<T*>(vector_address(a, r, x)) : nullptr;
+    const bool good = header_matches(r, record);
+    if (x.in_object == 0 && lane == 0 && r.ok != nullptr) {
+        r.ok[x.object] = good ? 1 : 0;
+    }
+    if (dst == nullptr) {
+        return;
+    }
+    const uint32_t keep = good ? ~0u : 0u;      // a foreign record's codes and scales are 0
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (dst[u] == nullptr) {
-                continue;
-            }
-            float f[kChunk];
+    for (int j = 0; j < R; ++j) {
+        const uint32_t at = ((j << lg) + lane) * E;
+        if (at < d) {
+            const uint32_t bits = scale[FMT == kMxFp4 ? j : 0] & keep;
+            const float s = FMT == kMxFp4 ? mx_scale(bits) : __uint_as_float(bits);
+            float f[E > 8 ? E : 8];
             if constexpr (FMT == kMxFp4) {
-                e2m1_values8(f, c[u][0]);
-                e2m1_values8(f + 8, c[u][1]);
+#pragma unroll
+                for (int i = 0; i < (E + 7) / 8; ++i) {
+                    mx_values8(f + 8 * i, c[j][i] & keep);
+                }
             } else {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    values4<FMT>(f + 4 * i, c[u][i]);
+                for (int i = 0; i < (E + 3) / 4; ++i) {
+                    values4<FMT>(f + 4 * i, c[j][i] & keep);
                 }
             }
             uint32_t w[words];
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk / 2; ++i) {
-                const float lo = f[2 * i] * scale[u], hi = f[2 * i + 1] * scale[u];
-                if constexpr (std::is_same_v<T, float>) {
-                    w[2 * i] = __float_as_uint(lo);
-                    w[2 * i + 1] = __float_as_uint(hi);
-                } else {
-                    w[i] = pack2<T>(lo, hi);
+                for (int i = 0; i < E; ++i) {
+                    w[i] = __float_as_uint(f[i] * s);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < words; ++i) {
+                    w[i] = pack2<T>(f[2 * i] * s, f[2 * i + 1] * s);
                 }
             }
-            store_chunk<T, WIDE>(dst[u], w, second[u]);
+            store_granule<T, E, SPLIT>(dst + at, w, at + 1 < d);
         }
     }
 }

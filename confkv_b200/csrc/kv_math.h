@@ -93,7 +93,12 @@ constexpr float kMostScale = FMT == kInt8 ? 0x1.020406p+121f : 0x1.249248p+119f;
 template <int FMT>
 KV_HD float scale_of(float amax)
 {
-    return fminf(amax / kTop<FMT>, kMostScale<FMT>);
+    if (amax < 0x1p-100f) {
+        return amax / kTop<FMT>;
+    }
+    // amax / top in three steps, rounded as a division is: the residual of the first is exact
+    const float y = 1.0f / kTop<FMT>, q = amax * y;
+    return fminf(fused(fused(-q, kTop<FMT>, amax), y, q), kMostScale<FMT>);
 }
 
 // A double as the float towards zero, its last bit set where something was lost: a later rounding to
