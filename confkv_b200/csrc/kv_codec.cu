@@ -93,24 +93,27 @@ uint32_t log2_up(uint32_t n)
     return l;
 }
 
-// The plan for vectors cut into granules of E values, in groups of at least `least` lanes (2^least): of the R in the
-// list the one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
-template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int... R>
+// The plan for vectors cut into granules of E values, in groups of at least 2^least lanes: of the R in the list the
+// one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int... R>
 Plan granule_plan(uint32_t head_dim, uint32_t least)
 {
     const uint32_t granules = (head_dim + E - 1) / E;
-    if (FMT == kv::kMxFp4) {
-        least = std::max(least, log2_up(kv::kMxBlock / E));    // a block has its granules in neighbouring lanes
+    uint32_t most = 5;
+    if (QUANTISE && FMT == kv::kMxFp4) {
+        // the lanes that share a block
+        least = std::max(least, log2_up(kv::kMxBlock / (E * SPAN)));
+        most = SPAN > 1 ? least : most;
     }
     Plan best{nullptr, 0};
     uint32_t held = ~0u;
     (
         [&] {
             const uint32_t lg = std::max(log2_up((granules + R - 1) / R), least);
-            if (lg <= 5 && (uint32_t{R} << lg) < held) {
+            if (lg <= most && (uint32_t{R} << lg) < held) {
                 held = uint32_t{R} << lg;
                 if constexpr (QUANTISE) {
-                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT>, lg};
+                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT, SPAN>, lg};
                 } else {
                     best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT>, lg};
                 }
@@ -118,6 +121,25 @@ Plan granule_plan(uint32_t head_dim, uint32_t least)
         }(),
         ...);
     return best;
+}
+
+// MXFP4 in granules of 2: a lane holds several granules of a block where the vector is short enough for it.
+template <bool QUANTISE, class T, bool SPLIT>
+Plan pair_plan(uint32_t head_dim)
+{
+    if constexpr (QUANTISE) {
+        Plan p{nullptr, 0};
+        if constexpr (SPLIT) {
+            p = granule_plan<true, kv::kMxFp4, T, 2, SPLIT, 4, 8, 12, 16, 24>(head_dim, 2);
+        } else {
+            p = granule_plan<true, kv::kMxFp4, T, 2, SPLIT, 4, 8, 12, 16, 24, 32>(head_dim, 2);
+        }
+        return p.kernel != nullptr ? p : granule_plan<true, kv::kMxFp4, T, 2, SPLIT, 1, 8, 16>(head_dim, 0);
+    } else if constexpr (SPLIT) {
+        return granule_plan<false, kv::kMxFp4, T, 2, SPLIT, 1, 4, 8, 16>(head_dim, 3);
+    } else {
+        return granule_plan<false, kv::kMxFp4, T, 2, SPLIT, 1, 8, 10, 14>(head_dim, 2);
+    }
 }
 
 template <int FMT, class T>
@@ -131,28 +153,34 @@ template <bool QUANTISE, int FMT, class T>
 Plan granule_plan(uint32_t head_dim, uint64_t alignment)
 {
     if (head_dim % 16 == 0 && alignment >= 32) {
+        constexpr uint32_t least = FMT == kv::kMxFp4 ? 1 : 0;
         if constexpr (sizeof(T) == 4) {
-            return granule_plan<QUANTISE, FMT, T, 16, false, 2, 3, 1>(head_dim, 0);
+            return granule_plan<QUANTISE, FMT, T, 16, false, 1, 2, 3, 1>(head_dim, least);
         } else {
-            return granule_plan<QUANTISE, FMT, T, 16, false, 4, 3, 5, 2, 1>(head_dim, 0);
+            return granule_plan<QUANTISE, FMT, T, 16, false, 1, 4, 3, 5, 2, 1>(head_dim, least);
         }
     }
     if (head_dim % 8 == 0 && alignment >= 8 * sizeof(T)) {
         if constexpr (QUANTISE) {
-            return granule_plan<QUANTISE, FMT, T, 8, false, 8, 6, 5, 4, 3>(head_dim, 1);
+            return granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5, 4, 3>(head_dim, 1);
         } else {
-            return granule_plan<QUANTISE, FMT, T, 8, false, 4, 3>(head_dim, 0);
+            return granule_plan<false, FMT, T, 8, false, 1, 4, 3>(head_dim, 1);
         }
     }
     if (head_dim % 4 == 0 && alignment >= 4 * sizeof(T)) {
-        return granule_plan<QUANTISE, FMT, T, 4, false, 8, 5, 4>(head_dim, 1);
+        if constexpr (QUANTISE && FMT == kv::kMxFp4) {
+            const Plan p = granule_plan<true, FMT, T, 4, false, 2, 4, 8, 16>(head_dim, 2);
+            return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 4, false, 1, 8, 16>(head_dim, 0);
+        } else {
+            return granule_plan<QUANTISE, FMT, T, 4, false, 1, 8, 5, 4>(head_dim, 1);
+        }
     }
+    const bool even = head_dim % 2 == 0 && alignment >= 2 * sizeof(T);
     if constexpr (FMT == kv::kMxFp4) {
-        return head_dim % 2 == 0 && alignment >= 2 * sizeof(T) ? granule_plan<QUANTISE, FMT, T, 2, false, 4, 8, 16>(head_dim, 0)
-                                                               : granule_plan<QUANTISE, FMT, T, 2, true, 4, 8, 16>(head_dim, 0);
+        return even ? pair_plan<QUANTISE, T, false>(head_dim) : pair_plan<QUANTISE, T, true>(head_dim);
     } else {
-        return head_dim % 2 == 0 && alignment >= 2 * sizeof(T) ? granule_plan<QUANTISE, FMT, T, 2, false, 8, 10, 14>(head_dim, 2)
-                                                               : granule_plan<QUANTISE, FMT, T, 1, false, 10, 16>(head_dim, 2);
+        return even ? granule_plan<QUANTISE, FMT, T, 2, false, 1, 8, 10, 14>(head_dim, 2)
+                    : granule_plan<QUANTISE, FMT, T, 1, false, 1, 10, 16>(head_dim, 2);
     }
 }
 

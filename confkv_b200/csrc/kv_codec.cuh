@@ -507,7 +507,9 @@ __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record
     }
 }
 
-template <int FMT, class T, int E, int R, bool SPLIT>
+// MXFP4: a block's granules are in neighbouring lanes, SPAN in each. SPAN = 1: the group has at least 32 / E lanes;
+// else it has 32 / (E * SPAN).
+template <int FMT, class T, int E, int R, bool SPLIT, int SPAN>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constant__ Args a)
 {
     using F = std::conditional_t<std::is_same_v<T, float>, double, float>;
@@ -544,30 +546,37 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constan
         const uint32_t blocks = scale_bytes(FMT, d);
         uint8_t* scales = reinterpret_cast<uint8_t*>(record) + r.scales_at + uint64_t{x.in_object} * blocks;
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if ((static_cast<uint32_t>(j) << lg) * E >= d) {
+        for (int first = 0; first < R; first += SPAN) {
+            if ((static_cast<uint32_t>(first) << lg) * E >= d) {
                 break;                          // of all lanes alike
             }
-            // a block's granules lie in neighbouring lanes; lg_group is large enough for that
-            uint32_t m = halves_max<T>(max_of<T, words>(0, w[j]));
+            uint32_t m = 0;
 #pragma unroll
-            for (uint32_t o = 1; o < kMxBlock / E; o <<= 1) {
+            for (int j = first; j < first + SPAN; ++j) {
+                m = max_of<T, words>(m, w[j]);
+            }
+            m = halves_max<T>(m);
+#pragma unroll
+            for (uint32_t o = 1; o < kMxBlock / (E * SPAN); o <<= 1) {
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             }
             const uint32_t byte = mx_scale_byte(as_float_bits<T>(m));
             const uint32_t keep = byte == 255u ? 0u : ~0u;      // codes 0 beside an infinity or a NaN
             const float inverse = mx_inverse(byte);
-            const uint32_t at = ((j << lg) + lane) * E;
-            if (write && at < d) {
-                uint32_t c[(E + 7) / 8];
-                mx_codes_of<T, E>(c, w[j], inverse);
 #pragma unroll
-                for (int i = 0; i < (E + 7) / 8; ++i) {
-                    c[i] &= keep;
-                }
-                store_bytes<E / 2>(codes + at / 2, c);
-                if (at % kMxBlock == 0) {
-                    scales[at / kMxBlock] = static_cast<uint8_t>(byte);
+            for (int j = first; j < first + SPAN; ++j) {
+                const uint32_t at = ((j << lg) + lane) * E;
+                if (write && at < d) {
+                    uint32_t c[(E + 7) / 8];
+                    mx_codes_of<T, E>(c, w[j], inverse);
+#pragma unroll
+                    for (int i = 0; i < (E + 7) / 8; ++i) {
+                        c[i] &= keep;
+                    }
+                    store_bytes<E / 2>(codes + at / 2, c);
+                    if (at % kMxBlock == 0) {
+                        scales[at / kMxBlock] = static_cast<uint8_t>(byte);
+                    }
                 }
             }
         }
