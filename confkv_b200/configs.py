@@ -18,6 +18,10 @@ reference C-ABI), per_object_graph (the same calls captured once into a CUDA
 graph and replayed; objects up to 64 KiB in the sweep) and batched (one
 seal_batch_async / open_batch_async per rank).
 
+--kv-format int8|fp8|mxfp4 (kv_small, kv_llama8b, tp8) seals each object's
+record (kv_codec) in the place of its bytes: quantise -> seal, and open ->
+dequantise. GB/s then counts the objects' bytes.
+
 One process per GPU, each with its own key handle and stream; no data crosses
 GPUs. Every timed iteration starts after a barrier and runs INNER back-to-back
 calls; each rank times its own work with CUDA events on its stream and the
@@ -40,6 +44,7 @@ from . import hostmem, multigpu, workloads
 from .batch import DeviceBatch
 from .clocks import ClockSampler
 from .gpu_aesgcm import GpuAes128GcmKey, GpuAesGcmLibrary
+from .kv_codec import FORMATS, KvCodec
 
 ALIGN = 256
 INNER = 4  # calls per timed iteration
@@ -183,6 +188,53 @@ class RankWork:
         return all(torch.equal(self.out[a:a + n], self.plain[a:a + n]) for a, n in zip(self.pt_off, self.lens))
 
 
+class QuantisedWork(RankWork):
+    """This rank's KV objects [n, planes, layers, tokens, heads, head_dim] sealed as records: one quantise call
+    ahead of the seals, one dequantise call behind the opens."""
+
+    def __init__(self, lib, key, objects: torch.Tensor, fmt: str, stream, ivs):
+        n, planes, layers, tokens, heads, head_dim = objects.shape
+        self.codec = KvCodec(lib, fmt, objects.dtype, planes=planes, layers=layers, heads=heads, head_dim=head_dim,
+                             device=objects.device)
+        self.objects, self.restored = objects, torch.zeros_like(objects)
+        self.ok = torch.zeros(n, dtype=torch.int32, device=objects.device)
+        size = self.codec.record_bytes(tokens)
+        self.records = torch.zeros((n, size), dtype=torch.uint8, device=objects.device)
+        super().__init__(lib, key, [size] * n, self.records.view(-1), [k * size for k in range(n)], stream, ivs)
+        self.opened = self.out[:n * size].view(n, size)
+
+    @property
+    def nbytes(self) -> int:
+        return self.objects.numel() * self.objects.element_size()
+
+    def seal_each(self):
+        self.codec.quantise(self.objects, self.records, stream=self.stream)
+        super().seal_each()
+
+    def seal_batched(self):
+        self.codec.quantise(self.objects, self.records, stream=self.stream)
+        super().seal_batched()
+
+    def open_each(self):
+        super().open_each()
+        self.codec.dequantise(self.opened, self.restored, ok=self.ok, stream=self.stream)
+
+    def open_batched(self):
+        super().open_batched()
+        self.codec.dequantise(self.opened, self.restored, ok=self.ok, stream=self.stream)
+
+    def reset_outputs(self):
+        super().reset_outputs()
+        self.restored.zero_()
+        self.ok.zero_()
+
+    def round_trip_ok(self) -> bool:
+        """The opened records are the sealed ones, and what was read back is what they stand for."""
+        again = torch.empty_like(self.restored)
+        self.codec.dequantise(self.records, again)
+        return super().round_trip_ok() and bool((self.ok == 1).all()) and torch.equal(again, self.restored)
+
+
 def barrier(world, dev):
     if world > 1:
         torch.distributed.barrier()
@@ -290,11 +342,14 @@ def main():
     ap.add_argument("--config", required=True, choices=["kv_small", "kv_llama8b", "ragged", "tp8", "sweep"])
     ap.add_argument("--api", default="both", choices=["both", "all", "per_object", "per_object_graph", "batched"],
                     help="both = per_object + batched; all adds per-object calls replayed from a CUDA graph")
+    ap.add_argument("--kv-format", choices=FORMATS, help="seal the objects' records (kv_small, kv_llama8b, tp8)")
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--iters", type=int, default=30)
     ap.add_argument("--min-log2", type=int, default=12)
     ap.add_argument("--max-log2", type=int, default=30)
     args = ap.parse_args()
+    if args.kv_format and args.config not in ("kv_small", "kv_llama8b", "tp8"):
+        ap.error("--kv-format takes the configurations of KV objects: kv_small, kv_llama8b, tp8")
     rank, world, local = multigpu.rank_env()
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
@@ -327,9 +382,16 @@ def main():
                 mine = multigpu.round_robin(64, rank, world)       # 64 objects over the GPUs
             else:
                 mine = list(range(32 if args.config == "kv_llama8b" else 64))   # per GPU
-            plain, offs, lens = bf16_plain(shape, len(mine), seed=50 + rank, dev=dev)
-            run(lens, plain, offs, {"object_shape": list(shape), "objects_per_gpu": len(mine),
-                                    "objects_all_gpus": len(mine) * world if args.config != "kv_small" else 64})
+            extra = {"object_shape": list(shape), "objects_per_gpu": len(mine),
+                     "objects_all_gpus": len(mine) * world if args.config != "kv_small" else 64}
+            if args.kv_format:
+                objects = workloads.bf16_batch(shape, len(mine), seed=50 + rank, device=dev)
+                work = QuantisedWork(lib, key, objects, args.kv_format, stream, workloads.make_ivs(1000 + rank, len(mine)))
+                emit({**extra, "kv_format": args.kv_format, "record_bytes": work.lens[0] if work.lens else 0},
+                     measure(work, apis, args.warmup, args.iters, world, dev))
+            else:
+                plain, offs, lens = bf16_plain(shape, len(mine), seed=50 + rank, dev=dev)
+                run(lens, plain, offs, extra)
         elif args.config == "ragged":
             case = workloads.ragged_case(4096, seed=3)
             mine = multigpu.round_robin(len(case.lengths), rank, world)

@@ -63,7 +63,17 @@ CODEC_SYMBOLS = (
 )
 
 
+def record_size(format: str, head_dim: int, vectors: int) -> int:
+    """Bytes of a record of `vectors` vectors: lmcache_gpu_kv_record_size without the library."""
+    mx = format == "mxfp4"
+    codes = vectors * ((head_dim + 1) // 2 if mx else head_dim)
+    scales = vectors * (-(-head_dim // MX_BLOCK) if mx else 4)
+    return HEADER_BYTES + -(-codes // 16) * 16 + -(-scales // 16) * 16
+
+
 def _declare(lib) -> None:
+    if getattr(lib, "_kv_codec_declared", False):
+        return
     vp = ctypes.c_void_p
     lib.lmcache_gpu_kv_record_size.argtypes = [vp, ctypes.c_uint32]
     lib.lmcache_gpu_kv_record_size.restype = ctypes.c_size_t
@@ -71,6 +81,7 @@ def _declare(lib) -> None:
         fn = getattr(lib, name)
         fn.argtypes = [vp, vp, ctypes.c_char_p, ctypes.c_size_t, ctypes.c_int, vp]
         fn.restype = ctypes.c_int
+    lib._kv_codec_declared = True
 
 
 def _as_list(x):
@@ -110,6 +121,10 @@ class KvCodec:
                                 self.head_dim)
         self._layout_ptr = ctypes.addressof(self._layout)
         self._sizes: dict[int, int] = {}
+        self._quantise = library.lib.lmcache_gpu_kv_quantise_async
+        self._dequantise = library.lib.lmcache_gpu_kv_dequantise_async
+        self._shape = (self.planes, self.layers, self.heads, self.head_dim)
+        self.signature = (self.dtype, *self._shape, self.device)
 
     # ---- records
     def record_bytes(self, tokens: int) -> int:
@@ -144,19 +159,20 @@ class KvCodec:
 
     # ---- arguments
     def _run(self, record, tokens, count, object_args, slots_args, ok) -> bytes:
-        size = self.record_bytes(tokens)
+        size = self._sizes.get(tokens) or self.record_bytes(tokens)
         if record.dtype != torch.uint8 or record.device != self.device:
             raise ValueError(f"kv codec: records are uint8 tensors on {self.device}")
-        if record.dim() == 1 and count == 1:
-            stride, room = 0, record.shape[0]
-        elif record.dim() == 2 and record.shape[0] == count:
-            stride, room = record.stride(0), record.shape[1]
+        shape, strides = record.shape, record.stride()
+        if len(shape) == 1 and count == 1:
+            stride, room = 0, shape[0]
+        elif len(shape) == 2 and shape[0] == count:
+            stride, room = strides[0], shape[1]
         else:
             raise ValueError("kv codec: one record, or a row of records, for every object")
         if room < size:
             raise ValueError(f"kv codec: a record of {tokens} tokens takes {size} bytes")
         ptr = record.data_ptr()
-        if record.stride(-1) != 1 and room > 1 or ptr % RECORD_ALIGN or count > 1 and (stride % RECORD_ALIGN or stride < size):
+        if strides[-1] != 1 or ptr % RECORD_ALIGN or count > 1 and (stride % RECORD_ALIGN or stride < size):
             raise ValueError("kv codec: records are contiguous, at multiples of 16 bytes, and do not overlap")
         ok_ptr = 0
         if ok is not None:
@@ -165,24 +181,27 @@ class KvCodec:
             ok_ptr = ok.data_ptr()
         return RUN.pack(*object_args, *slots_args, ptr, stride, size, ok_ptr, tokens, count)
 
-    def _object_run(self, obj, record, ok, writes) -> bytes:
+    def _read_run(self, obj, record, ok) -> bytes:
         if obj.dtype != self.dtype or obj.device != self.device:
             raise ValueError(f"kv codec: objects are {self.dtype} tensors on {self.device}")
         shape, strides = obj.shape, obj.stride()
-        if obj.dim() == 5:
+        if len(shape) == 5:
             count, stride = 1, 0
-        elif obj.dim() == 6:
+        elif len(shape) == 6:
             count, stride = shape[0], strides[0]
         else:
             raise ValueError("kv codec: objects are [planes, layers, tokens, heads, head_dim], or a row of them")
         planes, layers, tokens, heads, dim = shape[-5:]
-        if (planes, layers, heads, dim) != (self.planes, self.layers, self.heads, self.head_dim):
+        if (planes, layers, heads, dim) != self._shape:
             raise ValueError(f"kv codec: an object of shape {tuple(shape)} is not one of this codec's")
         if strides[-1] != 1 and dim > 1:
             raise ValueError("kv codec: the values of a vector have to follow one another")
-        if writes and _overlaps(shape, strides):
-            raise ValueError("kv codec: an object that is written to may not overlap itself")
         return self._run(record, tokens, count, (obj.data_ptr(), stride, *strides[-5:-1]), (0, 0), ok)
+
+    def _written_run(self, obj, record, ok) -> bytes:
+        if not obj.is_contiguous() and _overlaps(obj.shape, obj.stride()):
+            raise ValueError("kv codec: an object that is written to may not overlap itself")
+        return self._read_run(obj, record, ok)
 
     def _slots_run(self, slots, record, ok) -> bytes:
         if slots.dtype != torch.int64 or slots.device != self.device:
@@ -198,60 +217,53 @@ class KvCodec:
             raise ValueError("kv codec: the slots of an object have to follow one another")
         return self._run(record, tokens, count, (0,) * 6, (slots.data_ptr(), stride), ok)
 
-    def _runs(self, sources, records, ok, make) -> tuple[bytes, int]:
-        sources, records = _as_list(sources), _as_list(records)
-        oks = [None] * len(sources) if ok is None else _as_list(ok)
-        if not len(sources) == len(records) == len(oks):
+    def _call(self, fn, make, sources, records, ok, cache, stream) -> None:
+        if isinstance(sources, torch.Tensor):
+            sources, records = (sources,), _as_list(records)
+            ok = ok if ok is None else _as_list(ok)
+        if len(sources) != len(records) or ok is not None and len(ok) != len(sources):
             raise ValueError("kv codec: one tensor of records (and of verdicts) for every tensor of objects or slots")
-        return b"".join([make(s, r, k) for s, r, k in zip(sources, records, oks)]), len(sources)
-
-    def _call(self, name, runs, cache, stream) -> None:
-        raw, count = runs
+        if ok is None:
+            raw = b"".join([make(s, r, None) for s, r in zip(sources, records)])
+        else:
+            raw = b"".join([make(s, r, k) for s, r, k in zip(sources, records, ok)])
         if stream is None:
             handle = torch._C._cuda_getCurrentRawStream(self.device.index)
         else:
             if stream.device != self.device:
                 raise ValueError(f"kv codec: the stream is not one of {self.device}")
             handle = stream.cuda_stream
-        rc = getattr(self.library.lib, name)(self._layout_ptr, cache._pages_ptr if cache is not None else None, raw, count,
-                                             self.device.index, handle)
-        self.library.check(rc, name.removeprefix("lmcache_gpu_").removesuffix("_async"))
+        rc = fn(self._layout_ptr, cache, raw, len(sources), self.device.index, handle)
+        if rc != 0:
+            self.library.check(rc, fn.__name__.removeprefix("lmcache_gpu_").removesuffix("_async"))
 
     def _cache(self, cache) -> "PagedKvCache":
         if cache.signature != self.signature:
             raise ValueError("kv codec: the paged cache is not one of this codec's shape, type or device")
         return cache
 
-    @property
-    def signature(self):
-        return self.dtype, self.planes, self.layers, self.heads, self.head_dim, self.device
-
     # ---- calls
     def quantise(self, objects, records, stream: torch.cuda.Stream | None = None) -> None:
         """Write the records of objects. `objects`: a [planes, layers, tokens, heads, head_dim] tensor of any
         strides with contiguous vectors, a row of them [n, ...], or a sequence of either; `records`: for each a uint8
         tensor [>= R], or [n, >= R]."""
-        self._call("lmcache_gpu_kv_quantise_async",
-                   self._runs(objects, records, None, lambda o, r, k: self._object_run(o, r, k, False)), None, stream)
+        self._call(self._quantise, self._read_run, objects, records, None, None, stream)
 
     def dequantise(self, records, objects, ok=None, stream: torch.cuda.Stream | None = None) -> None:
         """Read records back into objects. `ok`: for each tensor of objects an int32 tensor of one verdict an object:
         1, or 0 where the record is not one of this codec's for so many tokens; such an object is zero-filled."""
-        self._call("lmcache_gpu_kv_dequantise_async",
-                   self._runs(objects, records, ok, lambda o, r, k: self._object_run(o, r, k, True)), None, stream)
+        self._call(self._dequantise, self._written_run, objects, records, ok, None, stream)
 
     def quantise_paged(self, cache: "PagedKvCache", slots, records, stream: torch.cuda.Stream | None = None) -> None:
         """Write the records of tokens of a paged cache. `slots`: an int64 tensor [tokens] on the device, a row of
         them [n, tokens], or a sequence of either; a slot below 0 or outside the cache is a token of zeros."""
-        self._call("lmcache_gpu_kv_quantise_async", self._runs(slots, records, None, self._slots_run),
-                   self._cache(cache), stream)
+        self._call(self._quantise, self._slots_run, slots, records, None, self._cache(cache)._pages_ptr, stream)
 
     def dequantise_paged(self, records, cache: "PagedKvCache", slots, ok=None,
                          stream: torch.cuda.Stream | None = None) -> None:
         """Read records back into slots of a paged cache, and write to no other slot. Slots below 0 or outside the
         cache are passed over; the others have to differ from one another."""
-        self._call("lmcache_gpu_kv_dequantise_async", self._runs(slots, records, ok, self._slots_run),
-                   self._cache(cache).writable(), stream)
+        self._call(self._dequantise, self._slots_run, slots, records, ok, self._cache(cache).writable()._pages_ptr, stream)
 
 
 class PagedKvCache:

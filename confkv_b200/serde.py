@@ -19,6 +19,12 @@ Objects are duck-typed like LMCache's MemoryObj: `.tensor` (a contiguous
 torch tensor on a CUDA device or on the host) if present, else `.byte_array`
 (a host buffer). Registered as serde type "gpu_aesgcm"; ConfKV's
 LMCACHE_AESGCM_BACKEND switch selects it with the value "gpu".
+
+With `kv_format` ("int8", "fp8" or "mxfp4") what is sealed is the object's
+record (kv_codec: codes and scales, a half to a quarter of a 16-bit cache) in
+the place of its bytes: quantise -> seal, and open -> dequantise. Objects then
+need a `.tensor` of bfloat16, float16 or float32 whose vectors are its last
+dimension, or `kv_head_dim` values where that dimension holds several heads.
 """
 
 from __future__ import annotations
@@ -36,6 +42,7 @@ from lmcache.v1.distributed.serde.factory import register_serde_factory
 from lmcache.v1.distributed.serde.key_provider import HkdfKeyProvider
 
 from .gpu_aesgcm import FRAME_OVERHEAD, GpuAes128GcmKey, GpuAesGcmLibrary
+from .kv_codec import DTYPES, FORMATS, KvCodec, record_size
 
 HKDF_INFO_PREFIX = b"lmcache-l2-aesgcm-v1"
 SERDE_TYPE = "gpu_aesgcm"
@@ -72,8 +79,16 @@ class GpuSerdeContext:
     """State shared by a serializer/deserializer pair: the device, one key
     handle per data-encryption key, and one CUDA stream per worker thread."""
 
-    def __init__(self, key_provider, device: int | None = None, library: GpuAesGcmLibrary | None = None):
+    def __init__(self, key_provider, device: int | None = None, library: GpuAesGcmLibrary | None = None,
+                 kv_format: str | None = None, kv_head_dim: int | None = None):
+        if kv_format is not None and kv_format not in FORMATS:
+            raise ValueError(f"gpu aesgcm: kv_format must be one of {', '.join(FORMATS)}")
+        if kv_head_dim is not None and not 1 <= kv_head_dim <= 65535:
+            raise ValueError("gpu aesgcm: kv_head_dim must be 1 to 65535")
         self.keys = key_provider
+        self.kv_format = kv_format
+        self._kv_head_dim = kv_head_dim
+        self._codecs: dict[tuple, KvCodec] = {}
         self._device = device
         self._library = library
         self._handles: dict[bytes, GpuAes128GcmKey] = {}
@@ -129,6 +144,90 @@ class GpuSerdeContext:
                 h.close()
             self._handles.clear()
 
+    # ---- records in the place of the objects' bytes (kv_format)
+    def vectors(self, shape, dtype) -> tuple[int, int]:
+        """(vectors, head_dim) of an object of this shape and type."""
+        if dtype not in DTYPES:
+            raise ValueError("gpu aesgcm: kv_format needs bfloat16, float16 or float32 objects")
+        numel = 1
+        for n in shape:
+            numel *= int(n)
+        d = self._kv_head_dim or (int(shape[-1]) if len(shape) else 0)
+        if d < 1 or d > 65535 or numel % d or len(shape) and int(shape[-1]) % d:
+            raise ValueError(f"gpu aesgcm: an object of shape {tuple(shape)} is not made of vectors of {d} values")
+        return numel // d, d
+
+    def plaintext_bytes(self, obj) -> int:
+        """Bytes that are sealed for an object: its own, or its record's."""
+        if self.kv_format is None:
+            return _bytes_view(obj).numel()
+        t = _kv_tensor(obj)
+        vectors, d = self.vectors(t.shape, t.dtype)
+        return record_size(self.kv_format, d, vectors)
+
+    def codec(self, t) -> tuple[KvCodec, tuple]:
+        """The codec for an object's tensor, and the shape in which it sees it: one row of vectors."""
+        vectors, d = self.vectors(t.shape, t.dtype)
+        with self._lock:
+            c = self._codecs.get((t.dtype, d))
+            if c is None:
+                if self._library is None:
+                    self._library = GpuAesGcmLibrary()
+                c = KvCodec(self._library, self.kv_format, t.dtype, planes=1, layers=1, heads=1, head_dim=d,
+                            device=self.device)
+                self._codecs[(t.dtype, d)] = c
+        return c, (1, 1, vectors, 1, d)
+
+    def quantise(self, objs, stream) -> list:
+        """Device records of objects, written on `stream` (the current one), with one call a codec."""
+        import torch
+
+        dev = torch.device("cuda", self.device)
+        records, calls = [], defaultdict(lambda: ([], []))
+        for obj in objs:
+            t = _kv_tensor(obj)
+            codec, shape = self.codec(t)
+            record = torch.empty(codec.record_bytes(shape[2]), dtype=torch.uint8, device=dev)
+            sources, into = calls[codec]
+            sources.append(t.to(dev, non_blocking=True).view(shape))
+            into.append(record)
+            records.append(record)
+        for codec, (sources, into) in calls.items():
+            codec.quantise(sources, into, stream=stream)
+        return records
+
+    def dequantise(self, records, objs, stream):
+        """Read device records back into objects on `stream` (the current one); the verdicts as a device tensor."""
+        import torch
+
+        dev = torch.device("cuda", self.device)
+        ok = torch.zeros(len(objs), dtype=torch.int32, device=dev)
+        calls, copies = defaultdict(lambda: ([], [], [])), []
+        for k, (record, obj) in enumerate(zip(records, objs)):
+            t = _kv_tensor(obj)
+            codec, shape = self.codec(t)
+            out = t if t.is_cuda else torch.empty(t.shape, dtype=t.dtype, device=dev)
+            if not t.is_cuda:
+                copies.append((t, out))
+            sources, into, oks = calls[codec]
+            sources.append(record)
+            into.append(out.view(shape))
+            oks.append(ok[k:k + 1])
+        for codec, (sources, into, oks) in calls.items():
+            codec.dequantise(sources, into, ok=oks, stream=stream)
+        for t, out in copies:
+            t.copy_(out, non_blocking=True)
+        return ok
+
+
+def _kv_tensor(obj):
+    t = getattr(obj, "tensor", None)
+    if t is None:
+        raise ValueError("gpu aesgcm: kv_format needs objects with a tensor")
+    if not t.is_contiguous():
+        raise ValueError("gpu aesgcm: tensor must be contiguous")
+    return t
+
 
 class GpuAesGcmSerializer(Serializer):
     def __init__(self, ctx: GpuSerdeContext):
@@ -138,8 +237,8 @@ class GpuAesGcmSerializer(Serializer):
         import torch
 
         ctx = self._ctx
-        src_t, dst_t = _bytes_view(src), _bytes_view(dst)
-        plaintext_len = src_t.numel()
+        dst_t = _bytes_view(dst)
+        plaintext_len = ctx.plaintext_bytes(src)
         frame_len = plaintext_len + FRAME_OVERHEAD
         if dst_t.numel() < frame_len:
             raise ValueError("gpu aesgcm: destination too small")
@@ -148,12 +247,10 @@ class GpuAesGcmSerializer(Serializer):
         stream = ctx.stream()
         dev = torch.device("cuda", ctx.device)
         with torch.cuda.stream(stream):
-            if plaintext_len == 0:
-                src_d = torch.empty(1, dtype=torch.uint8, device=dev)
-            elif src_t.is_cuda:
-                src_d = src_t
+            if ctx.kv_format is not None:
+                src_d, = ctx.quantise([src], stream)
             else:
-                src_d = src_t.to(dev, non_blocking=True)
+                src_d = _device_view(_bytes_view(src), dev, plaintext_len)
             frame_d = dst_t if dst_t.is_cuda else torch.empty(frame_len, dtype=torch.uint8, device=dev)
             gkey.seal_async(src_ptr=src_d.data_ptr(), plaintext_len=plaintext_len, dst_ptr=frame_d.data_ptr(),
                             dst_capacity=frame_d.numel(), iv=iv, stream_ptr=stream.cuda_stream)
@@ -163,6 +260,12 @@ class GpuAesGcmSerializer(Serializer):
         return frame_len
 
     def estimate_serialized_size(self, layout_desc) -> int:
+        ctx = self._ctx
+        if ctx.kv_format is not None:
+            if len(layout_desc.shapes) != 1 or len(layout_desc.dtypes) != 1:
+                raise ValueError("gpu aesgcm: kv_format takes objects of one tensor")
+            vectors, d = ctx.vectors(layout_desc.shapes[0], layout_desc.dtypes[0])
+            return record_size(ctx.kv_format, d, vectors) + FRAME_OVERHEAD
         return _plaintext_bytes(layout_desc) + FRAME_OVERHEAD
 
 
@@ -175,27 +278,32 @@ class GpuAesGcmDeserializer(Deserializer):
 
         ctx = self._ctx
         src_t, dst_t = _bytes_view(src), _bytes_view(dst)
-        plaintext_len = dst_t.numel()
+        plaintext_len = ctx.plaintext_bytes(dst)
         frame_len = plaintext_len + FRAME_OVERHEAD
         if src_t.numel() < frame_len:
             raise ValueError("gpu aesgcm: malformed frame")
+        direct = ctx.kv_format is None and dst_t.is_cuda and plaintext_len
         gkey = ctx.handle(ctx.keys.get_key(key.cache_salt))
         stream = ctx.stream()
         dev = torch.device("cuda", ctx.device)
         with torch.cuda.stream(stream):
             frame_d = src_t if src_t.is_cuda else src_t[:frame_len].to(dev, non_blocking=True)
-            out_d = dst_t if dst_t.is_cuda and plaintext_len else torch.empty(max(plaintext_len, 1),
-                                                                               dtype=torch.uint8, device=dev)
+            out_d = dst_t if direct else torch.empty(max(plaintext_len, 1), dtype=torch.uint8, device=dev)
             auth = torch.zeros(1, dtype=torch.int32, device=dev)
             gkey.open_async(src_ptr=frame_d.data_ptr(), frame_len=frame_len, dst_ptr=out_d.data_ptr(),
                             plaintext_len=plaintext_len, auth_ok_ptr=auth.data_ptr(), stream_ptr=stream.cuda_stream)
-            if plaintext_len and not dst_t.is_cuda:
+            if ctx.kv_format is not None:
+                # a rejected frame leaves a zeroed record, which reads back as zeros
+                ok_h = ctx.dequantise([out_d], [dst], stream).to("cpu", non_blocking=True)
+            elif plaintext_len and not dst_t.is_cuda:
                 dst_t.copy_(out_d[:plaintext_len], non_blocking=True)
             auth_h = auth.to("cpu", non_blocking=True)
         stream.synchronize()
         if int(auth_h.item()) != 1:
-            # the kernel zero-filled the plaintext destination
+            # the kernels zero-filled the plaintext destination
             raise InvalidTag("gpu aesgcm authentication failed")
+        if ctx.kv_format is not None and int(ok_h.item()) != 1:
+            raise ValueError(f"gpu aesgcm: the frame does not hold a {ctx.kv_format} record of this object")
 
 
 def _device_view(t, dev, n: int):
@@ -256,13 +364,14 @@ class GpuAesGcmSerdeProcessor(AsyncSerdeProcessor):
             handle = ctx.handle(dek)
             keep, copies, entries = [], [], []
             with torch.cuda.stream(stream):
-                for i in idx:
-                    src_t, dst_t = _bytes_view(srcs[i]), _bytes_view(dsts[i])
-                    P = src_t.numel()
+                sizes = [ctx.plaintext_bytes(srcs[i]) for i in idx]
+                if any(_bytes_view(dsts[i]).numel() < P + FRAME_OVERHEAD for i, P in zip(idx, sizes)):
+                    raise ValueError("gpu aesgcm: destination too small")
+                records = ctx.quantise([srcs[i] for i in idx], stream) if ctx.kv_format is not None else None
+                for j, (i, P) in enumerate(zip(idx, sizes)):
+                    dst_t = _bytes_view(dsts[i])
                     F = P + FRAME_OVERHEAD
-                    if dst_t.numel() < F:
-                        raise ValueError("gpu aesgcm: destination too small")
-                    src_d = _device_view(src_t, dev, P)
+                    src_d = records[j] if records is not None else _device_view(_bytes_view(srcs[i]), dev, P)
                     frame_d = dst_t if dst_t.is_cuda else torch.empty(F, dtype=torch.uint8, device=dev)
                     entries.append((src_d.data_ptr(), frame_d.data_ptr(), P, frame_d.numel(), os.urandom(12)))
                     keep += [src_d, frame_d]
@@ -284,26 +393,31 @@ class GpuAesGcmSerdeProcessor(AsyncSerdeProcessor):
         ctx = self._ctx
         dev = torch.device("cuda", ctx.device)
         stream = ctx.stream()
-        failed = False
+        failed = foreign = False
         for dek, idx in self._groups(keys).items():
             handle = ctx.handle(dek)
-            keep, copies, entries = [], [], []
+            keep, copies, entries, records = [], [], [], []
             with torch.cuda.stream(stream):
                 auth = torch.zeros(len(idx), dtype=torch.int32, device=dev)
                 for j, i in enumerate(idx):
                     src_t, dst_t = _bytes_view(srcs[i]), _bytes_view(dsts[i])
-                    P = dst_t.numel()
+                    P = ctx.plaintext_bytes(dsts[i])
                     F = P + FRAME_OVERHEAD
                     if src_t.numel() < F:
                         raise ValueError("gpu aesgcm: malformed frame")
                     frame_d = _device_view(src_t, dev, F)
-                    out_d = dst_t if dst_t.is_cuda and P else torch.empty(max(P, 1), dtype=torch.uint8, device=dev)
+                    direct = ctx.kv_format is None and dst_t.is_cuda and P
+                    out_d = dst_t if direct else torch.empty(max(P, 1), dtype=torch.uint8, device=dev)
+                    records.append(out_d)
                     entries.append((frame_d.data_ptr(), out_d.data_ptr(), P, F, auth.data_ptr() + 4 * j))
                     keep += [frame_d, out_d]
-                    if P and not dst_t.is_cuda:
+                    if ctx.kv_format is None and P and not dst_t.is_cuda:
                         copies.append((dst_t, out_d, P))
                 batch = ctx.batch(len(entries))
                 batch.open(handle, entries, stream)
+                ok_h = None
+                if ctx.kv_format is not None:
+                    ok_h = ctx.dequantise(records, [dsts[i] for i in idx], stream).to("cpu", non_blocking=True)
                 for dst_t, out_d, P in copies:
                     dst_t.copy_(out_d[:P], non_blocking=True)
                 auth_h = auth.to("cpu", non_blocking=True)
@@ -312,9 +426,12 @@ class GpuAesGcmSerdeProcessor(AsyncSerdeProcessor):
             if bool(status.any()):
                 raise ValueError("gpu aesgcm: an object descriptor was rejected")
             failed = failed or bool((auth_h != 1).any())
+            foreign = foreign or ok_h is not None and bool((ok_h != 1).any())
         if failed:
             # the kernels zero-filled every rejected object's plaintext
             raise InvalidTag("gpu aesgcm authentication failed")
+        if foreign:
+            raise ValueError(f"gpu aesgcm: a frame does not hold a {ctx.kv_format} record of its object")
         return True
 
     # ---- SerdeProcessor interface
@@ -346,7 +463,9 @@ class GpuAesGcmSerdeProcessor(AsyncSerdeProcessor):
 
 def create_gpu_aesgcm_serde(kwargs: dict) -> GpuAesGcmSerdeProcessor:
     """Factory with the kwargs of native_aesgcm_serde.py:236-292 plus
-    `device` (CUDA ordinal; default the current device)."""
+    `device` (CUDA ordinal; default the current device), `kv_format` (seal
+    int8, fp8 or mxfp4 records; default the objects' own bytes) and
+    `kv_head_dim` (values of a vector; default the objects' last dimension)."""
     if int(kwargs.get("aes_bits", 128)) != 128:
         raise ValueError("gpu aesgcm supports aes_bits=128 only")
     master_key_path = str(kwargs.get("master_key_path", ""))
@@ -356,7 +475,9 @@ def create_gpu_aesgcm_serde(kwargs: dict) -> GpuAesGcmSerdeProcessor:
         master_key = f.read()
     provider = HkdfKeyProvider(master_key, key_len=16, info_prefix=HKDF_INFO_PREFIX)
     device = kwargs.get("device")
-    ctx = GpuSerdeContext(provider, device=None if device is None else int(device))
+    kv_format, kv_head_dim = kwargs.get("kv_format"), kwargs.get("kv_head_dim")
+    ctx = GpuSerdeContext(provider, device=None if device is None else int(device), kv_format=kv_format or None,
+                          kv_head_dim=None if kv_head_dim is None else int(kv_head_dim))
     return GpuAesGcmSerdeProcessor(ctx, max_workers=int(kwargs.get("max_workers", 1)))
 
 
