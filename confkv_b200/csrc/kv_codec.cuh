@@ -377,9 +377,49 @@ __device__ __forceinline__ void store_granule(T* p, const uint32_t* w, bool seco
     }
 }
 
+// Two floats in a register pair and the instructions that take both at once, each rounded as its scalar form is.
+struct Pair {
+    uint64_t v;
+};
+
+__device__ __forceinline__ Pair make_pair(float lo, float hi)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+
+__device__ __forceinline__ float2 halves(Pair p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+
+__device__ __forceinline__ Pair mul(Pair a, Pair b)
+{
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+
+__device__ __forceinline__ Pair add(Pair a, Pair b)
+{
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+
+__device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c)
+{
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+
 // Values 2i and 2i + 1 of a granule's words.
 template <class T>
-__device__ __forceinline__ float2 pair_of(const uint32_t* w, int i)
+__device__ __forceinline__ float2 floats_of(const uint32_t* w, int i)
 {
     if constexpr (std::is_same_v<T, float>) {
         return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
@@ -388,6 +428,13 @@ __device__ __forceinline__ float2 pair_of(const uint32_t* w, int i)
     } else {
         return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
+}
+
+template <class T>
+__device__ __forceinline__ Pair pair_of(const uint32_t* w, int i)
+{
+    const float2 f = floats_of<T>(w, i);
+    return make_pair(f.x, f.y);
 }
 
 // The larger of m and the largest |x| of some words, as the bits of T without the sign, whose order is that of the
@@ -425,72 +472,106 @@ __device__ __forceinline__ uint32_t as_float_bits(uint32_t m)
     }
 }
 
-// q rounded to a whole number, ties to even, in the low byte of the result: adding 1.5 2^23 (2^52) leaves no
-// bit below 1.
-__device__ __forceinline__ uint32_t int8_bits(float q) { return __float_as_uint(q + 12582912.0f); }
-__device__ __forceinline__ uint32_t int8_bits(double q)
-{
-    return static_cast<uint32_t>(__double2loint(q + 6755399441055744.0));
-}
+// The rules by which a granule's codes come from its values; a rule gives the codes of two values in the low two bytes
+// (above them something else).
 
-// The codes of two values, in the low two bytes (of INT8, above them something else).
-template <int FMT, class F>
-__device__ __forceinline__ uint32_t codes2(const Divider<F>& d, float2 v)
-{
-    const F q0 = d.quotient(v.x), q1 = d.quotient(v.y);
-    if constexpr (FMT == kInt8) {
-        return __byte_perm(int8_bits(q0), int8_bits(q1), 0x0040);
-    } else {
-        return e4m3x2(for_rounding(q0), for_rounding(q1));
+// INT8 of 16-bit caches: one product and one rounding (int8_factor).
+struct Int8ByFactor {
+    Pair k, whole;
+    __device__ __forceinline__ explicit Int8ByFactor(float factor)
+        : k(make_pair(factor, factor)), whole(make_pair(kWhole, kWhole))
+    {
     }
-}
+    __device__ __forceinline__ uint32_t codes(float2 x) const
+    {
+        const float2 f = halves(fused(make_pair(x.x, x.y), k, whole));
+        return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x0040);
+    }
+};
+
+// The exact quotient, rounded to a whole number by adding 1.5 2^23 (2^52) or to e4m3.
+template <int FMT>
+struct ByQuotient {
+    Pair c, nb, y;
+    __device__ __forceinline__ explicit ByQuotient(const Divider<float>& d)
+        : c(make_pair(d.c, d.c)), nb(make_pair(-d.b, -d.b)), y(make_pair(d.y, d.y))
+    {
+    }
+    __device__ __forceinline__ uint32_t codes(float2 x) const
+    {
+        const Pair t = mul(make_pair(x.x, x.y), c);
+        const Pair q0 = mul(t, y);
+        const Pair q = fused(fused(nb, q0, t), y, q0);
+        if constexpr (FMT == kInt8) {
+            const float2 f = halves(add(q, make_pair(kWhole, kWhole)));
+            return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x0040);
+        } else {
+            const float2 f = halves(q);
+            return e4m3x2(f.x, f.y);
+        }
+    }
+};
+
+template <int FMT>
+struct ByDoubleQuotient {
+    const Divider<double>& d;
+    __device__ __forceinline__ uint32_t codes(float2 x) const
+    {
+        const double q0 = d.quotient(x.x), q1 = d.quotient(x.y);
+        if constexpr (FMT == kInt8) {
+            constexpr double whole = 6755399441055744.0;
+            return __byte_perm(__double2loint(q0 + whole), __double2loint(q1 + whole), 0x0040);
+        } else {
+            return e4m3x2(round_to_odd(q0), round_to_odd(q1));
+        }
+    }
+};
 
 // The E codes of a granule, INT8 and FP8.
-template <int FMT, class T, int E, class F>
-__device__ __forceinline__ void codes_of(uint32_t* c, const uint32_t* w, const Divider<F>& d)
+template <class T, int E, class Rule>
+__device__ __forceinline__ void codes_of(uint32_t* c, const uint32_t* w, const Rule& rule)
 {
     if constexpr (E >= 4) {
 #pragma unroll
         for (int i = 0; i < E / 4; ++i) {
-            c[i] = __byte_perm(codes2<FMT>(d, pair_of<T>(w, 2 * i)), codes2<FMT>(d, pair_of<T>(w, 2 * i + 1)), 0x5410);
+            c[i] = __byte_perm(rule.codes(floats_of<T>(w, 2 * i)), rule.codes(floats_of<T>(w, 2 * i + 1)), 0x5410);
         }
-    } else if constexpr (E == 2) {
-        c[0] = codes2<FMT>(d, pair_of<T>(w, 0));
+    } else if constexpr (E == 1 && sizeof(T) == 4) {
+        c[0] = rule.codes(make_float2(__uint_as_float(w[0]), 0.0f));
     } else {
-        float x;
-        if constexpr (sizeof(T) == 4) {
-            x = __uint_as_float(w[0]);
-        } else {
-            x = pair_of<T>(w, 0).x;
-        }
-        const F q = d.quotient(x);
-        if constexpr (FMT == kInt8) {
-            c[0] = int8_bits(q);
-        } else {
-            c[0] = e4m3x2(for_rounding(q), 0.0f);
-        }
+        c[0] = rule.codes(floats_of<T>(w, 0));
     }
 }
 
 // The E codes of a granule, MXFP4, of x * inverse.
 template <class T, int E>
-__device__ __forceinline__ void mx_codes_of(uint32_t* c, const uint32_t* w, float inverse)
+__device__ __forceinline__ void mx_codes_of(uint32_t* c, const uint32_t* w, Pair inverse)
 {
+    if constexpr (E >= 8) {
 #pragma unroll
-    for (int i = 0; i < (E + 7) / 8; ++i) {
-        uint32_t byte[4];
+        for (int i = 0; i < E / 8; ++i) {
+            float2 v[4];
 #pragma unroll
-        for (int k = 0; k < 4 && 8 * i + 2 * k < E; ++k) {
-            const float2 v = pair_of<T>(w, 4 * i + k);
-            byte[k] = e2m1x2(v.x * inverse, v.y * inverse);
+            for (int k = 0; k < 4; ++k) {
+                v[k] = halves(mul(pair_of<T>(w, 4 * i + k), inverse));
+            }
+            asm("{ .reg .b8 a, b, c, d;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+                "mov.b32 %0, {a, b, c, d}; }"
+                : "=r"(c[i])
+                : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
         }
-        if constexpr (E >= 8) {
-            c[i] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040), 0x5410);
-        } else if constexpr (E == 4) {
-            c[i] = __byte_perm(byte[0], byte[1], 0x0040);
-        } else {
-            c[i] = byte[0];
+    } else {
+        uint32_t byte[2];
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+            const float2 v = halves(mul(pair_of<T>(w, k), inverse));
+            byte[k] = e2m1x2(v.x, v.y);
         }
+        c[0] = E == 4 ? __byte_perm(byte[0], byte[E / 4], 0x0040) : byte[0];
     }
 }
 
@@ -512,7 +593,6 @@ __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record
 template <int FMT, class T, int E, int R, bool SPLIT, int SPAN>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constant__ Args a)
 {
-    using F = std::conditional_t<std::is_same_v<T, float>, double, float>;
     constexpr int words = kGranuleWords<T, E>;
     dev::pdl_release();
     dev::pdl_wait();
@@ -562,7 +642,8 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constan
             }
             const uint32_t byte = mx_scale_byte(as_float_bits<T>(m));
             const uint32_t keep = byte == 255u ? 0u : ~0u;      // codes 0 beside an infinity or a NaN
-            const float inverse = mx_inverse(byte);
+            const float scale = mx_inverse(byte);
+            const Pair inverse = make_pair(scale, scale);
 #pragma unroll
             for (int j = first; j < first + SPAN; ++j) {
                 const uint32_t at = ((j << lg) + lane) * E;
@@ -597,18 +678,32 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constan
         const bool finite = bits < kInfinity;
         const uint32_t keep = finite ? ~0u : 0u;    // codes 0 beside an infinity or a NaN
         const float amax = finite ? __uint_as_float(bits) : 0.0f;
-        const Divider<F> div = make_divider<F>(amax, kTop<FMT>);
+        const auto write_codes = [&](const auto& rule) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const uint32_t at = ((j << lg) + lane) * E;
-            if (at < d) {
-                uint32_t c[(E + 3) / 4];
-                codes_of<FMT, T, E>(c, w[j], div);
+            for (int j = 0; j < R; ++j) {
+                const uint32_t at = ((j << lg) + lane) * E;
+                if (at < d) {
+                    uint32_t c[(E + 3) / 4];
+                    codes_of<T, E>(c, w[j], rule);
 #pragma unroll
-                for (int i = 0; i < (E + 3) / 4; ++i) {
-                    c[i] &= keep;
+                    for (int i = 0; i < (E + 3) / 4; ++i) {
+                        c[i] &= keep;
+                    }
+                    store_bytes<E>(codes + at, c);
                 }
-                store_bytes<E>(codes + at, c);
+            }
+        };
+        if constexpr (sizeof(T) == 4) {
+            const Divider<double> div = make_divider<double>(amax, kTop<FMT>);
+            write_codes(ByDoubleQuotient<FMT>{div});
+        } else if constexpr (FMT == kFp8) {
+            write_codes(ByQuotient<FMT>(make_divider<float>(amax, kTop<FMT>)));
+        } else {
+            float factor;
+            if (int8_factor<std::is_same_v<T, __half>>(amax, &factor)) {
+                write_codes(Int8ByFactor(factor));
+            } else {
+                write_codes(ByQuotient<FMT>(make_divider<float>(amax, kTop<FMT>)));
             }
         }
         if (lane == 0) {
@@ -618,17 +713,18 @@ __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constan
     }
 }
 
-// The values of the codes in a word (INT8, FP8), before the scale.
+// The values of the codes in a word (INT8, FP8), before the scale, in twos.
 template <int FMT>
-__device__ __forceinline__ void values4(float* f, uint32_t word)
+__device__ __forceinline__ void values4(Pair* f, uint32_t word)
 {
     if constexpr (FMT == kInt8) {
         // 2^23 + 128 + code is a float whose bits are 0x4b0000xx
         const uint32_t u = word ^ 0x80808080u;
-        f[0] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f;
-        f[1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f;
-        f[2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f;
-        f[3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f;
+        const Pair bias = make_pair(-8388736.0f, -8388736.0f);
+        f[0] = add(make_pair(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)),
+                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), bias);
+        f[1] = add(make_pair(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)),
+                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), bias);
     } else {
         uint32_t lo, hi;
         asm("{ .reg .b16 a, b;\n\t"
@@ -637,16 +733,13 @@ __device__ __forceinline__ void values4(float* f, uint32_t word)
             "cvt.rn.f16x2.e4m3x2 %1, b; }"
             : "=r"(lo), "=r"(hi)
             : "r"(word));
-        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-        f[0] = a.x;
-        f[1] = a.y;
-        f[2] = b.x;
-        f[3] = b.y;
+        f[0] = pair_of<__half>(&lo, 0);
+        f[1] = pair_of<__half>(&hi, 0);
     }
 }
 
-// The eight values of the e2m1 codes in a word.
-__device__ __forceinline__ void mx_values8(float* f, uint32_t word)
+// The eight values of the e2m1 codes in a word, in twos.
+__device__ __forceinline__ void mx_values8(Pair* f, uint32_t word)
 {
     uint32_t h[4];
     asm("{ .reg .b8 a, b, c, d;\n\t"
@@ -659,9 +752,7 @@ __device__ __forceinline__ void mx_values8(float* f, uint32_t word)
         : "r"(word));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
+        f[i] = pair_of<__half>(h, i);
     }
 }
 
@@ -730,29 +821,29 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_const
         const uint32_t at = ((j << lg) + lane) * E;
         if (at < d) {
             const uint32_t bits = scale[FMT == kMxFp4 ? j : 0] & keep;
-            const float s = FMT == kMxFp4 ? mx_scale(bits) : __uint_as_float(bits);
-            float f[E > 8 ? E : 8];
+            const float one = FMT == kMxFp4 ? mx_scale(bits) : __uint_as_float(bits);
+            const Pair s = make_pair(one, one);
+            Pair f[E > 8 ? E / 2 : 4];
             if constexpr (FMT == kMxFp4) {
 #pragma unroll
                 for (int i = 0; i < (E + 7) / 8; ++i) {
-                    mx_values8(f + 8 * i, c[j][i] & keep);
+                    mx_values8(f + 4 * i, c[j][i] & keep);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < (E + 3) / 4; ++i) {
-                    values4<FMT>(f + 4 * i, c[j][i] & keep);
+                    values4<FMT>(f + 2 * i, c[j][i] & keep);
                 }
             }
-            uint32_t w[words];
-            if constexpr (sizeof(T) == 4) {
+            uint32_t w[E > 1 ? words : 2];
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    w[i] = __float_as_uint(f[i] * s);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < words; ++i) {
-                    w[i] = pack2<T>(f[2 * i] * s, f[2 * i + 1] * s);
+            for (int i = 0; i < (E + 1) / 2; ++i) {
+                const float2 v = halves(mul(f[i], s));
+                if constexpr (sizeof(T) == 4) {
+                    w[2 * i] = __float_as_uint(v.x);
+                    w[2 * i + 1] = __float_as_uint(v.y);
+                } else {
+                    w[i] = pack2<T>(v.x, v.y);
                 }
             }
             store_granule<T, E, SPLIT>(dst + at, w, at + 1 < d);

@@ -89,6 +89,40 @@ constexpr float kTop = FMT == kInt8 ? 127.0f : 448.0f;
 template <int FMT>
 constexpr float kMostScale = FMT == kInt8 ? 0x1.020406p+121f : 0x1.249248p+119f;
 
+// INT8 of 16-bit caches in one product and one rounding a value: with k = 127 / A rounded up, x k + 1.5 2^23 has
+// the code of x in its low byte, since it is rounded once, to a whole number, ties to even. k is off by 2^-23 of its
+// size at most, and a quotient that is no border is 2^-19 of its size or more away from every one, so that
+// only quotients that are borders matter, 254 x = M A for an odd M < 254. 127 then divides M or the whole
+// number B that A is times a power of two. M = 127 is the border of 63 and 64, which k from above leads to 64, the
+// even one. B = 254, the one multiple of 127 that bfloat16 has, is a power of two times 127: k is
+// exact, and the tie goes to even. Half has other multiples of 127; their vectors take the Divider (false), as do vectors
+// for which 127 / A is too large for a float.
+template <bool HALF>
+KV_HD bool int8_factor(float amax, float* k)
+{
+    const uint32_t bits = float_bits(amax);
+    *k = 0.0f;
+    if (amax == 0.0f) {
+        return true;
+    }
+    if (amax < 0x1p-119f || (HALF && ((bits >> 13 & 0x3ffu) | 0x400u) % 127u == 0)) {
+        return false;
+    }
+    int e = static_cast<int>(bits >> 23) - 127;
+    e = e > 126 ? 126 : e;
+    const float p = bits_float(static_cast<uint32_t>(127 - e) << 23);
+    const float b = amax * p;                       // 1 to 4
+    const float y = 1.0f / b, first = kTop<kInt8> * y;
+    // 127 / b, rounded to nearest: the residual is exact; then up where that is below it
+    const float near = fused(fused(-b, first, kTop<kInt8>), y, first);
+    const float left = fused(-b, near, kTop<kInt8>);
+    *k = bits_float(float_bits(near) + (left > 0.0f ? 1u : 0u)) * p;
+    return true;
+}
+
+// What is added to x k: 1.5 2^23, beside which a float has no bit below 1.
+constexpr float kWhole = 12582912.0f;
+
 // A vector's scale; one rounding, to float, which the values read back carry as 2^-24 of their size.
 template <int FMT>
 KV_HD float scale_of(float amax)

@@ -71,7 +71,46 @@ static uint64_t check_quotients(int format, int bits, int max_gap, int step, int
     return bad;
 }
 
+// The INT8 codes of check_quotients' quotients by int8_factor, both signs, against whole numbers.
+template <bool HALF>
+static uint64_t check_int8(int bits, int max_gap, int exponent, uint64_t* slow)
+{
+    const int64_t lo = int64_t{1} << (bits - 1), hi = int64_t{1} << bits;
+    uint64_t bad = 0;
+    for (int64_t b = lo; b < hi; ++b) {
+        const float amax = std::ldexp(static_cast<float>(b), exponent);
+        float k;
+        if (!kv::int8_factor<HALF>(amax, &k)) {
+            ++*slow;
+            continue;
+        }
+        for (int gap = 0; gap <= max_gap; ++gap) {
+            for (int64_t x = lo; x < hi; ++x) {
+                const float xv = std::ldexp(static_cast<float>(x), exponent - gap);
+                if (xv > amax) {
+                    break;
+                }
+                // 127 x 2^-gap / b rounded to a whole number, ties to even
+                const int64_t num = 127 * x, den = b << gap;
+                int64_t code = num / den;
+                const int64_t twice = 2 * (num - code * den);
+                code += twice > den || (twice == den && (code & 1) != 0) ? 1 : 0;
+                for (int sign = -1; sign <= 1; sign += 2) {
+                    const uint32_t f = kv::float_bits(kv::fused(sign * xv, k, kv::kWhole));
+                    bad += static_cast<int8_t>(f & 0xffu) != sign * code;
+                }
+            }
+        }
+    }
+    return bad;
+}
+
 extern "C" {
+
+uint64_t kv_check_int8(int bits, int max_gap, int exponent, uint64_t* slow)
+{
+    return bits > 8 ? check_int8<true>(bits, max_gap, exponent, slow) : check_int8<false>(bits, max_gap, exponent, slow);
+}
 
 // n / d by FastDiv against the machine's division for `count` values of n; the first that differs, or -1.
 int64_t kv_check_fast_div(uint32_t d, const uint32_t* n, size_t count)

@@ -30,6 +30,8 @@ def lib(tmp_path_factory):
     lib.kv_check_record_size.restype = u64
     lib.kv_check_quotients.argtypes = [i32] * 5
     lib.kv_check_quotients.restype = u64
+    lib.kv_check_int8.argtypes = [i32, i32, i32, ctypes.POINTER(u64)]
+    lib.kv_check_int8.restype = u64
     lib.kv_check_mx_byte.argtypes = [u32]
     lib.kv_check_mx_byte.restype = u32
     lib.kv_check_mx_inverse.argtypes = [u32]
@@ -78,6 +80,19 @@ def test_every_half_quotient_is_on_its_side_of_the_borders(lib, fmt, gap):
 @pytest.mark.parametrize("fmt,gap", [(0, 9), (1, 20)])
 def test_float32_quotients_are_on_their_sides_of_the_borders(lib, fmt, gap):
     assert lib.kv_check_quotients(fmt, 24, gap, 15000, -23) == 0
+
+
+@pytest.mark.parametrize("bits,exponent", [(8, -7), (8, 120), (8, -126), (11, -10), (11, 5), (11, -24)])
+def test_every_int8_code_by_one_product(lib, bits, exponent):
+    """Of every bfloat16 and half vector that does not take the divider: of half those whose A is a multiple of 127."""
+    slow = ctypes.c_uint64()
+    assert lib.kv_check_int8(bits, 9, exponent, ctypes.byref(slow)) == 0
+    assert slow.value == (0 if bits == 8 else 8)
+
+
+def test_int8_vectors_too_small_for_one_product(lib):
+    slow = ctypes.c_uint64()
+    assert lib.kv_check_int8(8, 9, -127, ctypes.byref(slow)) == 0 and slow.value == 128
 
 
 def test_microscale_bytes(lib):
