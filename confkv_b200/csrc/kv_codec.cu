@@ -161,7 +161,10 @@ Plan granule_plan(uint32_t head_dim, uint64_t alignment)
         }
     }
     if (head_dim % 8 == 0 && alignment >= 8 * sizeof(T)) {
-        if constexpr (QUANTISE) {
+        if constexpr (QUANTISE && FMT == kv::kMxFp4) {
+            const Plan p = granule_plan<true, FMT, T, 8, false, 2, 4, 6, 8>(head_dim, 1);
+            return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5, 4, 3>(head_dim, 1);
+        } else if constexpr (QUANTISE) {
             return granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5, 4, 3>(head_dim, 1);
         } else {
             return granule_plan<false, FMT, T, 8, false, 1, 4, 3>(head_dim, 1);

@@ -91,7 +91,9 @@ def round_trip(codec, x, device_view=None):
 
 # head sizes: one value, around a block, a chunk and a warp, odd ones, several chunks a lane, the largest group, beyond it
 HEAD_DIMS = [1, 2, 3, 7, 8, 15, 16, 17, 24, 31, 32, 33, 40, 48, 63, 64, 65, 72, 80, 96, 100, 112, 127, 128, 129, 160, 192, 200, 256,
-             272, 320, 500, 512, 520, 576, 768, 1000, 1024, 1040, 1536, 1552, 2050, 5000]
+             272, 320, 500, 512, 520, 576, 768, 1000, 1024, 1040, 1536, 1552, 2050, 5000,
+             # every number of granules a lane, for granules of 1, 2, 4 and 8 values
+             34, 36, 50, 56, 60, 66, 68, 77, 88, 104, 108, 120, 126, 136, 201, 202, 204, 264, 400, 700, 1200, 1600, 2000, 2560, 2576]
 
 
 @pytest.mark.parametrize("fmt", kv_ref.FORMATS)
@@ -217,6 +219,30 @@ def test_strided_objects(make, fmt, dtype, d):
         assert torch.equal(bits(view), bits(want)), name
         view.copy_(x)
         assert torch.equal(bits(whole), bits(before)), f"{name}: wrote beside the object"
+
+
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+def test_objects_of_unequal_alignment_in_one_call(make, fmt):
+    """Aligned and misaligned objects in turns, each to its own record."""
+    d = 64
+    codec = make(fmt, "bf16", 1, 2, 3, d)
+    xs = [values((1, 2, 20 + k, 3, d), torch.bfloat16, seed=k) for k in range(9)]
+    held, views_, recs, outs = [], [], [], []
+    for k, x in enumerate(xs):
+        for into in (views_, outs):
+            raw = torch.full((x.numel() + 64,), 2.0, dtype=torch.bfloat16, device="cuda")
+            held.append(raw)
+            into.append(raw[(0, 1, 8, 16)[k % 4]:][:x.numel()].view(x.shape))
+        views_[k].copy_(x)
+        recs.append(torch.zeros(codec.record_bytes(20 + k), dtype=torch.uint8, device="cuda"))
+    codec.quantise(views_, recs)
+    codec.dequantise(recs, outs)
+    for x, r, o in zip(xs, recs, outs):
+        assert_record(r, x, fmt)
+        assert torch.equal(bits(o), bits(kv_ref.read(r.cpu().numpy(), fmt, torch.bfloat16, x.shape)))
+    for raw in held:
+        inside = raw.numel() - 64
+        assert int((raw == 2.0).sum()) >= raw.numel() - inside
 
 
 def test_broadcast_source(make):
@@ -415,6 +441,25 @@ def test_offsets_beyond_32_bits(make):
     row.fill_(2)
     codec.dequantise(recs, row)
     assert torch.equal(bits(row[1]), bits(kv_ref.read(recs[1].cpu().numpy(), "int8", torch.bfloat16, (1, 1, 3, heads, d))))
+
+
+def test_more_vectors_than_a_launch_numbers(make):
+    """Three objects of 2^30 vectors each in one row: 2^31 and more vectors are cut into several launches."""
+    tokens, heads = 1 << 20, 1 << 10
+    codec = make("int8", "bf16", 1, 1, heads, 1)
+    source = torch.tensor([2.0, -3.0, 5.0], dtype=torch.bfloat16, device="cuda").view(3, 1, 1, 1, 1, 1)
+    recs = torch.empty(3, codec.record_bytes(tokens), dtype=torch.uint8, device="cuda")
+    codec.quantise(source.expand(3, 1, 1, tokens, heads, 1), recs)
+    codes, scales = codec.split(recs, tokens)
+    for k, (code, amax) in enumerate(((127, 2.0), (-127, 3.0), (127, 5.0))):
+        assert kv_ref.HEADER == 32 and recs[k, :16].cpu().numpy().tobytes() == \
+            kv_ref.header("int8", torch.bfloat16, 1, 1, tokens, heads, 1)[:16].tobytes()
+        assert bool((codes[k] == code).all())
+        assert bool((scales[k] == float(np.float32(amax) / np.float32(127))).all())
+    # read back the last object alone, into every second place of a tensor
+    out = torch.full((1, 1, tokens, heads, 2), 9.0, dtype=torch.bfloat16, device="cuda")
+    codec.dequantise(recs[2], out[..., :1])
+    assert bool((out[..., 0] == 5).all()) and bool((out[..., 1] == 9).all())
 
 
 # ------------------------------------------------------------ streams, graphs, threads
