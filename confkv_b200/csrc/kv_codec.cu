@@ -148,7 +148,17 @@ Plan warp_plan(bool quantise)
     return Plan{quantise ? kv::quantise_warp_kernel<FMT, T> : kv::dequantise_warp_kernel<FMT, T>, 5};
 }
 
-// `alignment`: a power of two that divides all vectors' addresses.
+// The largest granules that divide the vector and its addresses (`alignment`: a power of two that divides them all),
+// and how many a lane holds. More a lane share the vector's address among more values, fewer keep the loads of
+// neighbouring lanes together. Measured with 6 objects [2, 32, 256, 8, d] of bfloat16, us:
+//   INT8 quantise   d = 200 (8): 8 a lane 89, 4 a lane 108; d = 72: 5 a lane 35, 3 a lane 46; d = 56: two lanes 29,
+//                   one lane 33
+//   INT8 dequantise d = 72 (8): 3 a lane 31, 5 a lane 37; d = 200: 4 a lane 75, 8 a lane 81
+//   d = 100 (4):    8 a lane 60 / 50, 4 a lane 79 / 57
+//   d = 66 (2):     10 a lane 56 / 50, 16 a lane 63 / 56;  d = 65 (1): 10 a lane 93 / 85, 16 a lane 121 / 104
+//   MXFP4 quantise  d = 40 (8): two granules of a block in a lane 19, one 29;  d = 100 (4): two 58, one 80;
+//                   d = 66 (2): four 59, one 126
+// Small granules cost instructions: 52 a value at d = 65, where granules of 16 have 7.5, and that bounds them.
 template <bool QUANTISE, int FMT, class T>
 Plan granule_plan(uint32_t head_dim, uint64_t alignment)
 {
@@ -163,7 +173,7 @@ Plan granule_plan(uint32_t head_dim, uint64_t alignment)
     if (head_dim % 8 == 0 && alignment >= 8 * sizeof(T)) {
         if constexpr (QUANTISE && FMT == kv::kMxFp4) {
             const Plan p = granule_plan<true, FMT, T, 8, false, 2, 4, 6, 8>(head_dim, 1);
-            return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5, 4, 3>(head_dim, 1);
+            return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5>(head_dim, 1);
         } else if constexpr (QUANTISE) {
             return granule_plan<true, FMT, T, 8, false, 1, 8, 6, 5, 4, 3>(head_dim, 1);
         } else {
