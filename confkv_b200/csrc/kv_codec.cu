@@ -93,10 +93,10 @@ uint32_t log2_up(uint32_t n)
     return l;
 }
 
-// The plan for vectors cut into granules of E values, in groups of at least 2^least lanes: of the R in the list the
-// one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
-template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int... R>
-Plan granule_plan(uint32_t head_dim, uint32_t least)
+// The plan for vectors cut into granules of E values, in groups of at least 2^least lanes (LG >= 0: of 2^LG): of the R
+// in the list the one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int LG, int... R>
+Plan group_plan(uint32_t head_dim, uint32_t least)
 {
     const uint32_t granules = (head_dim + E - 1) / E;
     uint32_t most = 5;
@@ -104,6 +104,9 @@ Plan granule_plan(uint32_t head_dim, uint32_t least)
         // the lanes that share a block
         least = std::max(least, log2_up(kv::kMxBlock / (E * SPAN)));
         most = SPAN > 1 ? least : most;
+    }
+    if (LG >= 0) {
+        least = most = static_cast<uint32_t>(LG & 31);
     }
     Plan best{nullptr, 0};
     uint32_t held = ~0u;
@@ -113,14 +116,20 @@ Plan granule_plan(uint32_t head_dim, uint32_t least)
             if (lg <= most && (uint32_t{R} << lg) < held) {
                 held = uint32_t{R} << lg;
                 if constexpr (QUANTISE) {
-                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT, SPAN>, lg};
+                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT, SPAN, LG>, lg};
                 } else {
-                    best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT>, lg};
+                    best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT, LG>, lg};
                 }
             }
         }(),
         ...);
     return best;
+}
+
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int... R>
+Plan granule_plan(uint32_t head_dim, uint32_t least)
+{
+    return group_plan<QUANTISE, FMT, T, E, SPLIT, SPAN, -1, R...>(head_dim, least);
 }
 
 // MXFP4 in granules of 2: a lane holds several granules of a block where the vector is short enough for it.
@@ -154,8 +163,10 @@ Plan warp_plan(bool quantise)
 //   INT8 quantise   d = 200 (8): 8 a lane 89, 4 a lane 108; d = 72: 5 a lane 35, 3 a lane 46; d = 56: two lanes 29,
 //                   one lane 33
 //   INT8 dequantise d = 72 (8): 3 a lane 31, 5 a lane 37; d = 200: 4 a lane 75, 8 a lane 81
-//   d = 100 (4):    8 a lane 60 / 50, 4 a lane 79 / 57
-//   d = 66 (2):     10 a lane 56 / 50, 16 a lane 63 / 56;  d = 65 (1): 10 a lane 93 / 85, 16 a lane 121 / 104
+//   d = 100 (4):    8 a lane 60 / 50, 4 a lane 79 / 57;  8 a lane of 4 lanes, known to the compiler (LG) so that a
+//                   lane's granules are at constant distances, 49 / 48;  d = 204: 16 a lane of 4 90, 8 of 8 119
+//   d = 66 (2):     10 a lane 56 / 50, 16 a lane 63 / 56;  d = 126: 8 a lane of 8 81 / 71, not known to be 8 96 / 81
+//   d = 65 (1):     10 a lane 93 / 85, 16 a lane 121 / 104
 //   MXFP4 quantise  d = 40 (8): two granules of a block in a lane 19, one 29;  d = 100 (4): two 58, one 80;
 //                   d = 66 (2): four 59, one 126
 // Small granules cost instructions: 52 a value at d = 65, where granules of 16 have 7.5, and that bounds them.
@@ -185,6 +196,16 @@ Plan granule_plan(uint32_t head_dim, uint64_t alignment)
             const Plan p = granule_plan<true, FMT, T, 4, false, 2, 4, 8, 16>(head_dim, 2);
             return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 4, false, 1, 8, 16>(head_dim, 0);
         } else {
+            if constexpr (QUANTISE || sizeof(T) == 2) {
+                if (head_dim > 40 && head_dim <= 128) {
+                    return group_plan<QUANTISE, FMT, T, 4, false, 1, 2, 4, 8>(head_dim, 2);
+                }
+            }
+            if constexpr (QUANTISE && sizeof(T) == 2) {
+                if (head_dim > 128 && head_dim <= 256) {
+                    return group_plan<true, FMT, T, 4, false, 1, 2, 16>(head_dim, 2);
+                }
+            }
             return granule_plan<QUANTISE, FMT, T, 4, false, 1, 8, 5, 4>(head_dim, 1);
         }
     }
@@ -192,8 +213,13 @@ Plan granule_plan(uint32_t head_dim, uint64_t alignment)
     if constexpr (FMT == kv::kMxFp4) {
         return even ? pair_plan<QUANTISE, T, false>(head_dim) : pair_plan<QUANTISE, T, true>(head_dim);
     } else {
-        return even ? granule_plan<QUANTISE, FMT, T, 2, false, 1, 8, 10, 14>(head_dim, 2)
-                    : granule_plan<QUANTISE, FMT, T, 1, false, 1, 10, 16>(head_dim, 2);
+        if (!even) {
+            return granule_plan<QUANTISE, FMT, T, 1, false, 1, 10, 16>(head_dim, 2);
+        }
+        if (head_dim > 80 && head_dim <= 256) {
+            return group_plan<QUANTISE, FMT, T, 2, false, 1, 3, 8, 16>(head_dim, 3);
+        }
+        return granule_plan<QUANTISE, FMT, T, 2, false, 1, 8, 10, 14>(head_dim, 2);
     }
 }
 

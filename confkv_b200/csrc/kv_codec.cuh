@@ -610,16 +610,18 @@ __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record
     }
 }
 
+// LG: lg_group where it is known when compiling, else -1.
+//
 // MXFP4: a block's granules are in neighbouring lanes, SPAN in each. SPAN = 1: the group has at least 32 / E lanes;
 // else it has 32 / (E * SPAN).
-template <int FMT, class T, int E, int R, bool SPLIT, int SPAN>
+template <int FMT, class T, int E, int R, bool SPLIT, int SPAN, int LG>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constant__ Args a)
 {
     constexpr int words = kGranuleWords<T, E>;
     dev::pdl_release();
     dev::pdl_wait();
     const Run& r = run_of_tile(a, blockIdx.x);
-    const uint32_t lg = a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
+    const uint32_t lg = LG >= 0 ? static_cast<uint32_t>(LG & 31) : a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
     const uint32_t groups = kThreads >> lg;
     const uint32_t d = a.head_dim;
     const uint32_t v = (blockIdx.x - r.tile_start) * groups + (threadIdx.x >> lg);
@@ -791,7 +793,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     }
 }
 
-template <int FMT, class T, int E, int R, bool SPLIT>
+template <int FMT, class T, int E, int R, bool SPLIT, int LG>
 __global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_constant__ Args a)
 {
     constexpr int words = kGranuleWords<T, E>;
@@ -799,7 +801,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_const
     dev::pdl_release();
     dev::pdl_wait();
     const Run& r = run_of_tile(a, blockIdx.x);
-    const uint32_t lg = a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
+    const uint32_t lg = LG >= 0 ? static_cast<uint32_t>(LG & 31) : a.lg_group, lane = threadIdx.x & ((1u << lg) - 1u);
     const uint32_t groups = kThreads >> lg;
     const uint32_t d = a.head_dim;
     const uint32_t v = (blockIdx.x - r.tile_start) * groups + (threadIdx.x >> lg);
