@@ -162,6 +162,35 @@ def test_ties_go_to_even(make):
         [6, 0, 1, 1, 2, 2, 4, 4, -4, 0.5, 6]
 
 
+def quotients(dtype, firsts, gaps, exponent):
+    """Vectors of 64: a largest value (every one of `firsts`, whole numbers of the type's bits, times 2^exponent) and all
+    values of the type below it in `gaps` binades, of both signs in turns."""
+    bits_ = {torch.bfloat16: 8, torch.float16: 11}[dtype]
+    m = torch.arange(1 << (bits_ - 1), 1 << bits_, dtype=torch.float64)
+    rows = []
+    for a in firsts:
+        x = torch.cat([m[m <= a]] + [m * 2.0 ** -g for g in range(1, gaps)])
+        x = torch.nn.functional.pad(x, (0, -len(x) % 63)).view(-1, 63)
+        x[:, 1::2] *= -1
+        rows.append(torch.cat([torch.full((len(x), 1), float(a), dtype=torch.float64), x], 1))
+    return (torch.cat(rows) * 2.0 ** exponent).to(dtype)
+
+
+@pytest.mark.parametrize("fmt,gaps", [("int8", 10), ("fp8", 20)])
+@pytest.mark.parametrize("exponent", [-7, 110, -110])
+def test_every_code_of_bfloat16(make, fmt, gaps, exponent):
+    x = quotients(torch.bfloat16, range(128, 256), gaps, exponent).view(1, 1, -1, 1, 64)
+    round_trip(make(fmt, "bf16", 1, 1, 1, 64), x)
+
+
+@pytest.mark.parametrize("fmt,gaps", [("int8", 10), ("fp8", 10)])
+def test_codes_of_half(make, fmt, gaps):
+    """All multiples of 127 and of 7 times a power of two among the largest values, their neighbours, and some others."""
+    firsts = {k * 127 + o for k in range(9, 17) for o in (-1, 0, 1)} | {1024, 1025, 1120, 1344, 1568, 1792, 1793, 2047} | set(range(1030, 2048, 97))
+    x = quotients(torch.float16, sorted(f for f in firsts if 1024 <= f < 2048), gaps, -10).view(1, 1, -1, 1, 64)
+    round_trip(make(fmt, "fp16", 1, 1, 1, 64), x)
+
+
 def test_errors_are_within_half_a_step(make):
     """Against the source itself, with bounds from the formats: A / 254; 2^-4 of the value or half of e4m3's least
     step; a quarter of the value, half of e2m1's least step, or what saturates (A < 8 2^e, the largest code 6 2^e). To
@@ -398,6 +427,34 @@ def test_slots_of_rows_at_a_distance(make):
     codec.quantise_paged(PagedKvCache(codec, [l[0] for l in pool.unbind(0)]), table[:, 3:12], rec)
     for k in range(4):
         assert_record(rec[k], by_slots(host, table[k, 3:12].cpu()), "fp8")
+
+
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+def test_no_tokens_and_no_pages(make, fmt):
+    """Empty slots, and a cache without blocks, whose every slot is outside it."""
+    codec = make(fmt, "bf16", 2, 3, 2, 64)
+    _, pool = paged(3, 2, 4, 16, 2, 64, torch.bfloat16, "NHD", seed=1)
+    before = pool.clone()
+    cache = PagedKvCache(codec, list(pool.unbind(0)))
+    nothing = PagedKvCache(codec, list(pool[:, :, :0].unbind(0)))
+    slots = torch.empty(0, dtype=torch.int64, device="cuda")
+    some = torch.tensor([0, 5, -1], device="cuda")
+    rec = torch.full((codec.record_bytes(0),), 7, dtype=torch.uint8, device="cuda")
+    codec.quantise_paged(cache, slots, rec)
+    assert rec.cpu().numpy().tobytes() == kv_ref.header(fmt, torch.bfloat16, 2, 3, 0, 2, 64).tobytes()
+    ok = torch.zeros(1, dtype=torch.int32, device="cuda")
+    codec.dequantise_paged(rec, cache, slots, ok=ok)
+    assert int(ok) == 1
+    big = torch.full((codec.record_bytes(3),), 7, dtype=torch.uint8, device="cuda")
+    codec.quantise_paged(nothing, some, big)
+    assert_record(big, torch.zeros(2, 3, 3, 2, 64, dtype=torch.bfloat16), fmt)
+    ok.zero_()
+    codec.dequantise_paged(big, nothing, some, ok=ok)
+    assert int(ok) == 1 and torch.equal(pool, before)
+    # and rows of no objects
+    codec.quantise(torch.empty(0, 2, 3, 4, 2, 64, dtype=torch.bfloat16, device="cuda"),
+                   torch.empty(0, codec.record_bytes(4), dtype=torch.uint8, device="cuda"))
+    codec.quantise([], [])
 
 
 def test_a_nan_in_a_slot_that_is_not_named_stays_out(make):
