@@ -5,14 +5,14 @@
 // on the other, beside one comparison, one product and one rounding. At the 6.55 TB/s of a plain copy
 // that is 2.2e12 values a second, for which the SMs have 16 instructions of a lane a value at full clocks
 // and 13 at the 1.5 GHz to which the power limit takes them in a run of seconds; so the kernels read each byte once,
-// in the widest loads, and spend 7.5 and 6.1 instructions a value (INT8, counted). Everything is one launch (16 runs of objects, whatever
-// their sizes, in the kernel's parameters), without workspace or atomics.
+// in the widest loads, and spend 7.5 and 6.1 instructions a value (INT8, counted). A call is one launch for up to 16 runs
+// of objects of whatever sizes, which travel in the kernel's parameters; there is no workspace and there are no atomics.
 //
 // Measured on B200, [2, 32, 256, 8, 128] bfloat16 objects (32 MiB), events, L2 cold (quantise / dequantise):
-//   32 objects, INT8   231 / 236 us  (7.05 / 6.90 TB/s; 234 / 238 us in a run of seconds)
+//   32 objects, INT8   231 / 236 us  (7.05 / 6.90 TB/s; 234 to 239 / 238 us in a run of seconds)
 //   16 objects, FP8    116 / 120 us  (7.04 / 6.77 TB/s; 127 / 120 us)
 //   16 objects, MXFP4   98 / 102 us  (6.96 / 6.68 TB/s; 108 / 101 us)
-//   1 object, INT8     9.7 / 9.7 us  (5.25 TB/s: the ramp and the tail of 8192 short blocks)
+//   1 object, INT8     9.7 / 9.7 us  (5.25 TB/s: the ramp and the tail of 2048 short blocks)
 //   1 token, INT8      2.1 / 2.1 us  (a launch)
 #pragma once
 

@@ -116,6 +116,7 @@ class KvCodec:
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         if self.device.type != "cuda" or self.device.index is None:
             raise ValueError("kv codec: device must be a CUDA device with its index")
+        self._index = self.device.index
         _declare(library.lib)
         self._layout = KvLayout(FORMATS.index(format), DTYPES.index(dtype), self.planes, self.layers, self.heads,
                                 self.head_dim)
@@ -160,7 +161,7 @@ class KvCodec:
     # ---- arguments
     def _run(self, record, tokens, count, object_args, slots_args, ok) -> bytes:
         size = self._sizes.get(tokens) or self.record_bytes(tokens)
-        if record.dtype != torch.uint8 or record.device != self.device:
+        if record.dtype is not torch.uint8 or record.get_device() != self._index:
             raise ValueError(f"kv codec: records are uint8 tensors on {self.device}")
         shape, strides = record.shape, record.stride()
         if len(shape) == 1 and count == 1:
@@ -176,13 +177,13 @@ class KvCodec:
             raise ValueError("kv codec: records are contiguous, at multiples of 16 bytes, and do not overlap")
         ok_ptr = 0
         if ok is not None:
-            if ok.dtype != torch.int32 or ok.device != self.device or ok.numel() != count or not ok.is_contiguous():
+            if ok.dtype is not torch.int32 or ok.get_device() != self._index or ok.numel() != count or not ok.is_contiguous():
                 raise ValueError(f"kv codec: ok is an int32 tensor of one value an object on {self.device}")
             ok_ptr = ok.data_ptr()
         return RUN.pack(*object_args, *slots_args, ptr, stride, size, ok_ptr, tokens, count)
 
     def _read_run(self, obj, record, ok) -> bytes:
-        if obj.dtype != self.dtype or obj.device != self.device:
+        if obj.dtype is not self.dtype or obj.get_device() != self._index:
             raise ValueError(f"kv codec: objects are {self.dtype} tensors on {self.device}")
         shape, strides = obj.shape, obj.stride()
         if len(shape) == 5:
@@ -204,16 +205,17 @@ class KvCodec:
         return self._read_run(obj, record, ok)
 
     def _slots_run(self, slots, record, ok) -> bytes:
-        if slots.dtype != torch.int64 or slots.device != self.device:
+        if slots.dtype is not torch.int64 or slots.get_device() != self._index:
             raise ValueError(f"kv codec: slots are int64 tensors on {self.device}")
-        if slots.dim() == 1:
+        shape, strides = slots.shape, slots.stride()
+        if len(shape) == 1:
             count, stride = 1, 0
-        elif slots.dim() == 2:
-            count, stride = slots.shape[0], slots.stride(0)
+        elif len(shape) == 2:
+            count, stride = shape[0], strides[0]
         else:
             raise ValueError("kv codec: slots are [tokens], or a row of them")
-        tokens = slots.shape[-1]
-        if slots.stride(-1) != 1 and tokens > 1:
+        tokens = shape[-1]
+        if strides[-1] != 1 and tokens > 1:
             raise ValueError("kv codec: the slots of an object have to follow one another")
         return self._run(record, tokens, count, (0,) * 6, (slots.data_ptr(), stride), ok)
 
@@ -223,17 +225,19 @@ class KvCodec:
             ok = ok if ok is None else _as_list(ok)
         if len(sources) != len(records) or ok is not None and len(ok) != len(sources):
             raise ValueError("kv codec: one tensor of records (and of verdicts) for every tensor of objects or slots")
-        if ok is None:
+        if len(sources) == 1:
+            raw = make(sources[0], records[0], None if ok is None else ok[0])
+        elif ok is None:
             raw = b"".join([make(s, r, None) for s, r in zip(sources, records)])
         else:
             raw = b"".join([make(s, r, k) for s, r, k in zip(sources, records, ok)])
         if stream is None:
-            handle = torch._C._cuda_getCurrentRawStream(self.device.index)
+            handle = torch._C._cuda_getCurrentRawStream(self._index)
         else:
             if stream.device != self.device:
                 raise ValueError(f"kv codec: the stream is not one of {self.device}")
             handle = stream.cuda_stream
-        rc = fn(self._layout_ptr, cache, raw, len(sources), self.device.index, handle)
+        rc = fn(self._layout_ptr, cache, raw, len(sources), self._index, handle)
         if rc != 0:
             self.library.check(rc, fn.__name__.removeprefix("lmcache_gpu_").removesuffix("_async"))
 

@@ -160,6 +160,19 @@ uint64_t kv_check_quotients(int format, int bits, int max_gap, int step, int exp
                      : check_quotients<float>(format, bits, max_gap, step, exponent);
 }
 
+// scale_of against the machine's division for every float of a binade; the number that differ.
+uint64_t kv_check_scales(int format, int exponent)
+{
+    uint64_t bad = 0;
+    for (uint32_t m = 0; m < 1u << 23; ++m) {
+        const float a = kv::bits_float(static_cast<uint32_t>(exponent + 127) << 23 | m);
+        const float want = format == kv::kInt8 ? a / 127.0f : a / 448.0f;
+        const float got = format == kv::kInt8 ? kv::scale_of<kv::kInt8>(a) : kv::scale_of<kv::kFp8>(a);
+        bad += want != got;
+    }
+    return bad;
+}
+
 uint32_t kv_check_mx_byte(uint32_t bits) { return kv::mx_scale_byte(bits); }
 float kv_check_mx_inverse(uint32_t byte) { return kv::mx_inverse(byte); }
 float kv_check_scale(int format, float amax)

@@ -146,6 +146,9 @@ class Fake:
     def data_ptr(self):
         return self._ptr
 
+    def get_device(self):
+        return self.device.index if self.device.type == "cuda" else -1
+
     def is_contiguous(self):
         return self._strides == torch.empty(self.shape, device="meta").stride()
 

@@ -36,6 +36,8 @@ def lib(tmp_path_factory):
     lib.kv_check_mx_byte.restype = u32
     lib.kv_check_mx_inverse.argtypes = [u32]
     lib.kv_check_mx_inverse.restype = ctypes.c_float
+    lib.kv_check_scales.argtypes = [i32, i32]
+    lib.kv_check_scales.restype = u64
     lib.kv_check_scale.argtypes = [i32, ctypes.c_float]
     lib.kv_check_scale.restype = ctypes.c_float
     return lib
@@ -117,6 +119,12 @@ def test_scales(lib, fmt, top):
         want = min(np.float32(a) / np.float32(top), kv_ref.MOST_SCALE[top])
         assert np.float32(s) == want
         assert np.isfinite(np.float32(s) * np.float32(top))
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("exponent", [0, -100, -101, 120])
+def test_every_scale_is_the_rounded_quotient(lib, fmt, exponent):
+    assert lib.kv_check_scales(fmt, exponent) == 0
 
 
 @pytest.mark.parametrize("fmt", kv_ref.FORMATS)
