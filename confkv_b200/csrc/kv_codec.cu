@@ -93,10 +93,10 @@ uint32_t log2_up(uint32_t n)
     return l;
 }
 
-// The plan for vectors cut into granules of E values, in groups of at least 2^least lanes (LG >= 0: of 2^LG): of the R
-// in the list the one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
-template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int LG, int... R>
-Plan group_plan(uint32_t head_dim, uint32_t least)
+// The plan for vectors cut into granules of E values, in groups of at least 2^least lanes: of the R in the list the
+// one that leaves the fewest lanes idle, the first of equals. No kernel: no group is large enough.
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int... R>
+Plan granule_plan(uint32_t head_dim, uint32_t least)
 {
     const uint32_t granules = (head_dim + E - 1) / E;
     uint32_t most = 5;
@@ -104,9 +104,6 @@ Plan group_plan(uint32_t head_dim, uint32_t least)
         // the lanes that share a block
         least = std::max(least, log2_up(kv::kMxBlock / (E * SPAN)));
         most = SPAN > 1 ? least : most;
-    }
-    if (LG >= 0) {
-        least = most = static_cast<uint32_t>(LG & 31);
     }
     Plan best{nullptr, 0};
     uint32_t held = ~0u;
@@ -116,9 +113,9 @@ Plan group_plan(uint32_t head_dim, uint32_t least)
             if (lg <= most && (uint32_t{R} << lg) < held) {
                 held = uint32_t{R} << lg;
                 if constexpr (QUANTISE) {
-                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT, SPAN, LG>, lg};
+                    best = Plan{kv::quantise_kernel<FMT, T, E, R, SPLIT, SPAN, -1>, lg};
                 } else {
-                    best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT, LG>, lg};
+                    best = Plan{kv::dequantise_kernel<FMT, T, E, R, SPLIT, -1>, lg};
                 }
             }
         }(),
@@ -126,10 +123,45 @@ Plan group_plan(uint32_t head_dim, uint32_t least)
     return best;
 }
 
-template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int SPAN, int... R>
-Plan granule_plan(uint32_t head_dim, uint32_t least)
+// Granules of E values, R a lane in groups of 2^LG lanes, where a group holds the vector and no plan has been found
+// before. Not for quantising MXFP4, whose groups are bound to its blocks.
+template <bool QUANTISE, int FMT, class T, int E, bool SPLIT, int R, int LG>
+void fit(uint32_t head_dim, Plan* p)
 {
-    return group_plan<QUANTISE, FMT, T, E, SPLIT, SPAN, -1, R...>(head_dim, least);
+    if (p->kernel == nullptr && head_dim <= static_cast<uint32_t>((E * R) << LG)) {
+        if constexpr (E == 1) {
+            p->kernel = QUANTISE ? kv::quantise_single_kernel<FMT, T, R, LG> : kv::dequantise_single_kernel<FMT, T, R, LG>;
+        } else if constexpr (QUANTISE) {
+            p->kernel = kv::quantise_kernel<FMT, T, E, R, SPLIT, 1, LG>;
+        } else {
+            p->kernel = kv::dequantise_kernel<FMT, T, E, R, SPLIT, LG>;
+        }
+        p->lg_group = LG;
+    }
+}
+
+template <bool QUANTISE, int FMT, class T, bool SPLIT>
+Plan fit_pairs(uint32_t head_dim)
+{
+    Plan p{nullptr, 0};
+    fit<QUANTISE, FMT, T, 2, SPLIT, 4, 2>(head_dim, &p);
+    fit<QUANTISE, FMT, T, 2, SPLIT, 6, 2>(head_dim, &p);
+    if constexpr (SPLIT) {
+        fit<QUANTISE, FMT, T, 2, SPLIT, 4, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 6, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 4, 4>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 8, 4>(head_dim, &p);
+    } else {
+        fit<QUANTISE, FMT, T, 2, SPLIT, 8, 2>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 10, 2>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 6, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 8, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 12, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 2, SPLIT, 16, 3>(head_dim, &p);
+    }
+    fit<QUANTISE, FMT, T, 2, SPLIT, 16, 4>(head_dim, &p);
+    fit<QUANTISE, FMT, T, 2, SPLIT, 16, 5>(head_dim, &p);
+    return p;
 }
 
 // MXFP4 in granules of 2: a lane holds several granules of a block where the vector is short enough for it.
@@ -144,10 +176,8 @@ Plan pair_plan(uint32_t head_dim)
             p = granule_plan<true, kv::kMxFp4, T, 2, SPLIT, 4, 8, 12, 16, 24, 32>(head_dim, 2);
         }
         return p.kernel != nullptr ? p : granule_plan<true, kv::kMxFp4, T, 2, SPLIT, 1, 8, 16>(head_dim, 0);
-    } else if constexpr (SPLIT) {
-        return granule_plan<false, kv::kMxFp4, T, 2, SPLIT, 1, 4, 8, 16>(head_dim, 3);
     } else {
-        return granule_plan<false, kv::kMxFp4, T, 2, SPLIT, 1, 8, 10, 14>(head_dim, 2);
+        return fit_pairs<false, kv::kMxFp4, T, SPLIT>(head_dim);
     }
 }
 
@@ -163,13 +193,15 @@ Plan warp_plan(bool quantise)
 //   INT8 quantise   d = 200 (8): 8 a lane 89, 4 a lane 108; d = 72: 5 a lane 35, 3 a lane 46; d = 56: two lanes 29,
 //                   one lane 33
 //   INT8 dequantise d = 72 (8): 3 a lane 31, 5 a lane 37; d = 200: 4 a lane 75, 8 a lane 81
-//   d = 100 (4):    8 a lane 60 / 50, 4 a lane 79 / 57;  8 a lane of 4 lanes, known to the compiler (LG) so that a
-//                   lane's granules are at constant distances, 49 / 48;  d = 204: 16 a lane of 4 90, 8 of 8 119
-//   d = 66 (2):     10 a lane 56 / 50, 16 a lane 63 / 56;  d = 126: 8 a lane of 8 81 / 71, not known to be 8 96 / 81
-//   d = 65 (1):     10 a lane 93 / 85, 16 a lane 121 / 104
-//   MXFP4 quantise  d = 40 (8): two granules of a block in a lane 19, one 29;  d = 100 (4): two 58, one 80;
+//   MXFP4 quantise  d = 40 (8): two granules of a block in a lane 19, one 29;  d = 100 (4): two 57, one 80;
 //                   d = 66 (2): four 59, one 126
-// Small granules cost instructions: 52 a value at d = 65, where granules of 16 have 7.5, and that bounds them.
+// With granules of 4 and fewer values instructions bound the kernel (419 of a warp for four vectors of 65 values, 52 a
+// value, before `fit`), so the group is a constant and lane i's granules are at constant distances (INT8 quantise,
+// known and not known when compiling: d = 100 (4) 49 and 61, d = 126 (2) 80 and 96), and single values are worked on in
+// twos (d = 65: 67 and 92). R and LG are the fastest of 13 pairs each at 14 to 19 head sizes, of which a few:
+//   d = 36 (4)  5 of two lanes 22, 3 of four 30       d = 204 (4)  8 of eight lanes 92, 16 of four 89 (252: 101, 110)
+//   d = 34 (2)  6 of four 32, 4 of eight 54           d = 126 (2)  8 of eight 80, 16 of four 119, 4 of sixteen 112
+//   d = 33 (1)  12 of four 34, 8 of eight 55          d = 127 (1)  8 of sixteen 113, 16 of eight 134
 template <bool QUANTISE, int FMT, class T>
 Plan granule_plan(uint32_t head_dim, uint64_t alignment)
 {
@@ -196,30 +228,43 @@ Plan granule_plan(uint32_t head_dim, uint64_t alignment)
             const Plan p = granule_plan<true, FMT, T, 4, false, 2, 4, 8, 16>(head_dim, 2);
             return p.kernel != nullptr ? p : granule_plan<true, FMT, T, 4, false, 1, 8, 16>(head_dim, 0);
         } else {
+            Plan p{nullptr, 0};
             if constexpr (QUANTISE || sizeof(T) == 2) {
-                if (head_dim > 40 && head_dim <= 128) {
-                    return group_plan<QUANTISE, FMT, T, 4, false, 1, 2, 4, 8>(head_dim, 2);
-                }
+                fit<QUANTISE, FMT, T, 4, false, 5, 1>(head_dim, &p);
             }
-            if constexpr (QUANTISE && sizeof(T) == 2) {
-                if (head_dim > 128 && head_dim <= 256) {
-                    return group_plan<true, FMT, T, 4, false, 1, 2, 16>(head_dim, 2);
-                }
+            fit<QUANTISE, FMT, T, 4, false, 3, 2>(head_dim, &p);
+            fit<QUANTISE, FMT, T, 4, false, 4, 2>(head_dim, &p);
+            fit<QUANTISE, FMT, T, 4, false, 5, 2>(head_dim, &p);
+            fit<QUANTISE, FMT, T, 4, false, 6, 2>(head_dim, &p);
+            if constexpr (!QUANTISE && sizeof(T) == 4) {
+                fit<QUANTISE, FMT, T, 4, false, 4, 3>(head_dim, &p);
+            } else {
+                fit<QUANTISE, FMT, T, 4, false, 8, 2>(head_dim, &p);
+                fit<QUANTISE, FMT, T, 4, false, 12, 2>(head_dim, &p);
             }
-            return granule_plan<QUANTISE, FMT, T, 4, false, 1, 8, 5, 4>(head_dim, 1);
+            fit<QUANTISE, FMT, T, 4, false, 8, 3>(head_dim, &p);
+            fit<QUANTISE, FMT, T, 4, false, 8, 4>(head_dim, &p);
+            fit<QUANTISE, FMT, T, 4, false, 8, 5>(head_dim, &p);
+            return p;
         }
     }
     const bool even = head_dim % 2 == 0 && alignment >= 2 * sizeof(T);
     if constexpr (FMT == kv::kMxFp4) {
         return even ? pair_plan<QUANTISE, T, false>(head_dim) : pair_plan<QUANTISE, T, true>(head_dim);
     } else {
-        if (!even) {
-            return granule_plan<QUANTISE, FMT, T, 1, false, 1, 10, 16>(head_dim, 2);
+        if (even) {
+            return fit_pairs<QUANTISE, FMT, T, false>(head_dim);
         }
-        if (head_dim > 80 && head_dim <= 256) {
-            return group_plan<QUANTISE, FMT, T, 2, false, 1, 3, 8, 16>(head_dim, 3);
-        }
-        return granule_plan<QUANTISE, FMT, T, 2, false, 1, 8, 10, 14>(head_dim, 2);
+        Plan p{nullptr, 0};
+        fit<QUANTISE, FMT, T, 1, false, 8, 2>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 12, 2>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 8, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 12, 3>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 8, 4>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 12, 4>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 16, 4>(head_dim, &p);
+        fit<QUANTISE, FMT, T, 1, false, 16, 5>(head_dim, &p);
+        return p;
     }
 }
 

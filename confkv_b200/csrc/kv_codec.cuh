@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) dequantise_warp_kernel(const __grid_
 // granule may lack its second value, for odd head_dim and for vectors at odd addresses.
 
 template <class T, int E>
-constexpr int kGranuleWords = (E * sizeof(T) + 3) / 4;
+constexpr int kGranuleWords = E * sizeof(T) / 4;
 
 __device__ __forceinline__ void load32(uint32_t* w, const void* p)
 {
@@ -558,8 +558,6 @@ __device__ __forceinline__ void codes_of(uint32_t* c, const uint32_t* w, const R
         for (int i = 0; i < E / 4; ++i) {
             c[i] = __byte_perm(rule.codes(floats_of<T>(w, 2 * i)), rule.codes(floats_of<T>(w, 2 * i + 1)), 0x5410);
         }
-    } else if constexpr (E == 1 && sizeof(T) == 4) {
-        c[0] = rule.codes(make_float2(__uint_as_float(w[0]), 0.0f));
     } else {
         c[0] = rule.codes(floats_of<T>(w, 0));
     }
@@ -610,7 +608,7 @@ __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record
     }
 }
 
-// LG: lg_group where it is known when compiling, else -1.
+// LG: lg_group where it is known when compiling, else -1. E is 2 or more (quantise_single_kernel below).
 //
 // MXFP4: a block's granules are in neighbouring lanes, SPAN in each. SPAN = 1: the group has at least 32 / E lanes;
 // else it has 32 / (E * SPAN).
@@ -860,9 +858,9 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_const
                     values4<FMT>(f + 2 * i, c[j][i] & keep);
                 }
             }
-            uint32_t w[E > 1 ? words : 2];
+            uint32_t w[words];
 #pragma unroll
-            for (int i = 0; i < (E + 1) / 2; ++i) {
+            for (int i = 0; i < E / 2; ++i) {
                 const float2 v = halves(mul(f[i], s));
                 if constexpr (sizeof(T) == 4) {
                     w[2 * i] = __float_as_uint(v.x);
@@ -872,6 +870,147 @@ __global__ void __launch_bounds__(kThreads) dequantise_kernel(const __grid_const
                 }
             }
             store_granule<T, E, SPLIT>(dst + at, w, at + 1 < d);
+        }
+    }
+}
+
+// ------------------------------------------------------ single values
+//
+// INT8 and FP8 of vectors with an odd head size, or at odd addresses: granules of one value, of which a lane holds R, a
+// multiple of 4, in a group of 2^LG lanes. Instructions bound this (a load, a store and a test of the end a value), so
+// values are worked on in twos and codes in fours, and LG is constant: 8 objects of head size 65 from bfloat16 to INT8
+// and back 88 / 88 us (2.4 TB/s), where the granule kernels with E = 1 took 119 / 113.
+
+template <int FMT, class T, int R, int LG>
+__global__ void __launch_bounds__(kThreads) quantise_single_kernel(const __grid_constant__ Args a)
+{
+    constexpr int words = sizeof(T) == 4 ? R : R / 2;
+    constexpr uint32_t lanes = 1u << LG;
+    dev::pdl_release();
+    dev::pdl_wait();
+    const Run& r = run_of_tile(a, blockIdx.x);
+    const uint32_t lane = threadIdx.x & (lanes - 1u);
+    const uint32_t v = (blockIdx.x - r.tile_start) * (kThreads / lanes) + (threadIdx.x >> LG);
+    const bool mine = v < r.units;
+    const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
+    const T* src = mine && r.empty == 0 ? reinterpret_cast<const T*>(vector_address(a, r, x)) : nullptr;
+    // this lane's values: those at lane + j * lanes below the head size
+    const uint32_t left = lane < a.head_dim ? a.head_dim - lane : 0u;
+    const uint32_t there = src != nullptr ? left : 0u;
+    src += lane;
+    uint32_t w[words];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        uint32_t one = 0;
+        if (j * lanes < there) {
+            load_bytes<sizeof(T)>(&one, src + j * lanes);
+        }
+        if constexpr (sizeof(T) == 4) {
+            w[j] = one;
+        } else {
+            w[j / 2] = j % 2 == 0 ? one : __byte_perm(w[j / 2], one, 0x5410);
+        }
+    }
+    uint32_t m = halves_max<T>(max_of<T, words>(0, w));
+#pragma unroll
+    for (uint32_t o = 1; o < lanes; o <<= 1) {
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    if (!mine) {
+        return;
+    }
+    char* record = r.record + x.object * r.record_stride;
+    if (x.in_object == 0 && lane == 0) {
+        write_frame_of_record(r, record);
+    }
+    if (r.empty != 0) {
+        return;
+    }
+    uint8_t* codes = reinterpret_cast<uint8_t*>(record) + kHeaderBytes + uint64_t{x.in_object} * a.head_dim + lane;
+    const uint32_t bits = as_float_bits<T>(m);
+    const bool finite = bits < kInfinity;
+    const uint32_t keep = finite ? ~0u : 0u;
+    const float amax = finite ? __uint_as_float(bits) : 0.0f;
+    const auto write_codes = [&](const auto& rule) {
+#pragma unroll
+        for (int j = 0; j < R; j += 2) {
+            const uint32_t c = rule.codes(floats_of<T>(w, j / 2)) & keep;
+            if (j * lanes < left) {
+                codes[j * lanes] = static_cast<uint8_t>(c);
+            }
+            if ((j + 1) * lanes < left) {
+                codes[(j + 1) * lanes] = static_cast<uint8_t>(c >> 8);
+            }
+        }
+    };
+    if constexpr (sizeof(T) == 4) {
+        const Divider<double> div = make_divider<double>(amax, kTop<FMT>);
+        write_codes(ByDoubleQuotient<FMT>{div});
+    } else if constexpr (FMT == kFp8) {
+        write_codes(ByQuotient<FMT>(make_divider<float>(amax, kTop<FMT>)));
+    } else {
+        float factor;
+        if (int8_factor<std::is_same_v<T, __half>>(amax, &factor)) {
+            write_codes(Int8ByFactor(factor));
+        } else {
+            write_codes(ByQuotient<FMT>(make_divider<float>(amax, kTop<FMT>)));
+        }
+    }
+    if (lane == 0) {
+        reinterpret_cast<float*>(record + r.scales_at)[x.in_object] = finite ? scale_of<FMT>(amax) : bits_float(kNan);
+    }
+}
+
+template <int FMT, class T, int R, int LG>
+__global__ void __launch_bounds__(kThreads) dequantise_single_kernel(const __grid_constant__ Args a)
+{
+    constexpr uint32_t lanes = 1u << LG;
+    dev::pdl_release();
+    dev::pdl_wait();
+    const Run& r = run_of_tile(a, blockIdx.x);
+    const uint32_t lane = threadIdx.x & (lanes - 1u);
+    const uint32_t v = (blockIdx.x - r.tile_start) * (kThreads / lanes) + (threadIdx.x >> LG);
+    if (v >= r.units) {
+        return;
+    }
+    const VectorIndex x = vector_index(v, r.by_object, r.by_tokens, a.by_layers, a.by_heads);
+    const char* record = r.record + x.object * r.record_stride;
+    const uint32_t left = lane < a.head_dim && r.empty == 0 ? a.head_dim - lane : 0u;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(record) + kHeaderBytes + uint64_t{x.in_object} * a.head_dim + lane;
+    const uint32_t bits = r.empty == 0 ? reinterpret_cast<const uint32_t*>(record + r.scales_at)[x.in_object] : 0u;
+    uint32_t c[R / 4];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        uint32_t one = 0;
+        if (j * lanes < left) {
+            one = codes[j * lanes];
+        }
+        c[j / 4] = j % 4 == 0 ? one : __byte_perm(c[j / 4], one, j % 4 == 1 ? 0x3240 : (j % 4 == 2 ? 0x3410 : 0x4210));
+    }
+    T* dst = r.empty == 0 ? reinterpret_cast<T*>(vector_address(a, r, x)) : nullptr;
+    const bool good = header_matches(r, record);
+    if (x.in_object == 0 && lane == 0 && r.ok != nullptr) {
+        r.ok[x.object] = good ? 1 : 0;
+    }
+    if (dst == nullptr) {
+        return;
+    }
+    dst += lane;
+    const uint32_t keep = good ? ~0u : 0u;
+    const Pair s = make_pair(__uint_as_float(bits & keep), __uint_as_float(bits & keep));
+#pragma unroll
+    for (int j = 0; j < R; j += 4) {
+        Pair f[2];
+        values4<FMT>(f, c[j / 4] & keep);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 p = halves(mul(f[i], s));
+            if ((j + 2 * i) * lanes < left) {
+                dst[(j + 2 * i) * lanes] = from_float<T>(p.x);
+            }
+            if ((j + 2 * i + 1) * lanes < left) {
+                dst[(j + 2 * i + 1) * lanes] = from_float<T>(p.y);
+            }
         }
     }
 }
