@@ -609,3 +609,61 @@ def test_same_calls_give_the_same_bytes(make):
         recs[k].fill_(k)                            # stale bytes do not show
         codec.quantise(x, recs[k])
     assert all(torch.equal(recs[0], recs[k]) for k in range(1, 4))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(gpu_lib):
+    codec = KvCodec(gpu_lib, "int8", torch.bfloat16, planes=2, layers=2, heads=4, head_dim=64, device=1)
+    x = values((2, 2, 33, 4, 64), torch.bfloat16, seed=1)
+    with torch.cuda.device(0):
+        rec = torch.zeros(codec.record_bytes(33), dtype=torch.uint8, device="cuda:1")
+        out = torch.zeros(x.shape, dtype=torch.bfloat16, device="cuda:1")
+        src = x.to("cuda:1")
+        codec.quantise(src, rec)                    # cuda:1's current stream
+        codec.dequantise(rec, out)
+        torch.cuda.synchronize(1)
+        assert torch.cuda.current_device() == 0
+    assert_record(rec, x, "int8")
+    assert torch.equal(bits(out), bits(kv_ref.read(rec.cpu().numpy(), "int8", torch.bfloat16, x.shape)))
+
+
+def test_codec_and_seal_in_one_graph(make, gpu_lib):
+    """Quantise, seal, open and read back captured together: no call waits for the host between them, and a replay
+    takes the object's new values."""
+    from confkv_b200.gpu_aesgcm import GpuAes128GcmKey
+
+    codec = make("mxfp4", "bf16", 2, 4, 8, 64)
+    x = torch.zeros(2, 4, 100, 8, 64, dtype=torch.bfloat16, device="cuda")
+    size = codec.record_bytes(100)
+    rec, opened = (torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(2))
+    frame = torch.zeros(size + 29, dtype=torch.uint8, device="cuda")
+    auth, ok = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+    out = torch.zeros_like(x)
+    s = torch.cuda.Stream()
+
+    def body():
+        codec.quantise(x, rec, stream=s)
+        key.seal_async(src_ptr=rec.data_ptr(), plaintext_len=size, dst_ptr=frame.data_ptr(), dst_capacity=size + 29,
+                       iv=bytes(12), stream_ptr=s.cuda_stream)
+        key.open_async(src_ptr=frame.data_ptr(), frame_len=size + 29, dst_ptr=opened.data_ptr(), plaintext_len=size,
+                       auth_ok_ptr=auth.data_ptr(), stream_ptr=s.cuda_stream)
+        codec.dequantise(opened, out, ok=ok, stream=s)
+
+    with GpuAes128GcmKey(gpu_lib, bytes(range(16))) as key:
+        torch.cuda.synchronize()
+        body()
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            body()
+        for seed in range(3):
+            host = values(x.shape, torch.bfloat16, seed=seed)
+            x.copy_(host)
+            for t in (opened, frame, auth, ok, out):
+                t.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert int(auth) == 1 and int(ok) == 1
+            assert_record(opened, host, "mxfp4")
+            assert torch.equal(bits(out), bits(kv_ref.read(opened.cpu().numpy(), "mxfp4", torch.bfloat16, host.shape)))
+        del g
