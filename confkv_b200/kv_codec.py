@@ -281,33 +281,44 @@ class PagedKvCache:
         self.layers = list(layers)
         if len(self.layers) != codec.layers or codec.layers * codec.planes > MAX_BASES:
             raise ValueError(f"kv codec: a paged cache has the codec's {codec.layers} layers, and {MAX_BASES} planes at most")
-        planes = [[], []]
+        # every plane is [blocks, block_size, heads, head_dim], all of one shape and with one set of strides
+        shape = strides = None
+        bases = [[] for _ in range(codec.planes)]
         for layer in self.layers:
-            parts = list(layer.unbind(0)) if isinstance(layer, torch.Tensor) and layer.dim() == 5 else \
-                [layer] if isinstance(layer, torch.Tensor) else list(layer)
-            if len(parts) != codec.planes:
+            joint = hasattr(layer, "data_ptr")              # one tensor a layer
+            parts = (layer,) if joint else tuple(layer)     # or keys and values apart
+            joint = joint and len(layer.shape) == 5
+            if (layer.shape[0] if joint else len(parts)) != codec.planes:
                 raise ValueError(f"kv codec: a layer has {codec.planes} planes")
-            for plane, t in zip(planes, parts):
-                plane.append(t)
-        every = planes[0] + planes[1]
-        first = every[0]
-        if first.dim() != 4:
+            for k, t in enumerate(parts):
+                if t.dtype is not codec.dtype or t.get_device() != codec._index:
+                    raise ValueError(f"kv codec: the layers are {codec.dtype} tensors on {codec.device}")
+                mine, by, ptr = t.shape, t.stride(), t.data_ptr()
+                if joint:
+                    step = by[0] * codec.dtype.itemsize
+                    for plane in range(codec.planes):
+                        bases[plane].append(ptr + plane * step)
+                    if shape is None:
+                        self._overlap = _overlaps(mine, by)
+                    mine, by = mine[1:], by[1:]
+                else:
+                    bases[k].append(ptr)
+                    if shape is None:
+                        self._overlap = _overlaps(mine, by)
+                if shape is None:
+                    shape, strides = mine, by
+                elif mine != shape or by != strides:
+                    raise ValueError("kv codec: all planes have the same shape and strides")
+        if len(shape) != 4:
             raise ValueError("kv codec: a plane is [blocks, block_size, heads, head_dim]")
-        for t in every:
-            if t.dtype != codec.dtype or t.device != codec.device:
-                raise ValueError(f"kv codec: the layers are {codec.dtype} tensors on {codec.device}")
-            if t.shape != first.shape or t.stride() != first.stride():
-                raise ValueError("kv codec: all planes have the same shape and strides")
-        blocks, size, heads, dim = first.shape
+        blocks, size, heads, dim = shape
         if (heads, dim) != (codec.heads, codec.head_dim) or size < 1 or blocks * size >= 1 << 31:
-            raise ValueError(f"kv codec: a plane of shape {tuple(first.shape)} is not one of this codec's")
-        if first.stride(-1) != 1 and dim > 1:
+            raise ValueError(f"kv codec: a plane of shape {tuple(shape)} is not one of this codec's")
+        if strides[-1] != 1 and dim > 1:
             raise ValueError("kv codec: the values of a vector have to follow one another")
         self.blocks, self.block_size = blocks, size
-        self._overlap = _overlaps(first.shape, first.stride())
-        self._bases = (ctypes.c_void_p * len(every))(*[t.data_ptr() for t in every])
-        self._pages = KvPages(ctypes.addressof(self._bases), blocks, size, 0, first.stride(0), first.stride(1),
-                              first.stride(2))
+        self._bases = (ctypes.c_void_p * (codec.planes * codec.layers))(*[p for plane in bases for p in plane])
+        self._pages = KvPages(ctypes.addressof(self._bases), blocks, size, 0, *strides[:3])
         self._pages_ptr = ctypes.addressof(self._pages)
 
     def writable(self) -> "PagedKvCache":

@@ -418,6 +418,24 @@ def test_paged_batches_and_foreign_records(make):
     assert torch.equal(bits(pool), bits(want.view(pool.shape)))
 
 
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+def test_blocks_that_hold_keys_and_values(make, fmt):
+    """[blocks, 2, block_size, heads, head_dim] seen as [2, blocks, ...], out and back into another such cache."""
+    codec = make(fmt, "bf16", 2, 3, 2, 80)
+    host = torch.randn(3, 2, 7, 16, 2, 80, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    pool = host.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+    slots = torch.randperm(7 * 16, generator=torch.Generator().manual_seed(4))[:50]
+    rec = torch.empty(codec.record_bytes(50), dtype=torch.uint8, device="cuda")
+    codec.quantise_paged(PagedKvCache(codec, list(pool.unbind(0))), slots.cuda(), rec)
+    x = by_slots(host, slots)
+    assert_record(rec, x, fmt)
+    dst = torch.full((3, 7, 2, 16, 2, 80), 3.0, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    codec.dequantise_paged(rec, PagedKvCache(codec, list(dst.unbind(0))), slots.cuda())
+    want = torch.full((3, 2, 7 * 16, 2, 80), 3.0, dtype=torch.bfloat16)
+    want[:, :, slots] = kv_ref.read(rec.cpu().numpy(), fmt, torch.bfloat16, x.shape).transpose(0, 1)
+    assert torch.equal(bits(dst), bits(want.view(3, 2, 7, 16, 2, 80)))
+
+
 def test_slots_of_rows_at_a_distance(make):
     """A request table's rows: slots [n, tokens] inside a wider matrix."""
     codec = make("fp8", "bf16", 1, 2, 2, 64)

@@ -251,6 +251,33 @@ def test_binding_refuses_bad_caches(codec, cpu_lib):
             codec.dequantise_paged([Fake((R,), U8)], cache, [slots])
 
 
+def test_caches_of_joint_and_separate_planes(codec, cpu_lib):
+    """[planes, ...] tensors, transposed ones, and pairs give the same addresses; a plane that lies on another is not
+    written to."""
+    block = 16 * 8 * 64
+    joint = [Fake((2, 9, 16, 8, 64), ptr=(1 << 20) + (k << 16)) for k in range(4)]
+    pairs = [(Fake(PLANE[1:], ptr=(1 << 20) + (k << 16)), Fake(PLANE[1:], ptr=(1 << 20) + (k << 16) + 9 * block * 2)) for k in range(4)]
+    a, b = PagedKvCache(codec, joint), PagedKvCache(codec, pairs)
+    assert list(a._bases) == list(b._bases) and len(a._bases) == 8
+    assert (a._pages.blocks, a._pages.block_size, a._pages.block_stride, a._pages.row_stride, a._pages.head_stride) == \
+        (b._pages.blocks, b._pages.block_size, b._pages.block_stride, b._pages.row_stride, b._pages.head_stride) == \
+        (9, 16, block, 512, 64)
+    mixed = PagedKvCache(codec, joint[:2] + pairs[2:])
+    assert list(mixed._bases) == list(a._bases)
+    # blocks that hold keys and values, [blocks, 2, ...], seen as [2, blocks, ...]
+    inside = [Fake((2, 9, 16, 8, 64), strides=(block, 2 * block, 512, 64, 1), ptr=1 << 20) for _ in range(4)]
+    c = PagedKvCache(codec, inside)
+    assert c.writable() is c and c._bases[4] - c._bases[0] == block * 2 and c._pages.block_stride == 2 * block
+    same = PagedKvCache(codec, [Fake((2, 9, 16, 8, 64), strides=(0, block, 512, 64, 1)) for _ in range(4)])
+    with pytest.raises(ValueError, match="overlap"):
+        same.writable()
+    one = KvCodec(cpu_lib, "int8", torch.bfloat16, planes=1, layers=2, heads=8, head_dim=64)
+    assert list(PagedKvCache(one, [Fake(PLANE[1:]), Fake((1, *PLANE[1:]))])._bases) == [1 << 20] * 2
+    for bad in ([Fake((3, 9, 16, 8, 64))] * 4, [Fake(PLANE[1:])] * 4, [Fake((2, 9, 16, 512))] * 4, [Fake((2, 1, 9, 16, 8, 64))] * 4):
+        with pytest.raises(ValueError, match="kv codec"):
+            PagedKvCache(codec, bad)
+
+
 def test_native_errors_reach_the_caller(codec):
     # what the binding lets through and the library refuses: an object at half an element
     class Stream:
