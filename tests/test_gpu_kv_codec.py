@@ -93,7 +93,9 @@ def round_trip(codec, x, device_view=None):
 HEAD_DIMS = [1, 2, 3, 7, 8, 15, 16, 17, 24, 31, 32, 33, 40, 48, 63, 64, 65, 72, 80, 96, 100, 112, 127, 128, 129, 160, 192, 200, 256,
              272, 320, 500, 512, 520, 576, 768, 1000, 1024, 1040, 1536, 1552, 2050, 5000,
              # every number of granules a lane, for granules of 1, 2, 4 and 8 values
-             34, 36, 50, 56, 60, 66, 68, 77, 88, 104, 108, 120, 126, 136, 201, 202, 204, 264, 400, 700, 1200, 1600, 2000, 2560, 2576]
+             34, 36, 50, 56, 60, 66, 68, 77, 88, 104, 108, 120, 126, 136, 201, 202, 204, 264, 400, 700, 1200, 1600, 2000, 2560, 2576,
+             # the largest groups of small granules, and what they no longer hold
+             44, 94, 140, 145, 172, 191, 257, 258, 260, 301, 386, 511, 513, 514, 516, 770, 772, 777, 1026, 1028]
 
 
 @pytest.mark.parametrize("fmt", kv_ref.FORMATS)
