@@ -99,6 +99,17 @@ def _overlaps(shape, strides) -> bool:
     return False
 
 
+def _meet(distance, dims) -> bool:
+    """Whether two planes of the same shape and strides, `distance` bytes apart, share memory: whether whole numbers
+    |a| < n give the distance as the sum of a * stride over `dims`, (stride, n) in falling order, of which each stride passes over
+    all that the smaller ones reach. So only the two multiples of a stride next to the distance come into question."""
+    if not dims:
+        return distance == 0
+    stride, n = dims[0]
+    a = distance // stride
+    return any(abs(k) < n and _meet(distance - k * stride, dims[1:]) for k in (a, a + 1))
+
+
 class KvCodec:
     """A format for the objects of one cache: [planes, layers, tokens, heads, head_dim] of `dtype`."""
 
@@ -266,8 +277,9 @@ class KvCodec:
     def dequantise_paged(self, records, cache: "PagedKvCache", slots, ok=None,
                          stream: torch.cuda.Stream | None = None) -> None:
         """Read records back into slots of a paged cache, and write to no other slot. Slots below 0 or outside the
-        cache are passed over; the others have to differ from one another."""
-        self._call(self._dequantise, self._slots_run, slots, records, ok, self._cache(cache).writable()._pages_ptr, stream)
+        cache are passed over; the others have to differ from one another. A cache whose planes share memory is
+        refused."""
+        self._call(self._dequantise, self._slots_run, slots, records, ok, self._cache(cache).apart()._pages_ptr, stream)
 
 
 class PagedKvCache:
@@ -298,13 +310,9 @@ class PagedKvCache:
                     step = by[0] * codec.dtype.itemsize
                     for plane in range(codec.planes):
                         bases[plane].append(ptr + plane * step)
-                    if shape is None:
-                        self._overlap = _overlaps(mine, by)
                     mine, by = mine[1:], by[1:]
                 else:
                     bases[k].append(ptr)
-                    if shape is None:
-                        self._overlap = _overlaps(mine, by)
                 if shape is None:
                     shape, strides = mine, by
                 elif mine != shape or by != strides:
@@ -317,11 +325,39 @@ class PagedKvCache:
         if strides[-1] != 1 and dim > 1:
             raise ValueError("kv codec: the values of a vector have to follow one another")
         self.blocks, self.block_size = blocks, size
+        self._starts, self._itemsize, self._within, self._between = bases, codec.dtype.itemsize, None, None
+        self._shape, self._strides = shape, strides
         self._bases = (ctypes.c_void_p * (codec.planes * codec.layers))(*[p for plane in bases for p in plane])
         self._pages = KvPages(ctypes.addressof(self._bases), blocks, size, 0, *strides[:3])
         self._pages_ptr = ctypes.addressof(self._pages)
 
+    def _meet_any(self, distances) -> bool:
+        dims = sorted(((s * self._itemsize, n) for n, s in zip(self._shape, self._strides) if n > 1), reverse=True)
+        return any(_meet(d, dims) for d in distances)
+
     def writable(self) -> "PagedKvCache":
-        if self._overlap:
+        """The cache, if no plane shares memory with itself or with its layer's other plane."""
+        if self._within is None:
+            self._within = self.blocks > 0 and (
+                _overlaps(self._shape, self._strides) or
+                len(self._starts) == 2 and self._meet_any({v - k for k, v in zip(*self._starts)}))
+        if self._within:
             raise ValueError("kv codec: a cache that is written to may not overlap itself")
+        return self
+
+    def apart(self) -> "PagedKvCache":
+        """The cache, if it is writable and no plane shares memory with another layer's either."""
+        self.writable()
+        if self._between is None:
+            starts = sorted(p for plane in self._starts for p in plane)
+            reach = sum(s * (n - 1) for n, s in zip(self._shape, self._strides)) * self._itemsize
+            distances = set()
+            for i, a in enumerate(starts if self.blocks > 0 else ()):
+                for b in starts[i + 1:]:
+                    if b - a > reach:
+                        break
+                    distances.add(b - a)
+            self._between = self._meet_any(distances)
+        if self._between:
+            raise ValueError("kv codec: the layers of a cache that is written to may not overlap one another")
         return self

@@ -306,3 +306,73 @@ def test_split_finds_codes_and_scales(cpu_lib, fmt):
         assert codes.shape == (*lead, *x.shape) and scales.shape == (*lead, 2, 3, 5, 2)
         assert torch.equal((codes.float() * scales[..., None]).half().expand(*lead, *x.shape),
                            kv_ref.read(rec.numpy(), fmt, torch.float16, x.shape).expand(*lead, *x.shape))
+
+
+def reached(fake, itemsize=2):
+    """The bytes of a tensor's elements, from all of its indices."""
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(fake.shape, fake.stride()):
+        at = (at[:, None] + torch.arange(n) * s).flatten()
+    return set((at[:, None] * itemsize + torch.arange(itemsize) + fake.data_ptr()).flatten().tolist())
+
+
+def write_to(codec, layers):
+    codec.dequantise_paged([Fake((R,), U8)], PagedKvCache(codec, layers), [Fake((3,), I64, "cpu")])
+
+
+def test_caches_with_shared_memory_are_not_written_to(codec):
+    """Whichever layer, or pair of planes, shares memory. Slots on the host are refused behind that check: their error
+    says that a cache is taken."""
+    block = 16 * 8 * 64
+    size = 2 * 9 * block * 2
+
+    def joint(k, strides=None):
+        return Fake((2, 9, 16, 8, 64), strides=strides, ptr=(1 << 20) + k * size)
+
+    def pair(a, b):
+        return tuple(Fake(PLANE[1:], ptr=(1 << 20) + p * (size // 2)) for p in (a, b))
+
+    aliasing = {"a later layer's planes": [joint(0), joint(1, (0, block, 512, 64, 1)), joint(2), joint(3)],
+                "planes half a block apart": [joint(0), joint(1), joint(2), joint(3, (block // 2, block, 512, 64, 1))],
+                "a pair of one tensor": [pair(0, 1), pair(2, 3), pair(4, 4), pair(6, 7)],
+                "pairs of one tensor": [pair(k, k) for k in range(4)],
+                "one layer twice": [joint(0), joint(1), joint(2), joint(1)],
+                "keys of one layer, values of another": [pair(0, 1), pair(2, 3), pair(4, 0), pair(6, 7)]}
+    for name, layers in aliasing.items():
+        with pytest.raises(ValueError, match="overlap"):
+            write_to(codec, layers)
+        # such a cache can be read
+        with pytest.raises(ValueError, match="slots"):
+            codec.quantise_paged(PagedKvCache(codec, layers), [Fake((3,), I64, "cpu")], [Fake((R,), U8)])
+    # all layers of a block side by side, [blocks, layers, planes, ...], or of a row, [blocks, block_size, layers, planes, ...]
+    whole = (4 * 2 * block, 512, 64, 1)
+    rows = (16 * 4 * 2 * 512, 4 * 2 * 512, 64, 1)
+    apart = {"in turn": [joint(k) for k in range(4)], "pairs": [pair(2 * k, 2 * k + 1) for k in range(4)],
+             "by block": [Fake(PLANE, strides=(block, *whole), ptr=(1 << 20) + 4 * k * block) for k in range(4)],
+             "by row": [Fake(PLANE, strides=(512, *rows), ptr=(1 << 20) + 4 * k * 512) for k in range(4)]}
+    for name, layers in apart.items():
+        with pytest.raises(ValueError, match="slots"):
+            write_to(codec, layers)
+    writable = PagedKvCache(codec, apart["in turn"])
+    assert writable.writable() is writable
+    for name in ("a later layer's planes", "planes half a block apart", "a pair of one tensor"):
+        with pytest.raises(ValueError, match="overlap"):
+            PagedKvCache(codec, aliasing[name]).writable()
+
+
+def test_shared_memory_is_what_the_indices_say(cpu_lib):
+    """Two layers at every distance, of tensors with and without gaps between vectors, rows and blocks, against the sets of
+    their bytes."""
+    codec = KvCodec(cpu_lib, "int8", torch.bfloat16, planes=1, layers=2, heads=2, head_dim=3)
+    seen = set()
+    for strides in ((12, 6, 3, 1), (24, 6, 3, 1), (40, 14, 4, 1), (30, 3, 9, 1), (100, 40, 16, 1)):
+        first = Fake((3, 2, 2, 3), strides=strides, ptr=1 << 20)
+        mine = reached(first)
+        for elements in range(0, 300):
+            second = Fake((3, 2, 2, 3), strides=strides, ptr=(1 << 20) + 2 * elements)
+            meet = bool(mine & reached(second))
+            seen.add(meet)
+            for layers in ([first, second], [second, first]):
+                with pytest.raises(ValueError, match="overlap" if meet else "slots"):
+                    codec.dequantise_paged([Fake((64,), U8)], PagedKvCache(codec, layers), [Fake((1,), I64, "cpu")])
+    assert seen == {True, False}
