@@ -42,7 +42,7 @@ from lmcache.v1.distributed.serde.factory import register_serde_factory
 from lmcache.v1.distributed.serde.key_provider import HkdfKeyProvider
 
 from .gpu_aesgcm import FRAME_OVERHEAD, GpuAes128GcmKey, GpuAesGcmLibrary
-from .kv_codec import DTYPES, FORMATS, KvCodec, record_size
+from .kv_codec import DTYPES, FORMATS, HEADER_BYTES, KvCodec, record_size
 
 HKDF_INFO_PREFIX = b"lmcache-l2-aesgcm-v1"
 SERDE_TYPE = "gpu_aesgcm"
@@ -196,6 +196,13 @@ class GpuSerdeContext:
             codec.quantise(sources, into, stream=stream)
         return records
 
+    def forget(self, records) -> None:
+        """Clear the headers of record buffers on the current stream, before frames are opened into them: memory that a
+        rejected descriptor leaves unwritten may hold an earlier record, which must not pass for this object's."""
+        import torch
+
+        torch._foreach_zero_([r[:HEADER_BYTES] for r in records])
+
     def dequantise(self, records, objs, stream):
         """Read device records back into objects on `stream` (the current one); the verdicts as a device tensor."""
         import torch
@@ -290,6 +297,8 @@ class GpuAesGcmDeserializer(Deserializer):
             frame_d = src_t if src_t.is_cuda else src_t[:frame_len].to(dev, non_blocking=True)
             out_d = dst_t if direct else torch.empty(max(plaintext_len, 1), dtype=torch.uint8, device=dev)
             auth = torch.zeros(1, dtype=torch.int32, device=dev)
+            if ctx.kv_format is not None:
+                ctx.forget([out_d])
             gkey.open_async(src_ptr=frame_d.data_ptr(), frame_len=frame_len, dst_ptr=out_d.data_ptr(),
                             plaintext_len=plaintext_len, auth_ok_ptr=auth.data_ptr(), stream_ptr=stream.cuda_stream)
             if ctx.kv_format is not None:
@@ -413,6 +422,8 @@ class GpuAesGcmSerdeProcessor(AsyncSerdeProcessor):
                     keep += [frame_d, out_d]
                     if ctx.kv_format is None and P and not dst_t.is_cuda:
                         copies.append((dst_t, out_d, P))
+                if ctx.kv_format is not None:
+                    ctx.forget(records)
                 batch = ctx.batch(len(entries))
                 batch.open(handle, entries, stream)
                 ok_h = None
