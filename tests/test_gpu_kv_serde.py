@@ -89,6 +89,18 @@ def test_refused_configurations_and_objects(tmp_path):
         ser.serialize(DevObj(torch.zeros(4, 64, dtype=torch.bfloat16)), Buf(16), KEY)        # destination too small
 
 
+def test_a_short_frames_object_is_zeroed():
+    """A frame that cannot hold the object's record is refused before any device access, and a host object is zeroed."""
+    de = gpu_serde.GpuAesGcmDeserializer(gpu_serde.GpuSerdeContext(key_provider=None, kv_format="int8"))
+    out = torch.full((4, 64), 5.0, dtype=torch.bfloat16)
+    size = kv_ref.record_bytes("int8", 64, 4)[1] + 29
+    for n in (0, 28, size - 1):
+        out.fill_(5)
+        with pytest.raises(ValueError, match="malformed"):
+            de.deserialize(Buf(n), DevObj(out), KEY)
+        assert not out.any()
+
+
 # ------------------------------------------------------------ GPU
 
 @pytest.mark.gpu
@@ -285,3 +297,43 @@ def test_an_object_that_is_not_opened_reads_as_zeros(key_path, where, monkeypatc
             assert same(outs[k], as_read(xs[k], "int8"))
     finally:
         proc.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+def test_frames_of_other_lengths_leave_zeros(key_path, where):
+    """Another format's frame, shorter or longer than the reader's, and a frame of whole bytes: refused, one or several at
+    once, and the objects are zeros afterwards."""
+    x = kv((2, 4, 64, 8, 64))
+    names = ("int8", "mxfp4", None)
+    procs = {f: processor("gpu", key_path, **({} if f is None else {"kv_format": f})) for f in names}
+    try:
+        frames = {}
+        for f in names:
+            frames[f] = Buf(procs[f].estimate_serialized_size(MemoryLayoutDesc([x.shape], [x.dtype])))
+            assert run_ser(procs[f], DevObj(x.cuda()), frames[f]) is True
+        cut = Buf(len(frames["int8"].bytes()) - 1)
+        ctypes.memmove(cut.address, frames["int8"].address, len(cut.bytes()))
+        for reader, frame, error in (("int8", frames["mxfp4"], ValueError), ("int8", cut, ValueError), ("int8", Buf(3), ValueError),
+                                     ("mxfp4", frames["int8"], gpu_serde.InvalidTag),
+                                     ("int8", frames[None], gpu_serde.InvalidTag), ("mxfp4", frames[None], gpu_serde.InvalidTag)):
+            def out():
+                return torch.full(x.shape, 5.0, dtype=x.dtype, device=where)
+
+            o = out()
+            assert run_de(procs[reader], frame, DevObj(o)) is False and not o.any()
+            o = out()
+            with pytest.raises(error):
+                procs[reader].deserializer.deserialize(frame, DevObj(o), KEY)
+            assert not o.any()
+            # among frames that are its own, of the same and of another tenant: the whole task fails, and none of its
+            # objects keeps what it held before
+            o = [out() for _ in range(3)]
+            assert run_de_many(procs[reader], [frames[reader], frame, frames[reader]], [DevObj(t) for t in o],
+                               [KEY, KEY, OTHER_TENANT]) is False
+            assert not o[1].any()
+            if error is not ValueError:
+                assert same(o[0], as_read(x, reader)) and not o[2].any()
+    finally:
+        for p in procs.values():
+            p.close()
