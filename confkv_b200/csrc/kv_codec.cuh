@@ -511,19 +511,20 @@ struct Int8ByFactor {
     }
 };
 
-// The exact quotient, rounded to a whole number by adding 1.5 2^23 (2^52) or to e4m3.
+// The exact quotient, rounded to a whole number by adding 1.5 2^23 (2^52) or to e4m3: Divider's steps with -t, -c and
+// -y, which keep the sign of a zero.
 template <int FMT>
 struct ByQuotient {
-    Pair c, nb, y;
+    Pair nc, b, ny;
     __device__ __forceinline__ explicit ByQuotient(const Divider<float>& d)
-        : c(make_pair(d.c, d.c)), nb(make_pair(-d.b, -d.b)), y(make_pair(d.y, d.y))
+        : nc(make_pair(-d.c, -d.c)), b(make_pair(d.b, d.b)), ny(make_pair(-d.y, -d.y))
     {
     }
     __device__ __forceinline__ uint32_t codes(float2 x) const
     {
-        const Pair t = mul(make_pair(x.x, x.y), c);
-        const Pair q0 = mul(t, y);
-        const Pair q = fused(fused(nb, q0, t), y, q0);
+        const Pair nt = mul(make_pair(x.x, x.y), nc);
+        const Pair q0 = mul(nt, ny);
+        const Pair q = fused(fused(b, q0, nt), ny, q0);
         if constexpr (FMT == kInt8) {
             const float2 f = halves(add(q, make_pair(kWhole, kWhole)));
             return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x0040);

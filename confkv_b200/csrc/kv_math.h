@@ -49,6 +49,9 @@ constexpr uint32_t kNan = 0x7fffffffu;
 // is a whole number T < 2^18 and b a whole number B < 2^11, times powers of two, a border a whole number
 // M < 2^8 times one, and T 2^i and M B (or T and M B 2^i) differ by a whole number. float32 caches (T < 2^31,
 // B < 2^24, so 2^-32) do the same in double.
+//
+// Both products of the correction are taken with their signs turned, q = q0 + (b q0 - t)(-y): where x is a zero the residual is +0,
+// +0 (-y) = -0, and q0 - 0 is q0 with the sign of x; with t - b q0 it would be q0 + 0, which is +0 for either zero.
 template <class F>
 struct Divider {
     F c, b, y;
@@ -56,8 +59,8 @@ struct Divider {
     {
         const F t = static_cast<F>(x) * c;
         const F q0 = t * y;
-        const F r = fused(-b, q0, t);
-        return fused(r, y, q0);
+        const F r = fused(b, q0, -t);
+        return fused(r, -y, q0);
     }
 };
 

@@ -15,7 +15,8 @@
  * The quotient is not rounded before the code is. s is a float of the vector (in INT8 and FP8 at most
  * FLT_MAX / 127 and FLT_MAX / 448, rounded down, so that no code times s overflows); 2^e is a byte
  * e + 127 of the block. A value read back is code * s rounded to float and then to the object's type
- * (code * 2^e is exact in float). Zero vectors have codes and scale 0. A vector (block) with a
+ * (code * 2^e is exact in float). FP8 and MXFP4 codes of zero have the sign of their x, a zero or a value that
+ * rounds to one; INT8 has one zero. The scale of a zero vector is 0 (its block's byte 0). A vector (block) with a
  * value that is not finite has codes 0 and scale NaN (byte 255): all of it reads back as NaN.
  *
  * Record, R = lmcache_gpu_kv_record_size bytes, little endian; V = planes * layers * tokens * heads

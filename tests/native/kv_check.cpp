@@ -1,6 +1,7 @@
 // Host build of the KV codec's arithmetic (csrc/kv_math.h, kv_layout.h) for tests/test_kv_layout.py.
 #include <cstdint>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "kv_math.h"
 
@@ -105,7 +106,31 @@ static uint64_t check_int8(int bits, int max_gap, int exponent, uint64_t* slow)
     return bad;
 }
 
+// Zeros of both signs, and values so small that their quotients are zero: the quotients that do not have their sign.
+template <class F>
+static uint64_t check_signs(int format, int exponent)
+{
+    uint64_t bad = 0;
+    const float top = format == kv::kInt8 ? 127.0f : 448.0f, tiny = kv::bits_float(1);
+    for (uint32_t b = 0; b < 256; ++b) {
+        const float amax = b == 0 ? 0.0f : std::ldexp(static_cast<float>(b), exponent);
+        const kv::Divider<F> div = kv::make_divider<F>(amax, top);
+        for (float x : {0.0f, tiny, std::ldexp(1.0f, -140), std::ldexp(1.0f, -126)}) {
+            if (x <= amax) {
+                bad += std::signbit(div.quotient(x)) || !std::signbit(div.quotient(-x));
+                bad += std::signbit(kv::for_rounding(div.quotient(x))) || !std::signbit(kv::for_rounding(div.quotient(-x)));
+            }
+        }
+    }
+    return bad;
+}
+
 extern "C" {
+
+uint64_t kv_check_signs(int format, int exponent, int wide)
+{
+    return wide != 0 ? check_signs<double>(format, exponent) : check_signs<float>(format, exponent);
+}
 
 uint64_t kv_check_int8(int bits, int max_gap, int exponent, uint64_t* slow)
 {

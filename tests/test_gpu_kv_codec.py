@@ -687,3 +687,32 @@ def test_codec_and_seal_in_one_graph(make, gpu_lib):
             assert_record(opened, host, "mxfp4")
             assert torch.equal(bits(out), bits(kv_ref.read(opened.cpu().numpy(), "mxfp4", torch.bfloat16, host.shape)))
         del g
+
+
+# every kernel's way to a code: granules of 16, 8, 4, 2 and 1 values, whole warps, a lane, several vectors a warp
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [1, 16, 33, 36, 40, 66, 100, 127, 128, 320, 514, 1030, 2576])
+def test_zeros_keep_their_sign(make, fmt, dtype, d):
+    """Records equal to the reference's in every byte: zeros of both signs, values that round to zero, vectors of nothing
+    else."""
+    t = DTYPES[dtype]
+    x = values((1, 2, 8, 2, d), t, seed=d)
+    flat = x.view(-1, d)
+    flat[:, d // 2] = -0.0
+    flat[8:16] *= torch.where(torch.arange(d) % 3 == 1, 2.0 ** -12, 1.0).to(t)      # below half of the least code
+    flat[16] = -0.0
+    flat[17] = 0.0
+    flat[18] = torch.where(torch.arange(d) % 2 == 0, 0.0, -0.0).to(t)
+    flat[19] = -torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    flat[20, 0], flat[20, 1:] = torch.finfo(t).max, -torch.finfo(t).smallest_normal
+    codec = make(fmt, dtype, 1, 2, 2, d)
+    rec = torch.full((codec.record_bytes(8),), GUARD, dtype=torch.uint8, device="cuda")
+    codec.quantise(x.cuda(), rec)
+    want = kv_ref.record(x, fmt)
+    got = rec.cpu().numpy()
+    assert np.array_equal(got, want), np.nonzero(got != want)[0][:8]
+    if fmt != "int8":
+        out = torch.empty_like(x, device="cuda")
+        codec.dequantise(rec, out)
+        assert bool((torch.signbit(out.cpu()) == torch.signbit(x)).all())

@@ -147,3 +147,12 @@ def test_reference_errors_are_within_half_a_step(fmt, dtype):
         a = x.abs().amax(-1, keepdim=True)
         bound = a / 254 if fmt == "int8" else torch.maximum(x.abs() / 16, a / 448 * 2.0 ** -10)
     assert bool((err <= bound).all()), float((err - bound).max())
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("wide", [0, 1])
+@pytest.mark.parametrize("exponent", [-140, -133, -7, 0, 100, 119])
+def test_quotients_of_zero_keep_their_sign(lib, fmt, wide, exponent):
+    lib.kv_check_signs.argtypes = [ctypes.c_int] * 3
+    lib.kv_check_signs.restype = ctypes.c_uint64
+    assert lib.kv_check_signs(fmt, exponent, wide) == 0
