@@ -44,7 +44,7 @@ from . import hostmem, multigpu, workloads
 from .batch import DeviceBatch
 from .clocks import ClockSampler
 from .gpu_aesgcm import GpuAes128GcmKey, GpuAesGcmLibrary
-from .kv_codec import FORMATS, KvCodec
+from .kv_codec import FORMATS, MX_BLOCK, KvCodec
 
 ALIGN = 256
 INNER = 4  # calls per timed iteration
@@ -188,6 +188,27 @@ class RankWork:
         return all(torch.equal(self.out[a:a + n], self.plain[a:a + n]) for a, n in zip(self.pt_off, self.lens))
 
 
+def within_format(x: torch.Tensor, y: torch.Tensor, fmt: str) -> bool:
+    """Whether y is what a record of x [..., head_dim] may read back as. A code is off by half a step: A / 254 (int8), 2^-4
+    of the value or half of the least step 2^-9 of A / 448 (fp8), a quarter of the value, what saturates above 6 included, or of
+    the block's unit, A / 4 or 2^-127 at most (mxfp4). To that come the roundings to float of the scale and of its
+    product, 2^-24 each (2^-150 below the normal floats, and 448 times as much at the largest code), and the one to the
+    type. A vector (block) with a value that is not finite reads back as NaN."""
+    info = torch.finfo(x.dtype)
+    x, y = x.double(), y.double()
+    v = x.abs()
+    if fmt == "mxfp4":
+        d = x.shape[-1]
+        blocks = torch.nn.functional.pad(v, (0, -d % MX_BLOCK)).unflatten(-1, (-1, MX_BLOCK))
+        a = blocks.amax(-1).repeat_interleave(MX_BLOCK, -1)[..., :d]
+        step = torch.maximum(v, (a / 4).clamp(min=2.0 ** -127)) / 4
+    else:
+        a = v.amax(-1, keepdim=True)
+        step = a / 254 if fmt == "int8" else torch.maximum(v / 16, a / 448 * 2.0 ** -10)
+    more = y.abs() * (info.eps / 2 + 2.0 ** -22) + info.smallest_normal * info.eps + 2.0 ** -141
+    return bool(torch.where(torch.isfinite(a), (x - y).abs() <= step + more, torch.isnan(y)).all())
+
+
 class QuantisedWork(RankWork):
     """This rank's KV objects [n, planes, layers, tokens, heads, head_dim] sealed as records: one quantise call
     ahead of the seals, one dequantise call behind the opens."""
@@ -229,10 +250,13 @@ class QuantisedWork(RankWork):
         self.ok.zero_()
 
     def round_trip_ok(self) -> bool:
-        """The opened records are the sealed ones, and what was read back is what they stand for."""
+        """The opened records are the sealed ones, what was read back is what they stand for, and that is as near to the
+        source objects as the format goes."""
         again = torch.empty_like(self.restored)
         self.codec.dequantise(self.records, again)
-        return super().round_trip_ok() and bool((self.ok == 1).all()) and torch.equal(again, self.restored)
+        return (super().round_trip_ok() and bool((self.ok == 1).all()) and
+                torch.equal(again.view(torch.uint8), self.restored.view(torch.uint8)) and
+                all(within_format(x, y, self.codec.format) for x, y in zip(self.objects, self.restored)))
 
 
 def barrier(world, dev):
