@@ -716,3 +716,24 @@ def test_zeros_keep_their_sign(make, fmt, dtype, d):
         out = torch.empty_like(x, device="cuda")
         codec.dequantise(rec, out)
         assert bool((torch.signbit(out.cpu()) == torch.signbit(x)).all())
+
+
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+def test_neighbours_of_objects_of_unequal_alignment(make, fmt):
+    """What lies before and behind each object of a call, aligned or not, keeps its values."""
+    d = 64
+    codec = make(fmt, "bf16", 1, 2, 3, d)
+    xs = [values((1, 2, 20 + k, 3, d), torch.bfloat16, seed=k) for k in range(9)]
+    raws, outs, recs, starts = [], [], [], [(0, 1, 8, 16)[k % 4] for k in range(9)]
+    for x, at in zip(xs, starts):
+        raws.append(torch.full((x.numel() + 64,), 2.0, dtype=torch.bfloat16, device="cuda"))
+        outs.append(raws[-1][at:at + x.numel()].view(x.shape))
+        recs.append(torch.from_numpy(kv_ref.record(x, fmt)).cuda())
+    codec.dequantise(recs, outs)
+    for x, r, raw, o, at in zip(xs, recs, raws, outs, starts):
+        assert torch.equal(bits(o), bits(kv_ref.read(r.cpu().numpy(), fmt, torch.bfloat16, x.shape)))
+        assert bool((raw[:at] == 2).all()) and bool((raw[at + x.numel():] == 2).all())
+    # and quantising leaves the sources and their neighbours alone
+    before = [raw.clone() for raw in raws]
+    codec.quantise(outs, recs)
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(before, raws))
