@@ -290,7 +290,8 @@ class PagedKvCache:
 
     def __init__(self, codec: KvCodec, layers):
         self.signature = codec.signature
-        self.layers = list(layers)
+        # pairs as tuples of their own: the addresses below are good only while their tensors live
+        self.layers = [layer if hasattr(layer, "data_ptr") else tuple(layer) for layer in layers]
         if len(self.layers) != codec.layers or codec.layers * codec.planes > MAX_BASES:
             raise ValueError(f"kv codec: a paged cache has the codec's {codec.layers} layers, and {MAX_BASES} planes at most")
         # every plane is [blocks, block_size, heads, head_dim], all of one shape and with one set of strides
@@ -298,7 +299,7 @@ class PagedKvCache:
         bases = [[] for _ in range(codec.planes)]
         for layer in self.layers:
             joint = hasattr(layer, "data_ptr")              # one tensor a layer
-            parts = (layer,) if joint else tuple(layer)     # or keys and values apart
+            parts = (layer,) if joint else layer            # or keys and values apart
             joint = joint and len(layer.shape) == 5
             if (layer.shape[0] if joint else len(parts)) != codec.planes:
                 raise ValueError(f"kv codec: a layer has {codec.planes} planes")

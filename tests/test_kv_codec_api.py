@@ -376,3 +376,21 @@ def test_shared_memory_is_what_the_indices_say(cpu_lib):
                 with pytest.raises(ValueError, match="overlap" if meet else "slots"):
                     codec.dequantise_paged([Fake((64,), U8)], PagedKvCache(codec, layers), [Fake((1,), I64, "cpu")])
     assert seen == {True, False}
+
+
+def test_a_cache_keeps_its_tensors(codec):
+    """Whatever its caller does with the lists that it was made of."""
+    import gc
+    import weakref
+
+    layers = [[Fake(PLANE[1:], ptr=(1 << 20) + (2 * k << 20)), Fake(PLANE[1:], ptr=(1 << 20) + (2 * k + 1 << 20))] for k in range(4)]
+    held = [weakref.ref(t) for pair in layers for t in pair]
+    cache = PagedKvCache(codec, layers)
+    for pair in layers:
+        pair.clear()
+    layers.clear()
+    gc.collect()
+    assert all(r() is not None for r in held)
+    del cache
+    gc.collect()
+    assert all(r() is None for r in held)
