@@ -222,8 +222,8 @@ class GpuSerdeContext:
         for k, (record, obj) in enumerate(zip(records, objs)):
             t = _kv_tensor(obj)
             codec, shape = self.codec(t)
-            out = t if t.is_cuda else torch.empty(t.shape, dtype=t.dtype, device=dev)
-            if not t.is_cuda:
+            out = t if t.device == dev else torch.empty(t.shape, dtype=t.dtype, device=dev)
+            if out is not t:                    # on the host, or on another device
                 copies.append((t, out))
             sources, into, oks = calls[codec]
             sources.append(record)

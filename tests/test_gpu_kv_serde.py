@@ -337,3 +337,48 @@ def test_frames_of_other_lengths_leave_zeros(key_path, where):
     finally:
         for p in procs.values():
             p.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_objects_on_another_device(key_path):
+    """Objects of another GPU than the backend's are copied to it and back, one or several at once."""
+    xs = [kv((2, 4, 33, 8, 64), seed=k) for k in range(3)]
+    proc = processor("gpu", key_path, kv_format="int8", device=0)
+    try:
+        frames = [Buf(proc.estimate_serialized_size(MemoryLayoutDesc([x.shape], [x.dtype]))) for x in xs]
+        srcs = [DevObj(x.to("cuda:1")) for x in xs]
+        torch.cuda.synchronize(1)
+        assert run_ser_many(proc, srcs, frames, [KEY] * 3) is True and run_ser(proc, srcs[0], frames[0]) is True
+        outs = [torch.full(x.shape, 5.0, dtype=x.dtype, device="cuda:1") for x in xs]
+        torch.cuda.synchronize(1)
+        assert run_de_many(proc, frames, [DevObj(o) for o in outs], [KEY] * 3) is True
+        for x, o in zip(xs, outs):
+            assert same(o, as_read(x, "int8"))
+        outs[0].fill_(5)
+        torch.cuda.synchronize(1)
+        assert run_de(proc, frames[0], DevObj(outs[0])) is True and same(outs[0], as_read(xs[0], "int8"))
+    finally:
+        proc.close()
+
+
+@pytest.mark.gpu
+def test_objects_on_the_backends_device_are_read_back_in_place(key_path, monkeypatch):
+    """And those on the host through a copy."""
+    x = kv((2, 4, 33, 8, 64))
+    proc = processor("gpu", key_path, kv_format="int8")
+    seen = []
+    try:
+        frame = Buf(proc.estimate_serialized_size(MemoryLayoutDesc([x.shape], [x.dtype])))
+        assert run_ser(proc, DevObj(x.cuda()), frame) is True
+        from confkv_b200.kv_codec import KvCodec
+
+        call = KvCodec.dequantise
+        monkeypatch.setattr(KvCodec, "dequantise", lambda self, records, objects, **more: (
+            seen.extend(o.data_ptr() for o in objects), call(self, records, objects, **more))[1])
+        for where in ("cuda", "cpu"):
+            out = torch.full(x.shape, 5.0, dtype=x.dtype, device=where)
+            assert run_de(proc, frame, DevObj(out)) is True and same(out, as_read(x, "int8"))
+            assert (seen.pop() == out.data_ptr()) == (where == "cuda") and not seen
+    finally:
+        proc.close()
