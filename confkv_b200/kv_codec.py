@@ -261,12 +261,13 @@ class KvCodec:
     def quantise(self, objects, records, stream: torch.cuda.Stream | None = None) -> None:
         """Write the records of objects. `objects`: a [planes, layers, tokens, heads, head_dim] tensor of any
         strides with contiguous vectors, a row of them [n, ...], or a sequence of either; `records`: for each a uint8
-        tensor [>= R], or [n, >= R]."""
+        tensor [>= R], or [n, >= R]; they may share memory with nothing else in the call."""
         self._call(self._quantise, self._read_run, objects, records, None, None, stream)
 
     def dequantise(self, records, objects, ok=None, stream: torch.cuda.Stream | None = None) -> None:
         """Read records back into objects. `ok`: for each tensor of objects an int32 tensor of one verdict an object:
-        1, or 0 where the record is not one of this codec's for so many tokens; such an object is zero-filled."""
+        1, or 0 where the record is not one of this codec's for so many tokens; such an object is zero-filled. The objects of a
+        call may not share memory."""
         self._call(self._dequantise, self._written_run, objects, records, ok, None, stream)
 
     def quantise_paged(self, cache: "PagedKvCache", slots, records, stream: torch.cuda.Stream | None = None) -> None:
@@ -277,7 +278,8 @@ class KvCodec:
     def dequantise_paged(self, records, cache: "PagedKvCache", slots, ok=None,
                          stream: torch.cuda.Stream | None = None) -> None:
         """Read records back into slots of a paged cache, and write to no other slot. Slots below 0 or outside the
-        cache are passed over; the others have to differ from one another. A cache whose planes share memory is
+        cache are passed over; the others have to differ from one another (of a slot named twice each value is one of the two
+        tokens'). A cache whose planes share memory is
         refused."""
         self._call(self._dequantise, self._slots_run, slots, records, ok, self._cache(cache).apart()._pages_ptr, stream)
 

@@ -107,7 +107,10 @@ int lmcache_gpu_kv_quantise_async(const lmcache_gpu_kv_layout* layout, const lmc
  *
  * Paged: slots below 0 or outside the cache are passed over, and no other slot than the named ones is
  * written to. The slots of one call have to differ from one another: of a slot named twice, each
- * vector is either of the two.
+ * value is one of the two tokens', and one vector may hold values of both.
+ *
+ * Destinations (objects, or the planes behind `bases`) must not share memory with one another or with any record:
+ * what is written twice is undefined.
  */
 int lmcache_gpu_kv_dequantise_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages,
                                     const lmcache_gpu_kv_run* runs, size_t count, int device, void* stream);

@@ -737,3 +737,28 @@ def test_neighbours_of_objects_of_unequal_alignment(make, fmt):
     before = [raw.clone() for raw in raws]
     codec.quantise(outs, recs)
     assert all(torch.equal(bits(a), bits(b)) for a, b in zip(before, raws))
+
+
+@pytest.mark.parametrize("fmt", kv_ref.FORMATS)
+@pytest.mark.parametrize("d", [64, 33, 5000])
+def test_a_slot_named_twice_holds_values_of_either_token(make, fmt, d):
+    """And no other slot changes; named twice on the way out it is two equal tokens."""
+    codec = make(fmt, "bf16", 1, 2, 3, d)
+    _, pool = paged(2, 1, 4, 16, 3, d, torch.bfloat16, "NHD", seed=5)
+    before = pool.clone()
+    cache = PagedKvCache(codec, list(pool.unbind(0)))
+    x = values((1, 2, 40, 3, d), torch.bfloat16, seed=6)
+    rec = torch.from_numpy(kv_ref.record(x, fmt)).cuda()
+    slots = torch.arange(40, device="cuda") // 2 + 7            # pairs of neighbouring tokens
+    codec.dequantise_paged(rec, cache, slots)
+    want = kv_ref.read(rec.cpu().numpy(), fmt, torch.bfloat16, x.shape)
+    got = pool.view(2, 64, 3, d).cpu()
+    here = bits(got[:, 7:27])
+    a, b = (bits(want[0, :, k::2]) for k in (0, 1))
+    assert bool(((here == a) | (here == b)).all())
+    rest = torch.ones(64, dtype=torch.bool)
+    rest[7:27] = False
+    assert torch.equal(bits(got[:, rest]), bits(before.view(2, 64, 3, d).cpu()[:, rest]))
+    out = torch.empty(codec.record_bytes(40), dtype=torch.uint8, device="cuda")
+    codec.quantise_paged(cache, slots, out)
+    assert_record(out, pool.view(2, 64, 3, d)[:, 7:27].repeat_interleave(2, 1).cpu()[None], fmt)
