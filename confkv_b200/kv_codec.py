@@ -350,8 +350,8 @@ class PagedKvCache:
 
     def apart(self) -> "PagedKvCache":
         """The cache, if it is writable and no plane shares memory with another layer's either."""
-        self.writable()
         if self._between is None:
+            self.writable()
             starts = sorted(p for plane in self._starts for p in plane)
             reach = sum(s * (n - 1) for n, s in zip(self._shape, self._strides)) * self._itemsize
             distances = set()
