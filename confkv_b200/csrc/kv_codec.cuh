@@ -9,7 +9,7 @@
 // of objects of whatever sizes, which travel in the kernel's parameters; there is no workspace and there are no atomics.
 //
 // Measured on B200, [2, 32, 256, 8, 128] bfloat16 objects (32 MiB), events, L2 cold (quantise / dequantise):
-//   32 objects, INT8   231 / 236 us  (7.05 / 6.90 TB/s; 234 to 239 / 238 us in a run of seconds)
+//   32 objects, INT8   231 / 236 us  (7.05 / 6.90 TB/s; 234 to 245 / 238 us in a run of seconds)
 //   16 objects, FP8    116 / 120 us  (7.04 / 6.77 TB/s; 127 / 120 us)
 //   16 objects, MXFP4   98 / 102 us  (6.96 / 6.68 TB/s; 108 / 101 us)
 //   1 object, INT8     9.7 / 9.7 us  (5.25 TB/s: the ramp and the tail of 2048 short blocks)
@@ -156,9 +156,11 @@ __device__ __forceinline__ uint32_t warp_max(uint32_t v)
 
 // --------------------------------------------------- one warp a vector
 //
-// For vectors that no group of lanes holds in its registers (above 2560 values, or above 512 to 1024 where they are at
-// addresses that take small loads): the warp goes over the vector twice, the second time out of L1 or L2. 32 chunks
-// to INT8 take 1157 us this way.
+// For vectors that no group of lanes holds in its registers: above 2560 values in granules of 16 (float32: 1536), 2048 in ones
+// of 8 (reading: 1024), 1024 in ones of 4 and 2 (writing MXFP4 in ones of 4: 2048), 512 in single values. The warp goes
+// over an INT8 or FP8 vector twice, the second time out of L1 or L2, and over an MXFP4 one block by block, with loads and stores of single
+// values: 1 GiB of bfloat16 vectors of 4096 to INT8 and back 708 / 585 us (2.3 / 2.8 TB/s), to MXFP4 794 / 847 us; 32 chunks to
+// INT8, for which there are faster ways, 1157 us.
 
 // The header, and the zero bytes behind the codes and behind the scales.
 __device__ __forceinline__ void write_frame_of_record(const Run& r, char* record, uint32_t lane)

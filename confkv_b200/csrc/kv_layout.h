@@ -49,7 +49,7 @@ KV_HD RecordLayout record_layout(int format, uint32_t head_dim, uint64_t vectors
     return r;
 }
 
-// n / d for n < 2^31 and a fixed d >= 1 by one high product: with l = ceil(log2 d) and
+// n / d for n < 2^31 and a fixed d >= 1 by one high product (Granlund and Montgomery's division by an invariant): with l = ceil(log2 d) and
 // m = floor(2^32 (2^l - d) / d) + 1, n / d = (hi(m n) + n) >> l (the sum stays below 2^32).
 struct FastDiv {
     uint32_t d, m, shift;

@@ -43,7 +43,7 @@ constexpr uint32_t kNan = 0x7fffffffu;
 // quotient that is computed must not cross a border between two codes. With 2^-E a power of two near
 // 1 / A, t = x (top 2^-E) is exact (11 + 7 bits at most for 16-bit caches; where t underflows the code is 0
 // anyway), b = A 2^-E is exact, and with y = 1 / b rounded, q0 = t y is within 2^-23 of t / b, of its
-// size. The residual t - b q0 is then added back, q = q0 + (t - b q0) y, which leaves one rounding of q and
+// size. The residual t - b q0 is then added back (Markstein's correction step), q = q0 + (t - b q0) y, which leaves one rounding of q and
 // some 2^-46. A quotient that is a border itself has few bits, so the residual and then q are
 // exact, and the tie goes to even. Any other is at least 2^-19 of its size away from every border: t
 // is a whole number T < 2^18 and b a whole number B < 2^11, times powers of two, a border a whole number

@@ -113,7 +113,7 @@ def read(rec, fmt, dtype, shape):
 
 
 def same_record(got, want, fmt, d, vectors):
-    """Equal bytes, but for the sign of an fp8 code of zero, which the format leaves open."""
+    """Equal bytes, but for the sign of an fp8 code of zero, which a test of its own compares."""
     got, want = np.array(got), np.array(want)
     if fmt == "fp8":
         for r in (got, want):

@@ -2,7 +2,7 @@
 
 Codes, scales and record bytes are the definition's, so records are compared byte for byte, and values
 read back bit for bit (one product in float32 and one rounding to the type on both sides): no tolerance but the sign
-of an fp8 zero, which the format leaves open."""
+of an fp8 zero, which test_zeros_keep_their_sign alone compares."""
 
 import threading
 
