@@ -1,10 +1,11 @@
 """Build the in-tree sm_100a library ``confkv_b200/libgpu_aesgcm.so``.
 
 nvcc compiles the CUDA kernels and C-ABI (gpu_aesgcm.cu: per-object calls;
-batch.cu: batched calls; kv_codec.cu: the KV-cache codec) and the host key
-schedule / GHASH table code in parallel, then links them into the shared
-object that the ctypes bindings load (``include/gpu_aesgcm_api.h``,
-``include/gpu_kv_codec_api.h``). Usage: ``python -m confkv_b200.build [-v]``.
+batch.cu: batched calls; kv_codec.cu: the KV-cache codec; kv_paged.cu: a paged
+cache's requests) and the host key schedule / GHASH table code in parallel, then
+links them into the shared object that the ctypes bindings load
+(``include/gpu_aesgcm_api.h``, ``include/gpu_kv_codec_api.h``,
+``include/gpu_kv_paged_api.h``). Usage: ``python -m confkv_b200.build [-v]``.
 """
 
 from __future__ import annotations
@@ -21,10 +22,11 @@ INCLUDE = ROOT / "include"
 LIB_NAME = "libgpu_aesgcm.so"
 LIB_PATH = PKG / LIB_NAME
 
-SOURCES = [CSRC / "gpu_aesgcm.cu", CSRC / "batch.cu", CSRC / "kv_codec.cu", CSRC / "host_crypto.cpp"]
+SOURCES = [CSRC / "gpu_aesgcm.cu", CSRC / "batch.cu", CSRC / "kv_codec.cu", CSRC / "kv_paged.cu", CSRC / "host_crypto.cpp"]
 HEADERS = [CSRC / "kernels.cuh", CSRC / "clmul.cuh", CSRC / "gh5.cuh", CSRC / "tiles.cuh", CSRC / "batch.cuh", CSRC / "small.cuh", CSRC / "host_common.h",
            CSRC / "host_crypto.h", CSRC / "kv_codec.cuh", CSRC / "kv_layout.h", CSRC / "kv_math.h",
-           INCLUDE / "gpu_aesgcm_api.h", INCLUDE / "gpu_kv_codec_api.h"]
+           CSRC / "kv_values.cuh", CSRC / "kv_paged.h", CSRC / "kv_paged.cuh", CSRC / "kv_attend.cuh",
+           INCLUDE / "gpu_aesgcm_api.h", INCLUDE / "gpu_kv_codec_api.h", INCLUDE / "gpu_kv_paged_api.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -27,6 +27,7 @@
 #include "kernels.cuh"
 #include "kv_layout.h"
 #include "kv_math.h"
+#include "kv_values.cuh"
 
 namespace confkv {
 namespace kv {
@@ -91,22 +92,6 @@ __device__ __forceinline__ char* vector_address(const Args& a, const Run& r, con
 }
 
 // ------------------------------------------------------------------ values
-
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(float x) { return x; }
-
-template <class T>
-__device__ __forceinline__ T from_float(float x)
-{
-    if constexpr (std::is_same_v<T, float>) {
-        return x;
-    } else if constexpr (std::is_same_v<T, __half>) {
-        return __float2half_rn(x);
-    } else {
-        return __float2bfloat16_rn(x);
-    }
-}
 
 // Two e4m3 codes, `lo` in the low byte; ties to even.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi)

@@ -1,0 +1,399 @@
+// The entry points of a paged cache's requests: checks, the kernels' parameters and their launch.
+#include <algorithm>
+#include <cmath>
+
+#include "gpu_kv_paged_api.h"
+#include "host_common.h"
+#include "kv_attend.cuh"
+#include "kv_paged.cuh"
+
+namespace kv = confkv::kv;
+using namespace confkv::host;
+
+namespace {
+
+bool aligned(const void* p, uint64_t to)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
+}
+
+bool array_ok(const void* p, uint64_t to)
+{
+    return p != nullptr && aligned(p, to);
+}
+
+// The largest power of two up to 16 that divides all that `bits` gathers.
+uint64_t alignment_of(uint64_t bits)
+{
+    bits |= 16;
+    return bits & (~bits + 1);
+}
+
+// cudaLaunchKernelEx with programmatic stream serialization, as launch_pdl, for grids of two dimensions and without a key
+// schedule's shared layout.
+template <class A, class... More>
+cudaError_t launch(void (*kernel)(A, More...), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t s, const A& a, More... more)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, more...);
+}
+
+// ------------------------------------------------------------------ block tables and slot maps
+
+struct Range {
+    uintptr_t begin, end;
+};
+
+Range range_of(const void* p, uint64_t bytes)
+{
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+    return Range{b, p != nullptr ? b + bytes : b};
+}
+
+bool meet(const Range& a, const Range& b)
+{
+    return a.begin < a.end && b.begin < b.end && a.begin < b.end && b.begin < a.end;
+}
+
+bool tables_ok(const lmcache_gpu_kv_tables& t)
+{
+    if (t.requests >= kv::kMaxRequests || t.width >= kv::kMost || t.ring >= kv::kMost || t.block_size == 0 ||
+        uint64_t{t.blocks} * t.block_size > kv::kMost || t.block_size > kv::kMost || t.table_stride < 0) {
+        return false;
+    }
+    if (!array_ok(t.cursor, 4) || !array_ok(t.cursor_after, 4) || (t.ring != 0 && !array_ok(t.free, 4)) ||
+        !aligned(t.slots, 8) || !aligned(t.starts, 8) || (t.slots != nullptr && t.capacity >= kv::kMost) ||
+        (t.slots == nullptr && t.starts != nullptr)) {
+        return false;
+    }
+    const uint64_t n = t.requests;
+    if (n != 0 && (!array_ok(t.held, 4) || !array_ok(t.lengths, 4) || !array_ok(t.kept, 4) ||
+                   (t.width != 0 && !array_ok(t.tables, 4)) || (n > 1 && t.table_stride < t.width))) {
+        return false;
+    }
+    if (t.table_stride > (int64_t{1} << 36)) {   // 2^24 rows of it stay below 2^63 bytes
+        return false;
+    }
+    const Range out[] = {range_of(t.kept, 4 * n),
+                         range_of(t.cursor_after, 8),
+                         range_of(t.slots, 8 * t.capacity),
+                         range_of(t.starts, 8 * (n + 1)),
+                         range_of(t.free, 4 * uint64_t{t.ring}),
+                         range_of(n != 0 && t.width != 0 ? t.tables : nullptr, 4 * ((n != 0 ? n - 1 : 0) * static_cast<uint64_t>(t.table_stride) + t.width))};
+    const Range in[] = {range_of(t.held, 4 * n), range_of(t.lengths, 4 * n), range_of(t.cursor, 8)};
+    for (size_t i = 0; i < std::size(out); ++i) {
+        for (size_t k = i + 1; k < std::size(out); ++k) {
+            if (meet(out[i], out[k])) {
+                return false;
+            }
+        }
+        for (const Range& r : in) {
+            if (meet(out[i], r)) {
+                return false;
+            }
+        }
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------ a layer of the cache
+
+bool layer_ok(const lmcache_gpu_kv_layout* l, const lmcache_gpu_kv_pages* p, uint32_t layer)
+{
+    if (l == nullptr || p == nullptr || l->dtype < kv::kBf16 || l->dtype > kv::kFp32 || l->planes < 1 || l->planes > 2 ||
+        l->layers < 1 || l->layers > 65535 || l->heads < 1 || l->heads > 65535 || l->head_dim < 1 || l->head_dim > 65535 ||
+        layer >= l->layers) {
+        return false;
+    }
+    if (p->bases == nullptr || p->block_size == 0 || p->blocks > kv::kMaxTokens ||
+        p->blocks * p->block_size > kv::kMaxTokens || p->block_size > kv::kMaxTokens || p->block_stride < 0 || p->row_stride < 0 || p->head_stride < 0) {
+        return false;
+    }
+    for (uint32_t plane = 0; plane < l->planes; ++plane) {
+        const void* base = p->bases[plane * l->layers + layer];
+        if ((base == nullptr && p->blocks != 0) || !aligned(base, kv::element_bytes(l->dtype))) {
+            return false;
+        }
+    }
+    return true;
+}
+
+// The bits of all addresses of the layer's vectors, in bytes.
+uint64_t layer_bits(const lmcache_gpu_kv_layout& l, const lmcache_gpu_kv_pages& p, uint32_t layer, int64_t element)
+{
+    uint64_t bits = 0;
+    for (uint32_t plane = 0; plane < l.planes; ++plane) {
+        bits |= reinterpret_cast<uintptr_t>(p.bases[plane * l.layers + layer]);
+    }
+    bits |= p.blocks > 1 ? p.block_stride * element : 0;
+    bits |= p.block_size > 1 ? p.row_stride * element : 0;
+    bits |= l.heads > 1 ? p.head_stride * element : 0;
+    return bits;
+}
+
+template <class G>
+constexpr auto append_of = kv::append_kernel<G>;
+
+// ------------------------------------------------------------------ attention
+
+using AttendKernel = void (*)(const kv::AttendArgs);
+using JoinKernel = void (*)(const kv::AttendArgs, uint32_t);
+
+// How a launch does its work.
+struct AttendPlan {
+    AttendKernel kernel;
+    JoinKernel join;
+    uint32_t heads;             // query heads of a row
+    uint32_t workers;
+};
+
+constexpr uint32_t kSms = 148;
+
+template <class T>
+AttendPlan any_plan(uint32_t head_dim, uint32_t group)
+{
+    AttendPlan p{};
+    p.join = kv::join_kernel<T>;
+    p.workers = 4 * kSms;
+    if (head_dim <= 64) {
+        p.heads = group > 1 ? 8 : 1;
+        p.kernel = group > 1 ? kv::attend_any_kernel<T, 2, 8, 4> : kv::attend_any_kernel<T, 2, 1, 8>;
+    } else if (head_dim <= 128) {
+        p.heads = group > 1 ? 8 : 1;
+        p.kernel = group > 1 ? kv::attend_any_kernel<T, 4, 8, 4> : kv::attend_any_kernel<T, 4, 1, 8>;
+    } else if (head_dim <= 256) {
+        p.heads = group > 1 ? 4 : 1;
+        p.kernel = group > 1 ? kv::attend_any_kernel<T, 8, 4, 4> : kv::attend_any_kernel<T, 8, 1, 4>;
+    } else {
+        p.heads = 1;
+        p.kernel = kv::attend_any_kernel<T, 32, 1, 1>;
+    }
+    return p;
+}
+
+AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
+{
+    return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group)
+           : l.dtype == kv::kFp16 ? any_plan<__half>(l.head_dim, group)
+                                  : any_plan<float>(l.head_dim, group);
+}
+
+// The parts of the workspace, in bytes behind its start.
+struct Workspace {
+    uint64_t sums, partial, size;
+};
+
+Workspace workspace_of(const AttendPlan& p, uint32_t value_dim)
+{
+    Workspace w{};
+    const uint64_t places = uint64_t{2} * p.workers * p.heads;
+    w.sums = uint64_t{p.workers} * sizeof(int4);
+    w.partial = w.sums + places * sizeof(float2);
+    w.size = w.partial + places * ((value_dim + 3) / 4 * 4) * sizeof(float);
+    return w;
+}
+
+bool heads_ok(const lmcache_gpu_kv_layout& l, uint32_t query_heads, uint32_t value_dim)
+{
+    return l.heads >= 1 && l.heads <= 65535 && query_heads >= 1 && query_heads <= 65535 && query_heads % l.heads == 0 &&
+           l.head_dim >= 1 && l.head_dim <= 1024 && value_dim >= 1 && value_dim <= l.head_dim && l.planes >= 1 &&
+           l.planes <= 2 && (l.planes == 1 || value_dim == l.head_dim) && l.dtype >= kv::kBf16 && l.dtype <= kv::kFp32;
+}
+
+}  // namespace
+
+extern "C" int lmcache_gpu_kv_resize_async(const lmcache_gpu_kv_tables* tables, int device, void* stream)
+{
+    if (tables == nullptr || device < 0 || !tables_ok(*tables)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    const lmcache_gpu_kv_tables& t = *tables;
+    DeviceGuard guard(device);
+    if (!guard.ok()) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
+    kv::ResizeArgs a{};
+    a.tables = t.tables;
+    a.table_stride = t.table_stride;
+    a.held = t.held;
+    a.lengths = t.lengths;
+    a.free = t.free;
+    a.cursor = t.cursor;
+    a.kept = t.kept;
+    a.cursor_after = t.cursor_after;
+    a.slots = t.slots;
+    a.starts = t.starts;
+    a.capacity = t.slots != nullptr ? static_cast<uint32_t>(t.capacity) : kv::kMost;
+    a.requests = t.requests;
+    a.limit = kv::row_limit(t.width, t.block_size);
+    a.blocks = t.blocks;
+    a.ring = t.ring;
+    a.per = (t.requests + kv::kResizeThreads - 1) / kv::kResizeThreads;
+    a.by_block = kv::make_fast_div(t.block_size);
+    // the slots, and a few names a request
+    const uint64_t units = std::max<uint64_t>(t.slots != nullptr ? t.capacity : 0, uint64_t{t.requests} * std::min(t.width, 32u));
+    const uint64_t grid = std::clamp<uint64_t>(units / (2 * kv::kResizeThreads), 1, kSms);
+    return cuda_rc(launch(kv::resize_kernel, dim3(static_cast<uint32_t>(grid)), kv::kResizeThreads, 0,
+                          reinterpret_cast<cudaStream_t>(stream), a));
+}
+
+extern "C" int lmcache_gpu_kv_append_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
+                                           const lmcache_gpu_kv_vectors* vectors, int device, void* stream)
+{
+    if (!layer_ok(layout, pages, layer) || vectors == nullptr || device < 0) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    const lmcache_gpu_kv_layout& l = *layout;
+    const lmcache_gpu_kv_vectors& v = *vectors;
+    const int64_t element = kv::element_bytes(l.dtype);
+    const bool two = l.planes == 2;
+    if (uint64_t{l.heads} * l.head_dim > (1u << 30) || v.tokens > kv::kMaxTokens || v.key_stride < 0 || v.key_head_stride < 0 ||
+        (two && (v.value_stride < 0 || v.value_head_stride < 0))) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    if (v.tokens == 0) {
+        return LMCACHE_GPU_AESGCM_OK;
+    }
+    if (!array_ok(v.keys, element) || (two && !array_ok(v.values, element)) || !array_ok(v.slots, 8)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    if (pages->blocks == 0) {
+        return LMCACHE_GPU_AESGCM_OK;
+    }
+    DeviceGuard guard(device);
+    if (!guard.ok()) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
+    kv::AppendArgs a{};
+    uint64_t bits = layer_bits(l, *pages, layer, element) | l.head_dim * element;
+    for (uint32_t p = 0; p < l.planes; ++p) {
+        a.source[p] = static_cast<const char*>(p == 0 ? v.keys : v.values);
+        a.token_stride[p] = (p == 0 ? v.key_stride : v.value_stride) * element;
+        a.head_stride[p] = (p == 0 ? v.key_head_stride : v.value_head_stride) * element;
+        a.plane[p] = static_cast<char*>(pages->bases[p * l.layers + layer]);
+        bits |= reinterpret_cast<uintptr_t>(a.source[p]);
+        bits |= v.tokens > 1 ? a.token_stride[p] : 0;
+        bits |= l.heads > 1 ? a.head_stride[p] : 0;
+    }
+    a.block_stride = pages->block_stride * element;
+    a.row_stride = pages->row_stride * element;
+    a.page_head_stride = pages->head_stride * element;
+    a.cache_slots = static_cast<uint32_t>(pages->blocks * pages->block_size);
+    const uint32_t size = static_cast<uint32_t>(alignment_of(bits));
+    a.by_vector = kv::make_fast_div(static_cast<uint32_t>(l.head_dim * element / size));
+    a.by_heads = kv::make_fast_div(l.heads);
+    a.by_block = kv::make_fast_div(pages->block_size);
+    const uint64_t per_token = uint64_t{l.heads} * a.by_vector.d;
+    const uint64_t most = std::max<uint64_t>(1, (uint64_t{1} << 30) / per_token);
+    const auto kernel = size == 16 ? append_of<uint4> : size == 8 ? append_of<uint2> : size == 4 ? append_of<uint32_t> : append_of<uint16_t>;
+    for (uint64_t first = 0; first < v.tokens; first += most) {
+        const uint64_t n = std::min(most, v.tokens - first);
+        kv::AppendArgs b = a;
+        b.slots = v.slots + first;
+        for (uint32_t p = 0; p < l.planes; ++p) {
+            b.source[p] += first * a.token_stride[p];
+        }
+        b.units = static_cast<uint32_t>(n * per_token);
+        const uint32_t per_block = kv::kAppendThreads * kv::kAppendUnits;
+        const cudaError_t e = launch(kernel, dim3((b.units + per_block - 1) / per_block, l.planes), kv::kAppendThreads, 0,
+                                     reinterpret_cast<cudaStream_t>(stream), b);
+        if (e != cudaSuccess) {
+            return LMCACHE_GPU_AESGCM_ERR_CUDA;
+        }
+    }
+    return LMCACHE_GPU_AESGCM_OK;
+}
+
+extern "C" size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layout* layout, uint32_t query_heads, uint32_t value_dim)
+{
+    if (layout == nullptr || !heads_ok(*layout, query_heads, value_dim)) {
+        return 0;
+    }
+    return workspace_of(attend_plan(*layout, query_heads / layout->heads), value_dim).size;
+}
+
+extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
+                                           const lmcache_gpu_kv_attention* attention, int device, void* stream)
+{
+    if (!layer_ok(layout, pages, layer) || attention == nullptr || device < 0) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    const lmcache_gpu_kv_layout& l = *layout;
+    const lmcache_gpu_kv_attention& t = *attention;
+    const int64_t element = kv::element_bytes(l.dtype);
+    if (!heads_ok(l, t.query_heads, t.value_dim) || t.requests >= kv::kMaxRequests || t.width >= kv::kMost ||
+        t.query_stride < 0 || t.query_head_stride < 0 || t.out_stride < 0 || t.out_head_stride < 0 || t.lse_stride < 0 ||
+        t.table_stride < 0 || !std::isfinite(t.scale)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    const AttendPlan plan = attend_plan(l, t.query_heads / l.heads);
+    const Workspace w = workspace_of(plan, t.value_dim);
+    if (!array_ok(t.workspace, 16) || t.workspace_bytes < w.size) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    if (t.requests == 0) {
+        return LMCACHE_GPU_AESGCM_OK;
+    }
+    if (!array_ok(t.query, element) || !array_ok(t.out, element) || !aligned(t.lse, 4) || !array_ok(t.lengths, 4) ||
+        (t.width != 0 && !array_ok(t.tables, 4))) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    kv::AttendArgs a{};
+    a.group = t.query_heads / l.heads;
+    a.chunks = (a.group + plan.heads - 1) / plan.heads;
+    a.rows = l.heads * a.chunks;
+    a.limit = kv::row_limit(t.width, pages->block_size);
+    // the tiles of all rows have to be countable
+    if (uint64_t{t.requests} * a.rows >= (uint64_t{1} << 51) / (a.limit / kv::kTile + 1)) {
+        return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
+    }
+    DeviceGuard guard(device);
+    if (!guard.ok()) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
+    a.planes[0] = static_cast<const char*>(pages->bases[layer]);
+    a.planes[1] = static_cast<const char*>(pages->bases[(l.planes - 1) * l.layers + layer]);
+    a.block_stride = pages->block_stride * element;
+    a.row_stride = pages->row_stride * element;
+    a.page_head_stride = pages->head_stride * element;
+    a.query = static_cast<const char*>(t.query);
+    a.query_stride = t.query_stride * element;
+    a.query_head_stride = t.query_head_stride * element;
+    a.out = static_cast<char*>(t.out);
+    a.out_stride = t.out_stride * element;
+    a.out_head_stride = t.out_head_stride * element;
+    a.lse = t.lse;
+    a.lse_stride = t.lse_stride;
+    a.tables = t.tables;
+    a.table_stride = t.table_stride;
+    a.lengths = t.lengths;
+    char* const space = static_cast<char*>(t.workspace);
+    a.cut = reinterpret_cast<int4*>(space);
+    a.partial_sums = reinterpret_cast<float2*>(space + w.sums);
+    a.partial = reinterpret_cast<float*>(space + w.partial);
+    a.requests = t.requests;
+    a.blocks = static_cast<uint32_t>(pages->blocks);
+    a.window = t.window;
+    a.head_dim = l.head_dim;
+    a.value_dim = t.value_dim;
+    a.value_pad = (t.value_dim + 3) / 4 * 4;
+    a.scale = t.scale * kv::kLog2e;
+    a.by_block = kv::make_fast_div(pages->block_size);
+    a.by_chunks = kv::make_fast_div(a.chunks);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, 0, s, a);
+    if (e == cudaSuccess) {
+        e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads,
+                   static_cast<uint32_t>(kv::kAttendWarps * a.value_pad * sizeof(float)), s, a, plan.heads);
+    }
+    return cuda_rc(e);
+}

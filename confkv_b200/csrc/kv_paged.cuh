@@ -1,0 +1,281 @@
+// Kernels of a paged cache's requests (include/gpu_kv_paged_api.h): block tables and slot maps, and the writing of
+// new tokens. Attention is in kv_attend.cuh.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kernels.cuh"
+#include "kv_paged.h"
+
+namespace confkv {
+namespace kv {
+
+// ------------------------------------------------------------------ block tables and slot maps
+//
+// One launch without workspace: each block scans all requests' changes for itself (8 bytes a request, from L2 but for
+// the first block), so that it knows where any name or slot belongs, and then writes its share of them. The sums saturate at
+// 2^31 - 1, which is more than any ring or list of slots holds.
+
+constexpr uint32_t kResizeThreads = 512;
+constexpr uint32_t kMost = 0x7fffffffu;   // rings and lists of slots are shorter
+
+struct ResizeArgs {
+    int32_t* tables;
+    int64_t table_stride;
+    const int32_t* held;
+    const int32_t* lengths;
+    int32_t* free;
+    const int32_t* cursor;
+    int32_t* kept;
+    int32_t* cursor_after;
+    int64_t* slots;
+    int64_t* starts;
+    uint32_t capacity, requests, limit, blocks, ring;
+    uint32_t per;               // requests of a thread in the scan
+    FastDiv by_block;
+};
+
+__device__ __forceinline__ uint32_t add_most(uint32_t a, uint32_t b) { return min(a + b, kMost); }
+
+struct Sums {
+    uint32_t take, tokens, give;
+};
+
+__device__ __forceinline__ Sums add(const Sums& a, const Sums& b)
+{
+    return Sums{add_most(a.take, b.take), add_most(a.tokens, b.tokens), add_most(a.give, b.give)};
+}
+
+__device__ __forceinline__ Sums of_change(const Change& c) { return Sums{c.take, c.tokens, c.give}; }
+
+struct ResizeShared {
+    // exclusive sums in front of each thread's requests, refused ones left out
+    uint32_t take[kResizeThreads], tokens[kResizeThreads], give[kResizeThreads];
+    Sums warp[kResizeThreads / 32];
+    Sums before_refused;        // taken and listed in all
+    uint32_t refused;           // the first request that is refused
+    uint32_t given;
+};
+
+// The last of the threads' sums that is not above i.
+__device__ __forceinline__ uint32_t thread_of(const uint32_t* sums, uint32_t i)
+{
+    uint32_t t = 0;
+#pragma unroll
+    for (uint32_t step = kResizeThreads / 2; step != 0; step /= 2) {
+        if (sums[t + step] <= i) {
+            t += step;
+        }
+    }
+    return t;
+}
+
+__device__ __forceinline__ Change change_at(const ResizeArgs& a, uint32_t r)
+{
+    return change_of(a.held[r], a.lengths[r], a.limit, a.by_block);
+}
+
+__device__ __forceinline__ uint32_t ring_place(uint32_t first, uint32_t n, uint32_t ring)
+{
+    const uint32_t at = first + n;   // both at most `ring` < 2^31
+    return at >= ring ? at - ring : at;
+}
+
+__global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_constant__ ResizeArgs a)
+{
+    __shared__ ResizeShared s;
+    dev::pdl_release();
+    dev::pdl_wait();
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t / 32;
+    const Cursor cursor = cursor_of(a.cursor[0], a.cursor[1], a.ring);
+    const uint64_t begin = uint64_t{t} * a.per;
+    const uint32_t first = begin < a.requests ? static_cast<uint32_t>(begin) : a.requests;
+    const uint32_t last = begin + a.per < a.requests ? static_cast<uint32_t>(begin + a.per) : a.requests;
+    Sums mine{};
+    for (uint32_t r = first; r < last; ++r) {
+        mine = add(mine, of_change(change_at(a, r)));
+    }
+    Sums up = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const Sums o{__shfl_up_sync(~0u, up.take, d), __shfl_up_sync(~0u, up.tokens, d), __shfl_up_sync(~0u, up.give, d)};
+        if (lane >= d) {
+            up = add(up, o);
+        }
+    }
+    if (lane == 31) {
+        s.warp[warp] = up;
+    }
+    if (t == 0) {
+        s.refused = a.requests;
+    }
+    __syncthreads();
+    Sums sum{};   // in front of this thread's requests
+    for (uint32_t w = 0; w < warp; ++w) {
+        sum = add(sum, s.warp[w]);
+    }
+    {
+        const Sums o{__shfl_up_sync(~0u, up.take, 1), __shfl_up_sync(~0u, up.tokens, 1), __shfl_up_sync(~0u, up.give, 1)};
+        if (lane != 0) {
+            sum = add(sum, o);
+        }
+    }
+    // the first request of this thread's that does not fit
+    uint32_t refused = a.requests;
+    Sums at = sum;
+    for (uint32_t r = first; r < last; ++r) {
+        const Change c = change_at(a, r);
+        const Sums next = add(at, of_change(c));
+        if (c.tokens != 0 && (next.take > cursor.count || next.tokens > a.capacity)) {
+            refused = r;
+            break;
+        }
+        at = next;
+    }
+    if (refused < a.requests) {
+        atomicMin(&s.refused, refused);
+    }
+    __syncthreads();
+    const uint32_t stop = s.refused;
+    if (refused == stop && stop < a.requests) {
+        s.before_refused = at;                      // the thread that has it
+    } else if (stop == a.requests && t == kResizeThreads - 1) {
+        s.before_refused = at;                      // the sums of all
+    }
+    if (t == kResizeThreads - 1) {
+        s.given = add(sum, mine).give;
+    }
+    __syncthreads();
+    const Sums total = s.before_refused;
+    s.take[t] = min(sum.take, total.take);
+    s.tokens[t] = min(sum.tokens, total.tokens);
+    s.give[t] = sum.give;
+    __syncthreads();
+    const uint32_t given = min(s.given, a.ring - cursor.count);
+
+    if (blockIdx.x == 0) {
+        uint32_t start = s.tokens[t];
+        for (uint32_t r = first; r < last; ++r) {
+            const Change c = change_at(a, r);
+            const bool stays = c.tokens != 0 && r >= stop;
+            a.kept[r] = static_cast<int32_t>(stays ? c.held : c.kept);
+            if (a.starts != nullptr) {
+                a.starts[r] = start;
+            }
+            start += stays ? 0 : c.tokens;
+        }
+        if (t == 0) {
+            if (a.starts != nullptr) {
+                a.starts[a.requests] = total.tokens;
+            }
+            a.cursor_after[0] = static_cast<int32_t>(a.ring != 0 ? ring_place(cursor.first, total.take, a.ring) : 0);
+            a.cursor_after[1] = static_cast<int32_t>(cursor.count - total.take + given);
+        }
+    }
+
+    const uint32_t step = gridDim.x * kResizeThreads;
+    const uint32_t me = blockIdx.x * kResizeThreads + t;
+    // names taken: the ring's front goes behind the blocks that requests have
+    for (uint64_t i = me; i < total.take; i += step) {
+        const uint32_t n = static_cast<uint32_t>(i), bucket = thread_of(s.take, n);
+        uint32_t r = bucket * a.per, in = s.take[bucket];
+        Change c = change_at(a, r);
+        while (n - in >= c.take) {
+            in += c.take;
+            c = change_at(a, ++r);
+        }
+        a.tables[r * a.table_stride + c.before + (n - in)] = a.free[ring_place(cursor.first, n, a.ring)];
+    }
+    // names given back, behind the ring's end
+    const uint32_t end = a.ring != 0 ? ring_place(cursor.first, cursor.count, a.ring) : 0;
+    for (uint64_t i = me; i < given; i += step) {
+        const uint32_t n = static_cast<uint32_t>(i), bucket = thread_of(s.give, n);
+        uint32_t r = bucket * a.per, in = s.give[bucket];
+        Change c = change_at(a, r);
+        while (n - in >= c.give) {
+            in += c.give;
+            c = change_at(a, ++r);
+        }
+        a.free[ring_place(end, n, a.ring)] = a.tables[r * a.table_stride + (c.before - c.give) + (n - in)];
+    }
+    // slots of new tokens; a block that was taken just now is read from the ring
+    const uint32_t listed = a.slots != nullptr ? a.capacity : 0;
+    for (uint64_t i = me; i < listed; i += step) {
+        const uint32_t n = static_cast<uint32_t>(i);
+        int64_t slot = -1;
+        if (n < total.tokens) {
+            const uint32_t bucket = thread_of(s.tokens, n);
+            uint32_t r = bucket * a.per, in = s.tokens[bucket], taken = s.take[bucket];
+            Change c = change_at(a, r);
+            while (n - in >= c.tokens) {
+                in += c.tokens;
+                taken += c.take;
+                c = change_at(a, ++r);
+            }
+            const uint32_t token = c.held + (n - in);
+            const uint32_t block = quotient(a.by_block, token);
+            const int32_t name = block < c.before ? a.tables[r * a.table_stride + block]
+                                                  : a.free[ring_place(cursor.first, taken + (block - c.before), a.ring)];
+            if (name >= 0 && static_cast<uint32_t>(name) < a.blocks) {
+                slot = int64_t{name} * a.by_block.d + (token - block * a.by_block.d);
+            }
+        }
+        a.slots[n] = slot;
+    }
+}
+
+// ------------------------------------------------------------------ new tokens
+
+constexpr uint32_t kAppendThreads = 128;
+constexpr uint32_t kAppendUnits = 4;      // granules of a thread
+
+struct AppendArgs {
+    const char* source[2];
+    int64_t token_stride[2], head_stride[2];        // bytes
+    char* plane[2];
+    int64_t block_stride, row_stride, page_head_stride;
+    const int64_t* slots;
+    uint32_t units;                                 // granules of a plane in this launch
+    uint32_t cache_slots;
+    FastDiv by_vector, by_heads, by_block;          // granules of a vector, heads
+};
+
+// Copies granules of the size of G; blockIdx.y is the plane.
+template <class G>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a)
+{
+    dev::pdl_release();
+    dev::pdl_wait();
+    const uint32_t p = blockIdx.y;
+    const uint32_t first = blockIdx.x * (kAppendThreads * kAppendUnits) + threadIdx.x;
+    G value[kAppendUnits];
+    char* to[kAppendUnits];
+#pragma unroll
+    for (uint32_t k = 0; k < kAppendUnits; ++k) {
+        const uint32_t unit = first + k * kAppendThreads;
+        to[k] = nullptr;
+        if (unit < a.units) {
+            const uint32_t vector = quotient(a.by_vector, unit), granule = unit - vector * a.by_vector.d;
+            const uint32_t token = quotient(a.by_heads, vector), head = vector - token * a.by_heads.d;
+            const int64_t slot = a.slots[token];
+            if (slot >= 0 && slot < static_cast<int64_t>(a.cache_slots)) {
+                const uint32_t at = static_cast<uint32_t>(slot), block = quotient(a.by_block, at);
+                value[k] = *reinterpret_cast<const G*>(a.source[p] + token * a.token_stride[p] + head * a.head_stride[p] +
+                                                       granule * sizeof(G));
+                to[k] = a.plane[p] + block * a.block_stride + (at - block * a.by_block.d) * a.row_stride +
+                        head * a.page_head_stride + granule * sizeof(G);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kAppendUnits; ++k) {
+        if (to[k] != nullptr) {
+            *reinterpret_cast<G*>(to[k]) = value[k];
+        }
+    }
+}
+
+}  // namespace kv
+}  // namespace confkv

@@ -1,0 +1,71 @@
+// Host build of the paged cache's index arithmetic (csrc/kv_paged.h) for the CPU tests: each function on arrays.
+#include <cstdint>
+
+#include "kv_paged.h"
+
+using namespace confkv::kv;
+
+extern "C" {
+
+// held, length -> kept, before, take, give, tokens
+void changes(const int32_t* held, const int32_t* length, int n, uint32_t width, uint32_t block_size, uint32_t* out)
+{
+    const FastDiv d = make_fast_div(block_size);
+    const uint32_t limit = row_limit(width, block_size);
+    for (int i = 0; i < n; ++i) {
+        const Change c = change_of(held[i], length[i], limit, d);
+        uint32_t* o = out + 5 * i;
+        o[0] = c.kept;
+        o[1] = c.before;
+        o[2] = c.take;
+        o[3] = c.give;
+        o[4] = c.tokens;
+    }
+}
+
+void cursors(const int32_t* first, const int32_t* count, int n, uint32_t ring, uint32_t* out)
+{
+    for (int i = 0; i < n; ++i) {
+        const Cursor c = cursor_of(first[i], count[i], ring);
+        out[2 * i] = c.first;
+        out[2 * i + 1] = c.count;
+    }
+}
+
+void spans(const int32_t* length, int n, uint32_t limit, uint32_t window, uint32_t tile, uint32_t* out)
+{
+    for (int i = 0; i < n; ++i) {
+        const Span s = span_of(length[i], limit, window);
+        out[3 * i] = s.first;
+        out[3 * i + 1] = s.end;
+        out[3 * i + 2] = tiles_of(s, tile);
+    }
+}
+
+// 0 where all parts of `total` tiles are right: none empty, one behind the other, sizes at most one apart, every tile's worker
+// the one whose part it lies in (at the parts' ends, and at every tile where there are few)
+int check_parts(uint64_t total, uint32_t workers)
+{
+    if (part_start(total, workers, 0) != 0 || part_start(total, workers, workers) != total) {
+        return 1;
+    }
+    const uint64_t least = total / workers;
+    for (uint32_t c = 0; c < workers; ++c) {
+        const uint64_t a = part_start(total, workers, c), b = part_start(total, workers, c + 1);
+        if (b - a < least || b - a > least + 1 || a == b) {
+            return 2;
+        }
+        if (part_of(total, workers, a) != c || part_of(total, workers, b - 1) != c) {
+            return 3;
+        }
+        if (total < 5000) {
+            for (uint64_t t = a; t < b; ++t) {
+                if (part_of(total, workers, t) != c) {
+                    return 4;
+                }
+            }
+        }
+    }
+    return 0;
+}
+}
