@@ -5,6 +5,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels.cuh"
 #include "kv_paged.h"
@@ -41,6 +42,7 @@ struct AttendArgs {
     uint32_t head_dim, value_dim, value_pad;
     float scale;                                // times log2 e: exponents are of base 2
     FastDiv by_block, by_chunks;
+    FastDiv by_vector;                          // chunks of 16 bytes of a vector
 };
 
 // ------------------------------------------------------------------ parts
@@ -400,6 +402,442 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
             next_row(a, kTile, &p);
         }
     }
+}
+
+// ------------------------------------------------------------------ 16-bit types
+//
+// A warp takes 16 tokens at a time, in products of 16 x 8 x 16 whose rows are tokens or values and whose columns are query heads: scores =
+// K q (K's vectors as they lie), results = V^T p (V's vectors read across), so that 8 query heads fill an instruction's columns and
+// nothing is padded to 16 rows. Between the two the weights change places within the warp (movmatrix).
+// Each warp has stages of its own, filled by asynchronous copies of 16 bytes two or more tiles ahead, over the ends of rows too:
+// no warp waits for another but where a row ends and the four warps' sums are put together.
+
+constexpr uint32_t kWarpTokens = kTile / kAttendWarps;      // 16
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// 16 bytes to shared memory; zeros, and nothing read, where `there` is false.
+__device__ __forceinline__ void copy_16(uint32_t to, const char* from, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void copies_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+__device__ __forceinline__ void load_matrices_across(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t across(uint32_t x)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+template <class T>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+__device__ __forceinline__ float power_of_2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Two values in one register, `lo` in the low half.
+template <class T>
+__device__ __forceinline__ uint32_t pack(float lo, float hi)
+{
+    uint32_t r;
+    if constexpr (std::is_same_v<T, __half>) {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    } else {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    }
+    return r;
+}
+
+// DP: values of a vector in shared memory, a multiple of 64, zeros behind head_dim. NT: eights of query heads of a row. ONE: keys
+// and values are the same vectors. Vectors are whole chunks of 16 bytes; chunk c of token r lies at place c ^ (r % 8), so
+// that eight tokens' chunks of one column lie in different banks.
+template <class T, int DP, int NT, bool ONE, int STAGES>
+struct MmaShape {
+    static constexpr uint32_t kHeads = 8 * NT;
+    static constexpr uint32_t kRowBytes = DP * 2;
+    static constexpr uint32_t kPlaneBytes = kWarpTokens * kRowBytes;
+    static constexpr uint32_t kStageBytes = kPlaneBytes * (ONE ? 1 : 2);
+    static constexpr uint32_t kStages = kAttendWarps * STAGES * kStageBytes;
+    static constexpr uint32_t kMergeRow = DP + 4;               // floats; heads 2 apart lie 8 banks apart
+    static constexpr uint32_t kMergeBytes = 2 * kHeads * kMergeRow * 4;
+    static constexpr uint32_t kShared = kStages + kMergeBytes;
+    static_assert(kShared + 4096 <= 227 * 1024, "more than a block has");
+};
+
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(const __grid_constant__ AttendArgs a)
+{
+    using Shape = MmaShape<T, DP, NT, ONE, STAGES>;
+    constexpr int KT = DP / 16;
+    constexpr bool kTwoParts = std::is_same_v<T, __nv_bfloat16>;
+    constexpr float kBelow = 1.0f - 0x1p-8f;
+    constexpr float kRaise = std::is_same_v<T, __half> ? 15.0f : 0.0f;
+    constexpr uint32_t GH = Shape::kHeads;
+    extern __shared__ __align__(1024) char memory[];
+    __shared__ PartShared part_shared;
+    constexpr uint32_t kRow = Shape::kMergeRow;
+    __shared__ float2 merge_sums[2][kAttendWarps][GH];          // in turns: a warp may write its next row's while others read
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    dev::pdl_release();
+    // behind head_dim the stages hold zeros, which no copy touches
+    if (a.head_dim != DP) {
+        for (uint32_t i = threadIdx.x; i < Shape::kStages / 16; i += kAttendThreads) {
+            reinterpret_cast<uint4*>(memory)[i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+    }
+    dev::pdl_wait();
+    Part p;
+    if (!find_part<kAttendThreads>(a, part_shared, kTile, &p)) {
+        if (threadIdx.x == 0) {
+            note_cut(a, p, false, 0);
+        }
+        return;
+    }
+    char* const stages = memory + warp * (STAGES * Shape::kStageBytes);
+    const uint32_t stage_base = shared_address(stages);
+    float* const merge = reinterpret_cast<float*>(memory + Shape::kStages);    // [2][GH][kRow]
+    const uint32_t chunks = a.head_dim / 8;
+    const uint32_t tiles16 = (a.head_dim + 15) / 16, value_tiles = (a.value_dim + 15) / 16;
+
+    // what is copied runs ahead of what is computed: the next tile to copy, and the tokens that each tile under way has
+    Part ahead = p;
+    uint64_t copied = p.next;
+    uint32_t tokens_of[STAGES];                 // bit i: token i of this warp's 16 is one
+    uint32_t stage_in = 0, stage_out = 0;
+    const auto copy_tile = [&]() -> uint32_t {
+        uint32_t there = 0;
+        if (copied < ahead.end) {
+            const uint32_t key_head = quotient(a.by_chunks, ahead.row);
+            const int32_t* table = a.tables + ahead.request * a.table_stride;
+            const uint32_t token = ahead.span.first + ahead.tile * kTile + warp * kWarpTokens + lane % kWarpTokens;
+            int64_t offset = token < ahead.span.end ? token_offset(a, table, token) : -1;
+            there = __ballot_sync(~0u, offset >= 0) & 0xffffu;
+            offset = offset >= 0 ? offset + key_head * a.page_head_stride : 0;
+            const uint32_t to = stage_base + stage_in * Shape::kStageBytes;
+            for (uint32_t k = 0; k < kWarpTokens * chunks; k += 32) {
+                const uint32_t i = k + lane, r = quotient(a.by_vector, i), c = i - r * a.by_vector.d;   // r <= 16
+                const int64_t from = __shfl_sync(~0u, offset, r) + c * 16;
+                const uint32_t at = to + r * Shape::kRowBytes + ((c ^ (r % 8)) * 16);
+                const bool is = (there >> r & 1) != 0;
+                if (r < kWarpTokens) {
+                    copy_16(at, a.planes[0] + from, is);
+                    if constexpr (!ONE) {
+                        copy_16(at + Shape::kPlaneBytes, a.planes[1] + from, is);
+                    }
+                }
+            }
+            ++copied;
+            if (copied < ahead.end && ++ahead.tile == ahead.tiles) {
+                next_row(a, kTile, &ahead);
+            }
+        }
+        copies_end();
+        stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+        return there;
+    };
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) {
+        tokens_of[k] = copy_tile();
+    }
+
+    uint32_t place = 0, turn = 0;
+    while (p.next < p.end) {
+        const uint64_t left = p.end - p.next;
+        const uint32_t tiles = left < p.tiles - p.tile ? static_cast<uint32_t>(left) : p.tiles - p.tile;
+        const bool begins = p.tile == 0, ends = p.tile + tiles == p.tiles;
+        const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
+        const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
+        const uint32_t heads = min(GH, a.group - chunk * GH);
+        // q as the second factor: column lane / 4, values 2 (lane % 4) and the next, and 8 further on
+        uint32_t q[KT][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t g = n * 8 + lane / 4;
+            const char* from = a.query + p.request * a.query_stride + (head + g) * a.query_head_stride + (lane % 4) * 4;
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    q[k][n][j] = g < heads && static_cast<uint32_t>(k * 2 + j) < chunks
+                                     ? *reinterpret_cast<const uint32_t*>(from + k * 32 + j * 16) : 0u;
+                }
+            }
+        }
+        float m[NT][2], l[NT][2], o[KT][NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[k][n][i] = 0.0f;
+                }
+            }
+        }
+        bool any = false;
+        for (uint32_t t = 0; t < tiles; ++t) {
+            copies_wait<STAGES - 2>();
+            __syncwarp();
+            tokens_of[STAGES - 1] = copy_tile();
+            const uint32_t there = tokens_of[0];
+#pragma unroll
+            for (int k = 0; k < STAGES - 1; ++k) {
+                tokens_of[k] = tokens_of[k + 1];
+            }
+            const uint32_t keys = stage_base + stage_out * Shape::kStageBytes;
+            const uint32_t values = keys + (ONE ? 0 : Shape::kPlaneBytes);
+            stage_out = stage_out + 1 == STAGES ? 0 : stage_out + 1;
+            if (there == 0) {
+                continue;
+            }
+            any = true;
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            }
+            {
+                const uint32_t r = lane % 16, c = lane / 16;
+                const uint32_t row = keys + r * Shape::kRowBytes;
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    if (static_cast<uint32_t>(k) < tiles16) {
+                        uint32_t x[4];
+                        load_matrices(x, row + (((2 * k + c) ^ (r % 8)) * 16));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            multiply<T>(s[n], x, q[k][n][0], q[k][n][1]);
+                        }
+                    }
+                }
+            }
+            // tokens lane / 4 and lane / 4 + 8, heads 2 (lane % 4) and the next of each eight
+            const bool first = (there >> (lane / 4) & 1) != 0, second = (there >> (lane / 4 + 8) & 1) != 0;
+            float top[NT][2];
+            bool more = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    s[n][j] = first ? s[n][j] * a.scale : -INFINITY;
+                    s[n][j + 2] = second ? s[n][j + 2] * a.scale : -INFINITY;
+                    float x = fmaxf(s[n][j], s[n][j + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) {
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+                    }
+                    top[n][j] = fmaxf(m[n][j], x);
+                    more |= top[n][j] > m[n][j];
+                }
+            }
+            if (__any_sync(~0u, more)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float fade = power_of_2(m[n][j] - reference(top[n][j]));
+                        m[n][j] = top[n][j];
+                        l[n][j] *= fade;
+#pragma unroll
+                        for (int k = 0; k < KT; ++k) {
+                            o[k][n][j] *= fade;
+                            o[k][n][j + 2] *= fade;
+                        }
+                    }
+                }
+            }
+            uint32_t w[NT][2], rest[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float base[2] = {reference(m[n][0]) - kRaise, reference(m[n][1]) - kRaise};
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = power_of_2(s[n][i] - base[i % 2]);
+                    l[n][i % 2] += x[i];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (kTwoParts) {
+                        // the weight cut to 8 bits a little below itself, and the rest: both above 0, so that a value's infinity stays one
+                        const uint32_t lo = __float_as_uint(x[2 * h] * kBelow), hi = __float_as_uint(x[2 * h + 1] * kBelow);
+                        w[n][h] = across(__byte_perm(lo, hi, 0x7632));
+                        rest[n][h] = across(pack<T>(x[2 * h] - __uint_as_float(lo & 0xffff0000u),
+                                                    x[2 * h + 1] - __uint_as_float(hi & 0xffff0000u)));
+                    } else {
+                        w[n][h] = across(pack<T>(x[2 * h], x[2 * h + 1]));
+                    }
+                }
+            }
+            {
+                const uint32_t r = lane % 8 + lane / 16 * 8, c = lane / 8 % 2;
+                const uint32_t row = values + r * Shape::kRowBytes;
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    if (static_cast<uint32_t>(k) < value_tiles) {
+                        uint32_t x[4];
+                        load_matrices_across(x, row + (((2 * k + c) ^ (r % 8)) * 16));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            multiply<T>(o[k][n], x, w[n][0], w[n][1]);
+                            if constexpr (kTwoParts) {
+                                multiply<T>(o[k][n], x, rest[n][0], rest[n][1]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+
+        // the four warps' sums together
+        float2 (&sums)[kAttendWarps][GH] = merge_sums[turn];
+        turn ^= 1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {
+                    l[n][j] += __shfl_xor_sync(~0u, l[n][j], d);
+                }
+                l[n][j] = m[n][j] == -INFINITY && l[n][j] == 0.0f && any ? 1.0f : l[n][j] * power_of_2(-kRaise);
+                if (lane < 4) {
+                    sums[warp][n * 8 + lane * 2 + j] = make_float2(m[n][j], l[n][j]);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t g = n * 8 + lane % 4 * 2 + j;
+                float top_of_all = -INFINITY;
+#pragma unroll
+                for (uint32_t v = 0; v < kAttendWarps; ++v) {
+                    top_of_all = fmaxf(top_of_all, sums[v][g].x);
+                }
+                const float f = top_of_all == -INFINITY ? 1.0f : power_of_2(m[n][j] - top_of_all - kRaise);
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    o[k][n][j] *= f;
+                    o[k][n][j + 2] *= f;
+                }
+            }
+        }
+        // value lane / 4 (and 8 further on) of each 16, heads as above
+        float* const mine = merge + warp % 2 * (GH * kRow) + lane % 4 * 2 * kRow + lane / 4;
+        if (warp >= 2) {
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] = o[k][n][i];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (warp < 2) {
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] += o[k][n][i];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = begins && ends;
+        const uint32_t at_place = blockIdx.x * 2 + place;
+        for (uint32_t g = warp; g < heads; g += kAttendWarps) {
+            float2 part[kAttendWarps];
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kAttendWarps; ++w) {
+                part[w] = sums[w][g];
+                top = fmaxf(top, part[w].x);
+            }
+#pragma unroll
+            for (uint32_t w = 0; w < kAttendWarps; ++w) {
+                sum += part[w].y * (top == -INFINITY ? 1.0f : power_of_2(part[w].x - top));
+            }
+            const float factor = whole ? result_factor(top, sum) : 1.0f;
+            T* out = reinterpret_cast<T*>(a.out + p.request * a.out_stride + (head + g) * a.out_head_stride);
+            float* partial = a.partial + (uint64_t{at_place} * GH + g) * a.value_pad;
+            for (uint32_t d = lane; d < a.value_dim; d += 32) {
+                const float x = merge[g * kRow + d] + merge[(GH + g) * kRow + d];
+                if (whole) {
+                    out[d] = from_float<T>(x * factor);
+                } else {
+                    partial[d] = x;
+                }
+            }
+            if (lane == 0) {
+                if (!whole) {
+                    a.partial_sums[at_place * GH + g] = make_float2(top, sum);
+                } else if (a.lse != nullptr) {
+                    a.lse[p.request * a.lse_stride + head + g] = result_lse(top, sum);
+                }
+            }
+        }
+        if (threadIdx.x == 0 && p.next + tiles == p.end) {
+            note_cut(a, p, begins && !ends, place);
+        }
+        p.next += tiles;
+        place = 1;
+        if (p.next < p.end) {
+            next_row(a, kTile, &p);
+        }
+    }
+    copies_wait<0>();
 }
 
 // ------------------------------------------------------------------ joining

@@ -1,5 +1,6 @@
 // The entry points of a paged cache's requests: checks, the kernels' parameters and their launch.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "gpu_kv_paged_api.h"
@@ -154,6 +155,8 @@ struct AttendPlan {
     JoinKernel join;
     uint32_t heads;             // query heads of a row
     uint32_t workers;
+    uint32_t shared;            // bytes of dynamic shared memory
+    std::atomic<uint64_t>* allowed;     // devices on which the kernel may have them
 };
 
 constexpr uint32_t kSms = 148;
@@ -180,11 +183,61 @@ AttendPlan any_plan(uint32_t head_dim, uint32_t group)
     return p;
 }
 
-AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+AttendPlan mma_plan()
 {
+    static std::atomic<uint64_t> allowed{0};
+    using Shape = kv::MmaShape<T, DP, NT, ONE, STAGES>;
+    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, Shape::kHeads, BLOCKS * kSms,
+                      Shape::kShared, &allowed};
+}
+
+// Whether the 16-bit kernel takes vectors of this size, in a cache and of queries of this alignment.
+bool mma_takes(const lmcache_gpu_kv_layout& l, uint64_t cache_alignment, uint64_t query_alignment)
+{
+    return l.dtype != kv::kFp32 && l.head_dim % 8 == 0 && l.head_dim <= (l.planes == 2 ? 256u : 576u) && cache_alignment >= 16 &&
+           query_alignment >= 4;
+}
+
+template <class T>
+AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
+{
+    const uint32_t d = l.head_dim;
+    const bool two = group > 8;
+    if (l.planes == 2) {
+        return d <= 64    ? (two ? mma_plan<T, 64, 2, false, 4, 2>() : mma_plan<T, 64, 1, false, 4, 3>())
+               : d <= 128 ? (two ? mma_plan<T, 128, 2, false, 3, 1>() : mma_plan<T, 128, 1, false, 3, 2>())
+               : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>()
+                          : mma_plan<T, 256, 1, false, 3, 1>();
+    }
+    return d <= 128   ? (two ? mma_plan<T, 128, 2, true, 5, 2>() : mma_plan<T, 128, 1, true, 5, 2>())
+           : d <= 256 ? mma_plan<T, 256, 1, true, 5, 1>()
+           : d <= 320 ? mma_plan<T, 320, 1, true, 4, 1>()
+                      : mma_plan<T, 576, 1, true, 2, 1>();
+}
+
+AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t cache_alignment, uint64_t query_alignment)
+{
+    if (mma_takes(l, cache_alignment, query_alignment)) {
+        return l.dtype == kv::kBf16 ? mma_plan<__nv_bfloat16>(l, group) : mma_plan<__half>(l, group);
+    }
     return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group)
            : l.dtype == kv::kFp16 ? any_plan<__half>(l.head_dim, group)
                                   : any_plan<float>(l.head_dim, group);
+}
+
+// Once for each device and kernel: more shared memory than 48 KiB has to be asked for.
+cudaError_t allow_shared(const AttendPlan& p, int device)
+{
+    const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+    if (p.allowed == nullptr || (p.allowed->load(std::memory_order_acquire) & bit) != 0) {
+        return cudaSuccess;
+    }
+    const cudaError_t e = cudaFuncSetAttribute(p.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(p.shared));
+    if (e == cudaSuccess) {
+        p.allowed->fetch_or(bit, std::memory_order_release);
+    }
+    return e;
 }
 
 // The parts of the workspace, in bytes behind its start.
@@ -318,7 +371,10 @@ extern "C" size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layo
     if (layout == nullptr || !heads_ok(*layout, query_heads, value_dim)) {
         return 0;
     }
-    return workspace_of(attend_plan(*layout, query_heads / layout->heads), value_dim).size;
+    // the most that any alignment's kernel takes
+    const uint32_t group = query_heads / layout->heads;
+    return std::max(workspace_of(attend_plan(*layout, group, 16, 16), value_dim).size,
+                    workspace_of(attend_plan(*layout, group, 1, 1), value_dim).size);
 }
 
 extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
@@ -335,9 +391,13 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
         t.table_stride < 0 || !std::isfinite(t.scale)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
-    const AttendPlan plan = attend_plan(l, t.query_heads / l.heads);
+    const uint64_t query_bits = reinterpret_cast<uintptr_t>(t.query) | (t.requests > 1 ? t.query_stride * element : 0) |
+                                (t.query_heads > 1 ? t.query_head_stride * element : 0);
+    const AttendPlan plan = attend_plan(l, t.query_heads / l.heads, alignment_of(layer_bits(l, *pages, layer, element)),
+                                        alignment_of(query_bits));
     const Workspace w = workspace_of(plan, t.value_dim);
-    if (!array_ok(t.workspace, 16) || t.workspace_bytes < w.size) {
+    if (!array_ok(t.workspace, 16) ||
+        t.workspace_bytes < lmcache_gpu_kv_attend_workspace_size(layout, t.query_heads, t.value_dim)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     if (t.requests == 0) {
@@ -362,6 +422,9 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     }
     a.planes[0] = static_cast<const char*>(pages->bases[layer]);
     a.planes[1] = static_cast<const char*>(pages->bases[(l.planes - 1) * l.layers + layer]);
+    if (pages->blocks == 0) {
+        a.planes[0] = a.planes[1] = static_cast<const char*>(t.workspace);      // never read, but an address
+    }
     a.block_stride = pages->block_stride * element;
     a.row_stride = pages->row_stride * element;
     a.page_head_stride = pages->head_stride * element;
@@ -389,8 +452,13 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.scale = t.scale * kv::kLog2e;
     a.by_block = kv::make_fast_div(pages->block_size);
     a.by_chunks = kv::make_fast_div(a.chunks);
+    a.by_vector = kv::make_fast_div(std::max<uint32_t>(1, l.head_dim / 8));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, 0, s, a);
+    cudaError_t e = allow_shared(plan, device);
+    if (e != cudaSuccess) {
+        return LMCACHE_GPU_AESGCM_ERR_CUDA;
+    }
+    e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, plan.shared, s, a);
     if (e == cudaSuccess) {
         e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads,
                    static_cast<uint32_t>(kv::kAttendWarps * a.value_pad * sizeof(float)), s, a, plan.heads);
