@@ -47,14 +47,14 @@ struct AttendArgs {
 
 // ------------------------------------------------------------------ parts
 //
-// The rows' tiles, one row behind the other, are cut into equal parts, one a worker (a block): few long rows and many
-// short ones keep all SMs busy alike, whatever the lengths, which only the device knows. A worker that has a whole row writes its
-// result; of a row that is cut each worker writes what it has of it, its first row's in place 0 and another's in place 1,
-// and join_kernel puts them together.
+// The rows' units (tiles, and some for a row's beginning and end), one row behind the other, are cut into equal parts, one a worker
+// (a block): few long rows and many short ones keep all SMs busy alike, whatever the lengths, which only the device
+// knows. A worker that has a whole row writes its result; of a row that is cut each worker writes what it has of it, its
+// first row's in place 0 and another's in place 1, and join_kernel puts them together.
 
 struct PartShared {
     uint64_t warp[kAttendWarps];
-    uint64_t total, found_sum;
+    uint64_t found_sum;
     uint32_t found;
 };
 
@@ -72,22 +72,51 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v)
     return v;
 }
 
-// A worker's part [next, end) and where it begins: tile `tile` of row `row` of request `request`.
+// A worker's part, and a row of it with the tiles [piece.first, piece.last) that are the worker's.
 struct Part {
-    uint64_t next, end, total;
+    uint64_t begin, end, total, row_begin;      // units; row_begin: the row's first
     uint32_t workers;
-    uint32_t request, row, tile, tiles;
+    uint32_t request, row, tiles;
     Span span;
+    Piece piece;
 };
 
-// Every thread gets the same; false for a worker without a part.
-template <uint32_t THREADS>
-__device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, uint32_t tile, Part* p)
+__device__ __forceinline__ void set_row(const AttendArgs& a, Part* p)
 {
+    p->span = span_at(a, p->request);
+    p->tiles = tiles_of(p->span, kTile);
+}
+
+__device__ __forceinline__ void set_piece(Part* p)
+{
+    p->piece = piece_of(static_cast<int64_t>(p->begin) - static_cast<int64_t>(p->row_begin),
+                        static_cast<int64_t>(p->end) - static_cast<int64_t>(p->row_begin), p->tiles);
+}
+
+// On to the part's next row; false where it has no tiles of any other.
+__device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
+{
+    p->row_begin += p->tiles + kRowUnits;
+    if (p->row_begin + kRowUnits >= p->end) {
+        return false;
+    }
+    if (++p->row == a.rows) {
+        p->row = 0;
+        ++p->request;
+        set_row(a, p);
+    }
+    set_piece(p);
+    return true;
+}
+
+// Every thread gets the same; false for a worker that has no tiles.
+__device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Part* p)
+{
+    constexpr uint32_t kThreads = kAttendThreads;
     const uint32_t t = threadIdx.x;
     uint64_t sum = 0;
-    for (uint32_t r = t; r < a.requests; r += THREADS) {
-        sum += tiles_of(span_at(a, r), tile);
+    for (uint32_t r = t; r < a.requests; r += kThreads) {
+        sum += tiles_of(span_at(a, r), kTile) + kRowUnits;
     }
     sum = warp_sum(sum);
     if (t % 32 == 0) {
@@ -96,21 +125,21 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, ui
     __syncthreads();
     uint64_t total = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < THREADS / 32; ++w) {
+    for (uint32_t w = 0; w < kAttendWarps; ++w) {
         total += s.warp[w];
     }
     p->total = total * a.rows;
-    p->workers = p->total < gridDim.x ? static_cast<uint32_t>(p->total) : gridDim.x;
+    p->workers = workers_for(p->total, gridDim.x);
     if (blockIdx.x >= p->workers) {
         return false;
     }
-    p->next = part_start(p->total, p->workers, blockIdx.x);
+    p->begin = part_start(p->total, p->workers, blockIdx.x);
     p->end = part_start(p->total, p->workers, blockIdx.x + 1);
-    // the request that has tile `next`: the one whose rows begin at or before it
+    // the request that has unit `begin`: the one whose rows begin at or before it
     uint64_t base = 0;
-    for (uint32_t from = 0; from < a.requests; from += THREADS) {
+    for (uint32_t from = 0; from < a.requests; from += kThreads) {
         const uint32_t r = from + t;
-        const uint64_t n = r < a.requests ? uint64_t{tiles_of(span_at(a, r), tile)} * a.rows : 0;
+        const uint64_t n = r < a.requests ? uint64_t{tiles_of(span_at(a, r), kTile) + kRowUnits} * a.rows : 0;
         uint64_t up = n;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -124,39 +153,40 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, ui
         __syncthreads();
         uint64_t before = base, all = base;
 #pragma unroll
-        for (uint32_t w = 0; w < THREADS / 32; ++w) {
+        for (uint32_t w = 0; w < kAttendWarps; ++w) {
             before += w < t / 32 ? s.warp[w] : 0;
             all += s.warp[w];
         }
-        if (before + up > p->next && before + up - n <= p->next) {
+        if (before + up > p->begin && before + up - n <= p->begin) {
             s.found = r;
             s.found_sum = before + up - n;
         }
         base = all;
-        if (all > p->next) {
+        if (all > p->begin) {
             break;
         }
     }
     __syncthreads();
     p->request = s.found;
-    p->span = span_at(a, p->request);
-    p->tiles = tiles_of(p->span, tile);
-    const uint64_t in = p->next - s.found_sum;
-    p->row = static_cast<uint32_t>(in / p->tiles);
-    p->tile = static_cast<uint32_t>(in - uint64_t{p->row} * p->tiles);
-    return true;
+    set_row(a, p);
+    const uint64_t in = p->begin - s.found_sum, units = p->tiles + kRowUnits;
+    p->row = static_cast<uint32_t>(in / units);
+    p->row_begin = s.found_sum + p->row * units;
+    set_piece(p);
+    return p->piece.last > p->piece.first;
 }
 
-// The next row of a part.
-__device__ __forceinline__ void next_row(const AttendArgs& a, uint32_t tile, Part* p)
+// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row, the worker that
+// has its last tile, and in which of this worker's places it stands; else no request.
+__device__ __forceinline__ int4 no_cut() { return make_int4(-1, 0, 0, 0); }
+
+__device__ __forceinline__ int4 cut_of(const Part& p, uint32_t place)
 {
-    p->tile = 0;
-    if (++p->row == a.rows) {
-        p->row = 0;
-        ++p->request;
-        p->span = span_at(a, p->request);
-        p->tiles = tiles_of(p->span, tile);
+    if (p.piece.first != 0 || p.piece.last == p.tiles) {
+        return no_cut();
     }
+    return make_int4(static_cast<int>(p.request), static_cast<int>(p.row),
+                     static_cast<int>(part_of(p.total, p.workers, p.row_begin + kRowUnits + p.tiles - 1)), static_cast<int>(place));
 }
 
 // The vector of a token: where it starts in its plane, or -1 where its block is not one of the cache's.
@@ -184,19 +214,6 @@ __device__ __forceinline__ float result_factor(float m, float l)
 __device__ __forceinline__ float result_lse(float m, float l)
 {
     return m == -INFINITY ? (l == 0.0f ? -INFINITY : NAN) : kLn2 * (m + log2f(l));
-}
-
-// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row, the worker that
-// has its last tile, and in which of this worker's places it stands; else no request.
-__device__ __forceinline__ void note_cut(const AttendArgs& a, const Part& p, bool cut, uint32_t place)
-{
-    int4 c = make_int4(-1, 0, 0, 0);
-    if (cut) {
-        const uint64_t last_tile = p.next - p.tile + p.tiles - 1;
-        c = make_int4(static_cast<int>(p.request), static_cast<int>(p.row),
-                      static_cast<int>(part_of(p.total, p.workers, last_tile)), static_cast<int>(place));
-    }
-    a.cut[blockIdx.x] = c;
 }
 
 // ------------------------------------------------------------------ any type and head size
@@ -242,17 +259,15 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
     dev::pdl_wait();
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     Part p;
-    if (!find_part<kAttendThreads>(a, part_shared, kTile, &p)) {
+    if (!find_part(a, part_shared, &p)) {
         if (threadIdx.x == 0) {
-            note_cut(a, p, false, 0);
+            a.cut[blockIdx.x] = no_cut();
         }
         return;
     }
     uint32_t place = 0;
-    while (p.next < p.end) {
-        const uint64_t left = p.end - p.next;
-        const uint32_t tiles = left < p.tiles - p.tile ? static_cast<uint32_t>(left) : p.tiles - p.tile;
-        const bool begins = p.tile == 0, ends = p.tile + tiles == p.tiles;
+    for (;;) {
+        const uint32_t tiles = p.piece.last - p.piece.first;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(static_cast<uint32_t>(GH), a.group - chunk * GH);
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         }
         float m = -INFINITY, l = 0.0f;          // of head lane % N / U; l of token lane % U alone
         bool any = false;
-        const uint32_t from = p.span.first + p.tile * kTile;
+        const uint32_t from = p.span.first + p.piece.first * kTile;
         const uint32_t to = min(p.span.end, from + tiles * kTile);
         for (uint32_t at = from + warp * U; at < to; at += kAttendWarps * U) {
             int64_t offset[U];
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
             }
         }
         __syncthreads();
-        const bool whole = begins && ends;
+        const bool whole = tiles == p.tiles;
         const uint32_t at_place = blockIdx.x * 2 + place;
         for (uint32_t g = warp; g < heads; g += kAttendWarps) {
             float2 part[kAttendWarps];
@@ -393,14 +408,14 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
             }
         }
         __syncthreads();
-        if (threadIdx.x == 0 && p.next + tiles == p.end) {
-            note_cut(a, p, begins && !ends, place);
+        const int4 cut = cut_of(p, place);
+        if (!next_row(a, &p)) {
+            if (threadIdx.x == 0) {
+                a.cut[blockIdx.x] = cut;
+            }
+            break;
         }
-        p.next += tiles;
         place = 1;
-        if (p.next < p.end) {
-            next_row(a, kTile, &p);
-        }
     }
 }
 
@@ -527,9 +542,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     }
     dev::pdl_wait();
     Part p;
-    if (!find_part<kAttendThreads>(a, part_shared, kTile, &p)) {
+    if (!find_part(a, part_shared, &p)) {
         if (threadIdx.x == 0) {
-            note_cut(a, p, false, 0);
+            a.cut[blockIdx.x] = no_cut();
         }
         return;
     }
@@ -541,21 +556,20 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
 
     // what is copied runs ahead of what is computed: the next tile to copy, and the tokens that each tile under way has
     Part ahead = p;
-    uint64_t copied = p.next;
+    bool more_rows = true;
     uint32_t tokens_of[STAGES];                 // bit i: token i of this warp's 16 is one
     uint32_t stage_in = 0, stage_out = 0;
     const auto copy_tile = [&]() -> uint32_t {
         uint32_t there = 0;
-        if (copied < ahead.end) {
+        if (more_rows) {
             const uint32_t key_head = quotient(a.by_chunks, ahead.row);
             const int32_t* table = a.tables + ahead.request * a.table_stride;
-            const uint32_t token = ahead.span.first + ahead.tile * kTile + warp * kWarpTokens + lane % kWarpTokens;
+            const uint32_t token = ahead.span.first + ahead.piece.first * kTile + warp * kWarpTokens + lane % kWarpTokens;
             int64_t offset = token < ahead.span.end ? token_offset(a, table, token) : -1;
             there = __ballot_sync(~0u, offset >= 0) & 0xffffu;
             offset = offset >= 0 ? offset + key_head * a.page_head_stride : 0;
             const uint32_t to = stage_base + stage_in * Shape::kStageBytes;
-            for (uint32_t k = 0; k < kWarpTokens * chunks; k += 32) {
-                const uint32_t i = k + lane, r = quotient(a.by_vector, i), c = i - r * a.by_vector.d;   // r <= 16
+            const auto copy_chunk = [&](uint32_t r, uint32_t c) {
                 const int64_t from = __shfl_sync(~0u, offset, r) + c * 16;
                 const uint32_t at = to + r * Shape::kRowBytes + ((c ^ (r % 8)) * 16);
                 const bool is = (there >> r & 1) != 0;
@@ -565,10 +579,21 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                         copy_16(at + Shape::kPlaneBytes, a.planes[1] + from, is);
                     }
                 }
+            };
+            constexpr uint32_t kChunks = DP / 8;
+            if (32 % kChunks == 0 && chunks == kChunks) {
+#pragma unroll
+                for (uint32_t k = 0; k < kWarpTokens * kChunks / 32; ++k) {
+                    copy_chunk(k * (32 / kChunks) + lane / kChunks, lane % kChunks);
+                }
+            } else {
+                for (uint32_t k = 0; k < kWarpTokens * chunks; k += 32) {
+                    const uint32_t r = quotient(a.by_vector, k + lane);             // at most 16
+                    copy_chunk(r, k + lane - r * a.by_vector.d);
+                }
             }
-            ++copied;
-            if (copied < ahead.end && ++ahead.tile == ahead.tiles) {
-                next_row(a, kTile, &ahead);
+            if (++ahead.piece.first == ahead.piece.last) {
+                more_rows = next_row(a, &ahead);
             }
         }
         copies_end();
@@ -581,10 +606,8 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     }
 
     uint32_t place = 0, turn = 0;
-    while (p.next < p.end) {
-        const uint64_t left = p.end - p.next;
-        const uint32_t tiles = left < p.tiles - p.tile ? static_cast<uint32_t>(left) : p.tiles - p.tile;
-        const bool begins = p.tile == 0, ends = p.tile + tiles == p.tiles;
+    for (;;) {
+        const uint32_t tiles = p.piece.last - p.piece.first;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(GH, a.group - chunk * GH);
@@ -795,7 +818,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
             }
         }
         __syncthreads();
-        const bool whole = begins && ends;
+        const bool whole = tiles == p.tiles;
         const uint32_t at_place = blockIdx.x * 2 + place;
         for (uint32_t g = warp; g < heads; g += kAttendWarps) {
             float2 part[kAttendWarps];
@@ -828,30 +851,37 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
             }
         }
-        if (threadIdx.x == 0 && p.next + tiles == p.end) {
-            note_cut(a, p, begins && !ends, place);
+        const int4 cut = cut_of(p, place);
+        if (!next_row(a, &p)) {
+            if (threadIdx.x == 0) {
+                a.cut[blockIdx.x] = cut;
+            }
+            break;
         }
-        p.next += tiles;
         place = 1;
-        if (p.next < p.end) {
-            next_row(a, kTile, &p);
-        }
     }
     copies_wait<0>();
 }
 
 // ------------------------------------------------------------------ joining
 //
-// Block (c, g): query head g of the row that begins in worker c's part and is cut, if there is one: worker c's last
-// place, then the first place of all workers up to the row's last one, in four shares, one a warp.
+// Block (c, g): query head g of the row that begins in worker c's part and is cut, if there is one: worker c's place
+// of it, then the first place of all workers up to the row's last one. A thread has four values; where a head has fewer
+// than the block's threads hold, groups of threads share the pieces. The first pieces are on their way before their weights
+// are known: the kernel is a chain of a few trips to L2.
+
+constexpr uint32_t kMostWorkers = 4 * 148;
+constexpr uint32_t kJoinAhead = 4;
 
 template <class T>
 __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_constant__ AttendArgs a, uint32_t gh)
 {
-    __shared__ float2 merge_sums[kAttendWarps];
+    __shared__ float weights[kMostWorkers];
+    __shared__ float tops[kAttendWarps], sums[kAttendWarps];
+    __shared__ float4 merge[kAttendThreads];
     dev::pdl_release();
     dev::pdl_wait();
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t t = threadIdx.x, lane = t % 32, warp = t / 32;
     const uint32_t c = blockIdx.x, g = blockIdx.y;
     const int4 cut = a.cut[c];
     if (cut.x < 0) {
@@ -861,62 +891,114 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
     if (chunk * gh + g >= a.group) {
         return;
     }
-    extern __shared__ float merge[];            // [warps][value_pad]
     const uint32_t head = key_head * a.group + chunk * gh + g;
     const uint32_t pieces = cut.z - c + 1;
     const auto place = [&](uint32_t k) { return (k == 0 ? uint64_t{c} * 2 + cut.w : (uint64_t{c} + k) * 2) * gh + g; };
+    // columns of four values, and the groups of threads that share the pieces of one
+    const uint32_t columns = a.value_pad / 4;
+    const uint32_t groups = columns >= kAttendThreads ? 1 : kAttendThreads / columns;
+    const uint32_t column = columns >= kAttendThreads ? t : t % columns, group = columns >= kAttendThreads ? 0 : t / columns;
+    const auto value = [&](uint32_t k, uint32_t x) {
+        return *reinterpret_cast<const float4*>(a.partial + place(k) * a.value_pad + x * 4);
+    };
+    float4 ahead[kJoinAhead];
+    const bool works = group < groups && column < columns;
+#pragma unroll
+    for (uint32_t i = 0; i < kJoinAhead; ++i) {
+        const uint32_t k = group + i * groups;
+        ahead[i] = works && k < pieces ? value(k, column) : make_float4(0, 0, 0, 0);
+    }
     float top = -INFINITY;
-    for (uint32_t k = threadIdx.x; k < pieces; k += kAttendThreads) {
-        top = fmaxf(top, a.partial_sums[place(k)].x);
+    for (uint32_t k = t; k < pieces; k += kAttendThreads) {
+        const float2 x = a.partial_sums[place(k)];
+        weights[k] = x.x;
+        top = fmaxf(top, x.x);
     }
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
         top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     }
     if (lane == 0) {
-        merge_sums[warp].x = top;
+        tops[warp] = top;
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < kAttendWarps; ++w) {
-        top = fmaxf(top, merge_sums[w].x);
+        top = fmaxf(top, tops[w]);
     }
     const float base = reference(top);
-    const auto weight = [&](uint32_t k) { return top == -INFINITY ? 1.0f : exp2f(a.partial_sums[place(k)].x - base); };
     float sum = 0.0f;
-    for (uint32_t k = warp; k < pieces; k += kAttendWarps) {
-        sum += a.partial_sums[place(k)].y * weight(k);
+    for (uint32_t k = t; k < pieces; k += kAttendThreads) {
+        const float w = top == -INFINITY ? 1.0f : exp2f(weights[k] - base);
+        weights[k] = w;
+        sum += a.partial_sums[place(k)].y * w;
     }
-    __syncthreads();
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) {
+        sum += __shfl_xor_sync(~0u, sum, d);
+    }
     if (lane == 0) {
-        merge_sums[warp].y = sum;
-    }
-    for (uint32_t d = lane; d < a.value_dim; d += 32) {
-        float x = 0.0f;
-#pragma unroll 4
-        for (uint32_t k = warp; k < pieces; k += kAttendWarps) {
-            x = fmaf(a.partial[place(k) * a.value_pad + d], weight(k), x);
-        }
-        merge[warp * a.value_pad + d] = x;
+        sums[warp] = sum;
     }
     __syncthreads();
     sum = 0.0f;
 #pragma unroll
     for (uint32_t w = 0; w < kAttendWarps; ++w) {
-        sum += merge_sums[w].y;
+        sum += sums[w];
     }
     const float factor = result_factor(top, sum);
     const uint32_t request = cut.x;
     T* out = reinterpret_cast<T*>(a.out + request * a.out_stride + head * a.out_head_stride);
-    for (uint32_t d = threadIdx.x; d < a.value_dim; d += kAttendThreads) {
-        float x = 0.0f;
+    const auto fold = [](float4& s, float w, const float4& v) {
+        s.x = fmaf(w, v.x, s.x);
+        s.y = fmaf(w, v.y, s.y);
+        s.z = fmaf(w, v.z, s.z);
+        s.w = fmaf(w, v.w, s.w);
+    };
+    const auto write = [&](uint32_t x, const float4& s) {
+        const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (uint32_t w = 0; w < kAttendWarps; ++w) {
-            x += merge[w * a.value_pad + d];
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (x * 4 + i < a.value_dim) {
+                out[x * 4 + i] = from_float<T>(v[i] * factor);
+            }
         }
-        out[d] = from_float<T>(x * factor);
+    };
+    float4 s = make_float4(0, 0, 0, 0);
+    if (works) {
+#pragma unroll
+        for (uint32_t i = 0; i < kJoinAhead; ++i) {
+            const uint32_t k = group + i * groups;
+            if (k < pieces) {
+                fold(s, weights[k], ahead[i]);
+            }
+        }
+#pragma unroll 4
+        for (uint32_t k = group + kJoinAhead * groups; k < pieces; k += groups) {
+            fold(s, weights[k], value(k, column));
+        }
     }
-    if (threadIdx.x == 0 && a.lse != nullptr) {
+    if (groups > 1) {
+        merge[t] = s;
+        __syncthreads();
+        if (group == 0) {
+            for (uint32_t i = 1; i < groups; ++i) {
+                fold(s, 1.0f, merge[i * columns + column]);
+            }
+        }
+    }
+    if (works && group == 0) {
+        write(column, s);
+    }
+    // vectors of more than 512 values: the columns that are left
+    for (uint32_t x = column + kAttendThreads; groups == 1 && x < columns; x += kAttendThreads) {
+        float4 more = make_float4(0, 0, 0, 0);
+        for (uint32_t k = 0; k < pieces; ++k) {
+            fold(more, weights[k], value(k, x));
+        }
+        write(x, more);
+    }
+    if (t == 0 && a.lse != nullptr) {
         a.lse[request * a.lse_stride + head] = result_lse(top, sum);
     }
 }

@@ -412,8 +412,8 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.chunks = (a.group + plan.heads - 1) / plan.heads;
     a.rows = l.heads * a.chunks;
     a.limit = kv::row_limit(t.width, pages->block_size);
-    // the tiles of all rows have to be countable
-    if (uint64_t{t.requests} * a.rows >= (uint64_t{1} << 51) / (a.limit / kv::kTile + 1)) {
+    // the units of all rows have to be countable
+    if (uint64_t{t.requests} * a.rows >= (uint64_t{1} << 51) / (a.limit / kv::kTile + 1 + kv::kRowUnits)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     DeviceGuard guard(device);
@@ -460,8 +460,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     }
     e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, plan.shared, s, a);
     if (e == cudaSuccess) {
-        e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads,
-                   static_cast<uint32_t>(kv::kAttendWarps * a.value_pad * sizeof(float)), s, a, plan.heads);
+        e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads, 0, s, a, plan.heads);
     }
     return cuda_rc(e);
 }

@@ -88,14 +88,41 @@ KV_HD uint32_t tiles_of(const Span& s, uint32_t tile)
     return n == 0 ? 1u : (n + tile - 1) / tile;
 }
 
-// The tiles of all rows, one row behind the other, are cut into equal parts for `workers` <= total workers: worker
-// c has the tiles [part_start(c), part_start(c + 1)), one at least. total < 2^52, workers < 2^11.
+// Attention's work is counted in units: a row's tiles, and kRowUnits in front of them for its beginning and its end. The units of all rows, one row
+// behind the other, are cut into equal parts for `workers` <= total workers: worker c has the units [part_start(c),
+// part_start(c + 1)), one at least. total < 2^52, workers < 2^11.
+constexpr uint32_t kRowUnits = 3;
+
 KV_HD uint64_t part_start(uint64_t total, uint32_t workers, uint32_t c) { return total * c / workers; }
 
-// The worker that has a tile: the largest c with total c / workers < tile + 1.
-KV_HD uint32_t part_of(uint64_t total, uint32_t workers, uint64_t tile)
+// The worker that has a unit: the largest c with total c / workers < unit + 1.
+KV_HD uint32_t part_of(uint64_t total, uint32_t workers, uint64_t unit)
 {
-    return static_cast<uint32_t>(((tile + 1) * workers - 1) / total);
+    return static_cast<uint32_t>(((unit + 1) * workers - 1) / total);
+}
+
+// Few units are shared by fewer workers: cutting a row costs more than some tiles do.
+constexpr uint32_t kLeastUnits = 4;
+
+KV_HD uint32_t workers_for(uint64_t total, uint32_t most)
+{
+    const uint64_t n = total / kLeastUnits;
+    return n == 0 ? 1u : (n < most ? static_cast<uint32_t>(n) : most);
+}
+
+// The tiles [first, last) of a row that a part [begin, end) has, all counted from the row's first unit (`begin` may lie before
+// it). A part that ends in the units in front of the tiles has none; the next one then begins the row.
+struct Piece {
+    uint32_t first, last;
+};
+
+KV_HD Piece piece_of(int64_t begin, int64_t end, uint32_t tiles)
+{
+    const int64_t a = begin - kRowUnits, b = end - kRowUnits;
+    Piece p{};
+    p.first = a <= 0 ? 0u : static_cast<uint32_t>(a);
+    p.last = b <= 0 ? 0u : (b < tiles ? static_cast<uint32_t>(b) : tiles);
+    return p;
 }
 
 }  // namespace kv

@@ -42,6 +42,59 @@ void spans(const int32_t* length, int n, uint32_t limit, uint32_t window, uint32
     }
 }
 
+// 0 where the rows (of so many tiles each) are cut as join_kernel takes it: every tile is one worker's; a row that is cut
+// begins in one worker and goes on in the next ones, without a gap, to the one that part_of names for its last unit, and is in each of these
+// the first row that has tiles there.
+int check_rows(const uint32_t* tiles, int rows, uint32_t most)
+{
+    uint64_t total = 0;
+    for (int r = 0; r < rows; ++r) {
+        total += tiles[r] + kRowUnits;
+    }
+    const uint32_t workers = workers_for(total, most);
+    if (workers > total || workers > most) {
+        return 1;
+    }
+    uint64_t row_begin = 0;
+    for (int r = 0; r < rows; ++r) {
+        uint32_t next = 0, begun = 0, last = 0;
+        for (uint32_t c = 0; c < workers; ++c) {
+            const uint64_t a = part_start(total, workers, c), b = part_start(total, workers, c + 1);
+            if (b <= row_begin || a >= row_begin + tiles[r] + kRowUnits) {
+                continue;
+            }
+            const Piece p = piece_of(static_cast<int64_t>(a) - static_cast<int64_t>(row_begin),
+                                     static_cast<int64_t>(b) - static_cast<int64_t>(row_begin), tiles[r]);
+            if (p.last <= p.first) {
+                if (next != 0) {
+                    return 2;               // a gap within the row
+                }
+                continue;
+            }
+            if (p.first != next) {
+                return 3;
+            }
+            if (p.first == 0) {
+                begun = c;
+            } else if (c != last + 1) {
+                return 4;
+            } else if (a < row_begin) {
+                return 5;                   // not the first row with tiles
+            }
+            next = p.last;
+            last = c;
+        }
+        if (next != tiles[r]) {
+            return 6;
+        }
+        if (last != begun && part_of(total, workers, row_begin + kRowUnits + tiles[r] - 1) != last) {
+            return 7;
+        }
+        row_begin += tiles[r] + kRowUnits;
+    }
+    return 0;
+}
+
 // 0 where all parts of `total` tiles are right: none empty, one behind the other, sizes at most one apart, every tile's worker
 // the one whose part it lies in (at the parts' ends, and at every tile where there are few)
 int check_parts(uint64_t total, uint32_t workers)
