@@ -49,8 +49,8 @@ struct AttendArgs {
 //
 // The rows' units (tiles, and some for a row's beginning and end), one row behind the other, are cut into equal parts, one a worker
 // (a block): few long rows and many short ones keep all SMs busy alike, whatever the lengths, which only the device
-// knows. A worker that has a whole row writes its result; of a row that is cut each worker writes what it has of it, its
-// first row's in place 0 and another's in place 1, and join_kernel puts them together.
+// knows. A worker that has a whole row writes its result; of a row that is cut each worker writes what it has of it, into its place 1
+// where the row begins in its part and into its place 0 where it goes on there, and join_kernel puts them together.
 
 struct PartShared {
     uint64_t warp[kAttendWarps];
@@ -72,13 +72,13 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v)
     return v;
 }
 
-// A worker's part, and a row of it with the tiles [piece.first, piece.last) that are the worker's.
+// A worker's part, and a row of it with the tiles [first, last) that are the worker's.
 struct Part {
     uint64_t begin, end, total, row_begin;      // units; row_begin: the row's first
     uint32_t workers;
     uint32_t request, row, tiles;
     Span span;
-    Piece piece;
+    uint32_t first, last;
 };
 
 __device__ __forceinline__ void set_row(const AttendArgs& a, Part* p)
@@ -87,17 +87,11 @@ __device__ __forceinline__ void set_row(const AttendArgs& a, Part* p)
     p->tiles = tiles_of(p->span, kTile);
 }
 
-__device__ __forceinline__ void set_piece(Part* p)
-{
-    p->piece = piece_of(static_cast<int64_t>(p->begin) - static_cast<int64_t>(p->row_begin),
-                        static_cast<int64_t>(p->end) - static_cast<int64_t>(p->row_begin), p->tiles);
-}
-
 // On to the part's next row; false where it has no tiles of any other.
 __device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
 {
     p->row_begin += p->tiles + kRowUnits;
-    if (p->row_begin + kRowUnits >= p->end) {
+    if (p->row_begin >= p->end) {
         return false;
     }
     if (++p->row == a.rows) {
@@ -105,8 +99,9 @@ __device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
         ++p->request;
         set_row(a, p);
     }
-    set_piece(p);
-    return true;
+    p->first = 0;
+    p->last = cut_at(static_cast<int64_t>(p->end - p->row_begin), p->tiles);
+    return p->last != 0;
 }
 
 // Every thread gets the same; false for a worker that has no tiles.
@@ -172,21 +167,9 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
     const uint64_t in = p->begin - s.found_sum, units = p->tiles + kRowUnits;
     p->row = static_cast<uint32_t>(in / units);
     p->row_begin = s.found_sum + p->row * units;
-    set_piece(p);
-    return p->piece.last > p->piece.first;
-}
-
-// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row, the worker that
-// has its last tile, and in which of this worker's places it stands; else no request.
-__device__ __forceinline__ int4 no_cut() { return make_int4(-1, 0, 0, 0); }
-
-__device__ __forceinline__ int4 cut_of(const Part& p, uint32_t place)
-{
-    if (p.piece.first != 0 || p.piece.last == p.tiles) {
-        return no_cut();
-    }
-    return make_int4(static_cast<int>(p.request), static_cast<int>(p.row),
-                     static_cast<int>(part_of(p.total, p.workers, p.row_begin + kRowUnits + p.tiles - 1)), static_cast<int>(place));
+    p->first = cut_at(static_cast<int64_t>(p->begin - p->row_begin), p->tiles);
+    p->last = cut_at(static_cast<int64_t>(p->end - p->row_begin), p->tiles);
+    return p->last > p->first || next_row(a, p);
 }
 
 // The vector of a token: where it starts in its plane, or -1 where its block is not one of the cache's.
@@ -214,6 +197,19 @@ __device__ __forceinline__ float result_factor(float m, float l)
 __device__ __forceinline__ float result_lse(float m, float l)
 {
     return m == -INFINITY ? (l == 0.0f ? -INFINITY : NAN) : kLn2 * (m + log2f(l));
+}
+
+// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row and the worker that
+// ends it; else no request.
+__device__ __forceinline__ int4 no_cut() { return make_int4(-1, 0, 0, 0); }
+
+__device__ __forceinline__ int4 cut_of(const Part& p)
+{
+    if (p.first != 0 || p.last == p.tiles) {
+        return no_cut();
+    }
+    return make_int4(static_cast<int>(p.request), static_cast<int>(p.row),
+                     static_cast<int>(part_of(p.total, p.workers, p.row_begin + last_units(p.tiles))), 0);
 }
 
 // ------------------------------------------------------------------ any type and head size
@@ -265,9 +261,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         }
         return;
     }
-    uint32_t place = 0;
     for (;;) {
-        const uint32_t tiles = p.piece.last - p.piece.first;
+        const uint32_t tiles = p.last - p.first;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(static_cast<uint32_t>(GH), a.group - chunk * GH);
@@ -285,7 +280,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         }
         float m = -INFINITY, l = 0.0f;          // of head lane % N / U; l of token lane % U alone
         bool any = false;
-        const uint32_t from = p.span.first + p.piece.first * kTile;
+        const uint32_t from = p.span.first + p.first * kTile;
         const uint32_t to = min(p.span.end, from + tiles * kTile);
         for (uint32_t at = from + warp * U; at < to; at += kAttendWarps * U) {
             int64_t offset[U];
@@ -367,7 +362,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         }
         __syncthreads();
         const bool whole = tiles == p.tiles;
-        const uint32_t at_place = blockIdx.x * 2 + place;
+        const uint32_t at_place = blockIdx.x * 2 + (p.first == 0 ? 1 : 0);
         for (uint32_t g = warp; g < heads; g += kAttendWarps) {
             float2 part[kAttendWarps];
             float top = -INFINITY;
@@ -407,15 +402,14 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
                 }
             }
         }
-        __syncthreads();
-        const int4 cut = cut_of(p, place);
+        const int4 cut = cut_of(p);
         if (!next_row(a, &p)) {
             if (threadIdx.x == 0) {
                 a.cut[blockIdx.x] = cut;
             }
             break;
         }
-        place = 1;
+        __syncthreads();
     }
 }
 
@@ -564,7 +558,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
         if (more_rows) {
             const uint32_t key_head = quotient(a.by_chunks, ahead.row);
             const int32_t* table = a.tables + ahead.request * a.table_stride;
-            const uint32_t token = ahead.span.first + ahead.piece.first * kTile + warp * kWarpTokens + lane % kWarpTokens;
+            const uint32_t token = ahead.span.first + ahead.first * kTile + warp * kWarpTokens + lane % kWarpTokens;
             int64_t offset = token < ahead.span.end ? token_offset(a, table, token) : -1;
             there = __ballot_sync(~0u, offset >= 0) & 0xffffu;
             offset = offset >= 0 ? offset + key_head * a.page_head_stride : 0;
@@ -592,7 +586,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                     copy_chunk(r, k + lane - r * a.by_vector.d);
                 }
             }
-            if (++ahead.piece.first == ahead.piece.last) {
+            if (++ahead.first == ahead.last) {
                 more_rows = next_row(a, &ahead);
             }
         }
@@ -605,9 +599,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
         tokens_of[k] = copy_tile();
     }
 
-    uint32_t place = 0, turn = 0;
+    uint32_t turn = 0;
     for (;;) {
-        const uint32_t tiles = p.piece.last - p.piece.first;
+        const uint32_t tiles = p.last - p.first;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(GH, a.group - chunk * GH);
@@ -819,7 +813,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
         }
         __syncthreads();
         const bool whole = tiles == p.tiles;
-        const uint32_t at_place = blockIdx.x * 2 + place;
+        const uint32_t at_place = blockIdx.x * 2 + (p.first == 0 ? 1 : 0);
         for (uint32_t g = warp; g < heads; g += kAttendWarps) {
             float2 part[kAttendWarps];
             float top = -INFINITY, sum = 0.0f;
@@ -851,22 +845,21 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
             }
         }
-        const int4 cut = cut_of(p, place);
+        const int4 cut = cut_of(p);
         if (!next_row(a, &p)) {
             if (threadIdx.x == 0) {
                 a.cut[blockIdx.x] = cut;
             }
             break;
         }
-        place = 1;
     }
     copies_wait<0>();
 }
 
 // ------------------------------------------------------------------ joining
 //
-// Block (c, g): query head g of the row that begins in worker c's part and is cut, if there is one: worker c's place
-// of it, then the first place of all workers up to the row's last one. A thread has four values; where a head has fewer
+// Block (c, g): query head g of the row that begins in worker c's part and is cut, if there is one: worker c's place 1,
+// then place 0 of all workers up to the row's last one. A thread has four values; where a head has fewer
 // than the block's threads hold, groups of threads share the pieces. The first pieces are on their way before their weights
 // are known: the kernel is a chain of a few trips to L2.
 
@@ -893,7 +886,7 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
     }
     const uint32_t head = key_head * a.group + chunk * gh + g;
     const uint32_t pieces = cut.z - c + 1;
-    const auto place = [&](uint32_t k) { return (k == 0 ? uint64_t{c} * 2 + cut.w : (uint64_t{c} + k) * 2) * gh + g; };
+    const auto place = [&](uint32_t k) { return (uint64_t{c + k} * 2 + (k == 0 ? 1 : 0)) * gh + g; };
     // columns of four values, and the groups of threads that share the pieces of one
     const uint32_t columns = a.value_pad / 4;
     const uint32_t groups = columns >= kAttendThreads ? 1 : kAttendThreads / columns;

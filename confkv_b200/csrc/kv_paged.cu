@@ -160,6 +160,7 @@ struct AttendPlan {
 };
 
 constexpr uint32_t kSms = 148;
+static_assert(4 * kSms <= kv::kMostWorkers);
 
 template <class T>
 AttendPlan any_plan(uint32_t head_dim, uint32_t group)
@@ -459,7 +460,9 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
         return LMCACHE_GPU_AESGCM_ERR_CUDA;
     }
     e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, plan.shared, s, a);
-    if (e == cudaSuccess) {
+    // rows that no length makes long enough to be cut need no joining
+    const uint32_t most = t.window != 0 ? std::min(t.window, a.limit) : a.limit;
+    if (e == cudaSuccess && kv::tiles_of(kv::Span{0, most}, kv::kTile) > kv::kWholeTiles) {
         e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads, 0, s, a, plan.heads);
     }
     return cuda_rc(e);

@@ -110,19 +110,26 @@ KV_HD uint32_t workers_for(uint64_t total, uint32_t most)
     return n == 0 ? 1u : (n < most ? static_cast<uint32_t>(n) : most);
 }
 
-// The tiles [first, last) of a row that a part [begin, end) has, all counted from the row's first unit (`begin` may lie before
-// it). A part that ends in the units in front of the tiles has none; the next one then begins the row.
-struct Piece {
-    uint32_t first, last;
-};
+// Where a part's border at `x` units behind a row's first one (or before it) cuts the row: in front of which tile. A row of few tiles stays
+// whole, and no border leaves a few tiles alone: the pieces of a cut row have to be written, counted and joined.
+constexpr uint32_t kWholeTiles = 8;
+constexpr uint32_t kLeastTiles = 2;
 
-KV_HD Piece piece_of(int64_t begin, int64_t end, uint32_t tiles)
+KV_HD uint32_t first_units(uint32_t tiles)      // up to there a border lies in front of the row
 {
-    const int64_t a = begin - kRowUnits, b = end - kRowUnits;
-    Piece p{};
-    p.first = a <= 0 ? 0u : static_cast<uint32_t>(a);
-    p.last = b <= 0 ? 0u : (b < tiles ? static_cast<uint32_t>(b) : tiles);
-    return p;
+    return tiles <= kWholeTiles ? (tiles + kRowUnits) / 2 : kRowUnits + kLeastTiles;
+}
+
+KV_HD uint32_t last_units(uint32_t tiles)       // beyond there it lies behind the row
+{
+    return tiles <= kWholeTiles ? (tiles + kRowUnits) / 2 : kRowUnits + tiles - kLeastTiles - 1;
+}
+
+KV_HD uint32_t cut_at(int64_t x, uint32_t tiles)
+{
+    return x <= static_cast<int64_t>(first_units(tiles)) ? 0u
+           : x > static_cast<int64_t>(last_units(tiles)) ? tiles
+                                                         : static_cast<uint32_t>(x) - kRowUnits;
 }
 
 }  // namespace kv

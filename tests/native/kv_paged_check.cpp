@@ -42,9 +42,9 @@ void spans(const int32_t* length, int n, uint32_t limit, uint32_t window, uint32
     }
 }
 
-// 0 where the rows (of so many tiles each) are cut as join_kernel takes it: every tile is one worker's; a row that is cut
-// begins in one worker and goes on in the next ones, without a gap, to the one that part_of names for its last unit, and is in each of these
-// the first row that has tiles there.
+// 0 where the rows (of so many tiles each) are cut as joining takes it: every tile is one worker's; a row begins in the worker that
+// part_of names for first_units, goes on in the next ones without a gap, and ends in the one named for last_units; rows of few
+// tiles are whole, and no piece of another is shorter than kLeastTiles but between two borders.
 int check_rows(const uint32_t* tiles, int rows, uint32_t most)
 {
     uint64_t total = 0;
@@ -57,38 +57,35 @@ int check_rows(const uint32_t* tiles, int rows, uint32_t most)
     }
     uint64_t row_begin = 0;
     for (int r = 0; r < rows; ++r) {
-        uint32_t next = 0, begun = 0, last = 0;
+        const uint32_t begins = part_of(total, workers, row_begin + first_units(tiles[r]));
+        const uint32_t ends = part_of(total, workers, row_begin + last_units(tiles[r]));
+        uint32_t next = 0;
         for (uint32_t c = 0; c < workers; ++c) {
-            const uint64_t a = part_start(total, workers, c), b = part_start(total, workers, c + 1);
-            if (b <= row_begin || a >= row_begin + tiles[r] + kRowUnits) {
+            const int64_t a = static_cast<int64_t>(part_start(total, workers, c)) - static_cast<int64_t>(row_begin);
+            const int64_t b = static_cast<int64_t>(part_start(total, workers, c + 1)) - static_cast<int64_t>(row_begin);
+            if (b <= 0 || a >= static_cast<int64_t>(tiles[r] + kRowUnits)) {
                 continue;
             }
-            const Piece p = piece_of(static_cast<int64_t>(a) - static_cast<int64_t>(row_begin),
-                                     static_cast<int64_t>(b) - static_cast<int64_t>(row_begin), tiles[r]);
-            if (p.last <= p.first) {
-                if (next != 0) {
-                    return 2;               // a gap within the row
-                }
+            const uint32_t first = cut_at(a, tiles[r]), last = cut_at(b, tiles[r]);
+            if ((last > first) != (c >= begins && c <= ends)) {
+                return 2;
+            }
+            if (last <= first) {
                 continue;
             }
-            if (p.first != next) {
+            if (first != next) {
                 return 3;
             }
-            if (p.first == 0) {
-                begun = c;
-            } else if (c != last + 1) {
+            if ((first == 0 || last == tiles[r]) && last - first < (tiles[r] < kLeastTiles ? tiles[r] : kLeastTiles)) {
                 return 4;
-            } else if (a < row_begin) {
-                return 5;                   // not the first row with tiles
             }
-            next = p.last;
-            last = c;
+            next = last;
         }
         if (next != tiles[r]) {
-            return 6;
+            return 5;
         }
-        if (last != begun && part_of(total, workers, row_begin + kRowUnits + tiles[r] - 1) != last) {
-            return 7;
+        if (tiles[r] <= kWholeTiles && begins != ends) {
+            return 6;
         }
         row_begin += tiles[r] + kRowUnits;
     }
