@@ -214,9 +214,9 @@ __device__ __forceinline__ int4 cut_of(const Part& p)
 
 // ------------------------------------------------------------------ any type and head size
 //
-// Each warp takes U tokens at a time; a lane has values lane, lane + 32, .. of the vectors, R of them, and of GH query heads. The
-// products of GH U scores are summed over the lanes by halving: a lane passes on half of its sums at each step and ends with
-// one score (31 exchanges for 32 scores).
+// Each warp takes U tokens at a time. A lane has R values of a vector, in steps of VEC that follow one another (one load, where head size
+// and addresses allow), and of GH query heads. The products of GH U scores are summed over the lanes by halving: a lane passes on
+// half of its sums at each step and ends with one score (31 exchanges for 32 scores).
 
 // Sums of N values over the warp's lanes: lane i returns the sum of value i % N.
 template <int N>
@@ -244,10 +244,15 @@ __device__ __forceinline__ float lane_sums(float (&v)[N])
     return v[0];
 }
 
-template <class T, int R, int GH, int U>
-__global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid_constant__ AttendArgs a)
+template <class T, int VEC>
+struct alignas(sizeof(T) * VEC) Values {
+    T x[VEC];
+};
+
+template <class T, int VEC, int R, int GH, int U, int BLOCKS>
+__global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(const __grid_constant__ AttendArgs a)
 {
-    constexpr int N = GH * U;
+    constexpr int N = GH * U, STEPS = R / VEC;
     __shared__ PartShared part_shared;
     __shared__ float merge[kAttendWarps][GH][R * 32];
     __shared__ float2 merge_sums[kAttendWarps][GH];
@@ -261,46 +266,62 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         }
         return;
     }
+    const bool one = a.planes[0] == a.planes[1];
     for (;;) {
         const uint32_t tiles = p.last - p.first;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(static_cast<uint32_t>(GH), a.group - chunk * GH);
         const int32_t* table = a.tables + p.request * a.table_stride;
+        const uint32_t from = p.span.first + p.first * kTile;
+        const uint32_t to = min(p.span.end, from + tiles * kTile);
+        // where the warp's next U tokens lie; the table is read one turn ahead
+        int64_t offset[U];
+        const auto find_tokens = [&](uint32_t at) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                offset[u] = at + u < to ? token_offset(a, table, at + u) : -1;
+            }
+        };
+        find_tokens(from + warp * U);
         float q[GH][R], o[GH][R];
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-            const T* from = reinterpret_cast<const T*>(a.query + p.request * a.query_stride + (head + g) * a.query_head_stride);
+            const T* query = reinterpret_cast<const T*>(a.query + p.request * a.query_stride + (head + g) * a.query_head_stride);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const uint32_t d = lane + 32 * i;
-                q[g][i] = static_cast<uint32_t>(g) < heads && d < a.head_dim ? to_float(from[d]) * a.scale : 0.0f;
+                const uint32_t d = (lane + i / VEC * 32) * VEC + i % VEC;
+                q[g][i] = static_cast<uint32_t>(g) < heads && d < a.head_dim ? to_float(query[d]) * a.scale : 0.0f;
                 o[g][i] = 0.0f;
             }
         }
         float m = -INFINITY, l = 0.0f;          // of head lane % N / U; l of token lane % U alone
         bool any = false;
-        const uint32_t from = p.span.first + p.first * kTile;
-        const uint32_t to = min(p.span.end, from + tiles * kTile);
         for (uint32_t at = from + warp * U; at < to; at += kAttendWarps * U) {
-            int64_t offset[U];
+            Values<T, VEC> k[U][STEPS], v[U][STEPS];
+            uint32_t there = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                offset[u] = at + u < to ? token_offset(a, table, at + u) : -1;
-                any |= offset[u] >= 0;
-                offset[u] += offset[u] >= 0 ? key_head * a.page_head_stride : 0;
-            }
-            float k[U][R], v[U][R];
+                const bool is = offset[u] >= 0;
+                there |= is ? 1u << u : 0u;
+                const int64_t where = offset[u] + key_head * a.page_head_stride;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+                for (int i = 0; i < STEPS; ++i) {
+                    const uint32_t d = (lane + i * 32) * VEC;
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const uint32_t d = lane + 32 * i;
-                    const bool there = offset[u] >= 0;
-                    k[u][i] = there && d < a.head_dim ? to_float(reinterpret_cast<const T*>(a.planes[0] + offset[u])[d]) : 0.0f;
-                    v[u][i] = there && d < a.value_dim ? to_float(reinterpret_cast<const T*>(a.planes[1] + offset[u])[d]) : 0.0f;
+                    for (int j = 0; j < VEC; ++j) {
+                        k[u][i].x[j] = v[u][i].x[j] = from_float<T>(0.0f);
+                    }
+                    if (is && d < a.head_dim) {
+                        k[u][i] = *reinterpret_cast<const Values<T, VEC>*>(a.planes[0] + where + d * sizeof(T));
+                        if (!one) {
+                            v[u][i] = *reinterpret_cast<const Values<T, VEC>*>(a.planes[1] + where + d * sizeof(T));
+                        }
+                    }
                 }
             }
+            any |= there != 0;
+            find_tokens(at + kAttendWarps * U);
             float s[N];
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
@@ -309,16 +330,13 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
                     float x = 0.0f;
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
-                        x = fmaf(q[g][i], k[u][i], x);
+                        x = fmaf(q[g][i], to_float(k[u][i / VEC].x[i % VEC]), x);
                     }
                     s[g * U + u] = x;
                 }
             }
             float score = lane_sums<N>(s);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                score = lane % U == u && offset[u] < 0 ? -INFINITY : score;
-            }
+            score = (there >> (lane % U) & 1) != 0 ? score : -INFINITY;
             float top = score;
 #pragma unroll
             for (int d = 1; d < U; d *= 2) {
@@ -340,7 +358,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
                     const float w = __shfl_sync(~0u, weight, g * U + u);
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
-                        o[g][i] = fmaf(w, v[u][i], o[g][i]);
+                        const T y = one ? k[u][i / VEC].x[i % VEC] : v[u][i / VEC].x[i % VEC];
+                        o[g][i] = fmaf(w, to_float(y), o[g][i]);
                     }
                 }
             }
@@ -357,7 +376,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_any_kernel(const __grid
         for (int g = 0; g < GH; ++g) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                merge[warp][g][lane + 32 * i] = o[g][i];
+                merge[warp][g][(lane + i / VEC * 32) * VEC + i % VEC] = o[g][i];
             }
         }
         __syncthreads();

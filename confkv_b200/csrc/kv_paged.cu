@@ -162,26 +162,26 @@ struct AttendPlan {
 constexpr uint32_t kSms = 148;
 static_assert(4 * kSms <= kv::kMostWorkers);
 
-template <class T>
-AttendPlan any_plan(uint32_t head_dim, uint32_t group)
+template <class T, int VEC, int R, int GH, int U, int BLOCKS>
+AttendPlan any_plan()
 {
-    AttendPlan p{};
-    p.join = kv::join_kernel<T>;
-    p.workers = 4 * kSms;
-    if (head_dim <= 64) {
-        p.heads = group > 1 ? 8 : 1;
-        p.kernel = group > 1 ? kv::attend_any_kernel<T, 2, 8, 4> : kv::attend_any_kernel<T, 2, 1, 8>;
-    } else if (head_dim <= 128) {
-        p.heads = group > 1 ? 8 : 1;
-        p.kernel = group > 1 ? kv::attend_any_kernel<T, 4, 8, 4> : kv::attend_any_kernel<T, 4, 1, 8>;
-    } else if (head_dim <= 256) {
-        p.heads = group > 1 ? 4 : 1;
-        p.kernel = group > 1 ? kv::attend_any_kernel<T, 8, 4, 4> : kv::attend_any_kernel<T, 8, 1, 4>;
-    } else {
-        p.heads = 1;
-        p.kernel = kv::attend_any_kernel<T, 32, 1, 1>;
+    return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, GH, BLOCKS * kSms, 0, nullptr};
+}
+
+template <class T>
+AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
+{
+    if (fours) {
+        return d <= 128   ? (group == 1   ? any_plan<T, 4, 4, 1, 8, 4>()
+                             : group == 2 ? any_plan<T, 4, 4, 2, 8, 4>()
+                             : group <= 4 ? any_plan<T, 4, 4, 4, 8, 3>()
+                                          : any_plan<T, 4, 4, 8, 4, 3>())
+               : d <= 256 ? (group == 1 ? any_plan<T, 4, 8, 1, 4, 4>() : any_plan<T, 4, 8, 4, 4, 2>())
+                          : any_plan<T, 4, 32, 1, 2, 2>();
     }
-    return p;
+    return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 4>() : any_plan<T, 1, 4, 8, 4, 3>())
+           : d <= 256 ? (group == 1 ? any_plan<T, 1, 8, 1, 4, 4>() : any_plan<T, 1, 8, 4, 4, 2>())
+                      : any_plan<T, 1, 32, 1, 1, 2>();
 }
 
 template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
@@ -222,9 +222,10 @@ AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t 
     if (mma_takes(l, cache_alignment, query_alignment)) {
         return l.dtype == kv::kBf16 ? mma_plan<__nv_bfloat16>(l, group) : mma_plan<__half>(l, group);
     }
-    return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group)
-           : l.dtype == kv::kFp16 ? any_plan<__half>(l.head_dim, group)
-                                  : any_plan<float>(l.head_dim, group);
+    const bool fours = l.head_dim % 4 == 0 && cache_alignment >= 4 * kv::element_bytes(l.dtype);
+    return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group, fours)
+           : l.dtype == kv::kFp16 ? any_plan<__half>(l.head_dim, group, fours)
+                                  : any_plan<float>(l.head_dim, group, fours);
 }
 
 // Once for each device and kernel: more shared memory than 48 KiB has to be asked for.
@@ -374,8 +375,11 @@ extern "C" size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layo
     }
     // the most that any alignment's kernel takes
     const uint32_t group = query_heads / layout->heads;
-    return std::max(workspace_of(attend_plan(*layout, group, 16, 16), value_dim).size,
-                    workspace_of(attend_plan(*layout, group, 1, 1), value_dim).size);
+    uint64_t most = 0;
+    for (uint64_t alignment = 1; alignment <= 16; alignment *= 2) {
+        most = std::max(most, workspace_of(attend_plan(*layout, group, alignment, alignment), value_dim).size);
+    }
+    return most;
 }
 
 extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
