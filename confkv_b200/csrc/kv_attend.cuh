@@ -35,7 +35,7 @@ struct AttendArgs {
     const int32_t* lengths;
     float* partial;                             // [2 workers][GH][value_pad]
     float2* partial_sums;                       // [2 workers][GH]: maximum (of base 2), sum
-    int4* cut;                                  // [workers]: the cut row that begins in a worker's part, its last worker
+    int4* cut;                                  // [workers]: see note_cut()
     uint32_t requests, blocks, limit, window;
     uint32_t group, chunks;                     // query heads of a key head, rows that they are cut into
     uint32_t rows;                              // of a request
@@ -43,6 +43,9 @@ struct AttendArgs {
     float scale;                                // times log2 e: exponents are of base 2
     FastDiv by_block, by_chunks;
     FastDiv by_vector;                          // chunks of 16 bytes of a vector
+    Cutting cutting;
+    uint32_t cut_by_row;                        // the rows are few
+    uint32_t workers;                           // at most
 };
 
 // ------------------------------------------------------------------ parts
@@ -53,7 +56,7 @@ struct AttendArgs {
 // where the row begins in its part and into its place 0 where it goes on there, and join_kernel puts them together.
 
 struct PartShared {
-    uint64_t warp[kAttendWarps];
+    uint64_t warp[8];
     uint64_t found_sum;
     uint32_t found;
 };
@@ -100,14 +103,14 @@ __device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
         set_row(a, p);
     }
     p->first = 0;
-    p->last = cut_at(static_cast<int64_t>(p->end - p->row_begin), p->tiles);
+    p->last = cut_at(a.cutting, static_cast<int64_t>(p->end - p->row_begin), p->tiles);
     return p->last != 0;
 }
 
 // Every thread gets the same; false for a worker that has no tiles.
+template <uint32_t kThreads>
 __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Part* p)
 {
-    constexpr uint32_t kThreads = kAttendThreads;
     const uint32_t t = threadIdx.x;
     uint64_t sum = 0;
     for (uint32_t r = t; r < a.requests; r += kThreads) {
@@ -120,11 +123,11 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
     __syncthreads();
     uint64_t total = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kAttendWarps; ++w) {
+    for (uint32_t w = 0; w < kThreads / 32; ++w) {
         total += s.warp[w];
     }
     p->total = total * a.rows;
-    p->workers = workers_for(p->total, gridDim.x);
+    p->workers = workers_for(a.cutting, p->total, gridDim.x);
     if (blockIdx.x >= p->workers) {
         return false;
     }
@@ -148,7 +151,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
         __syncthreads();
         uint64_t before = base, all = base;
 #pragma unroll
-        for (uint32_t w = 0; w < kAttendWarps; ++w) {
+        for (uint32_t w = 0; w < kThreads / 32; ++w) {
             before += w < t / 32 ? s.warp[w] : 0;
             all += s.warp[w];
         }
@@ -165,10 +168,10 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
     p->request = s.found;
     set_row(a, p);
     const uint64_t in = p->begin - s.found_sum, units = p->tiles + kRowUnits;
-    p->row = static_cast<uint32_t>(in / units);
+    p->row = in < (uint64_t{1} << 32) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(units) : static_cast<uint32_t>(in / units);
     p->row_begin = s.found_sum + p->row * units;
-    p->first = cut_at(static_cast<int64_t>(p->begin - p->row_begin), p->tiles);
-    p->last = cut_at(static_cast<int64_t>(p->end - p->row_begin), p->tiles);
+    p->first = cut_at(a.cutting, static_cast<int64_t>(p->begin - p->row_begin), p->tiles);
+    p->last = cut_at(a.cutting, static_cast<int64_t>(p->end - p->row_begin), p->tiles);
     return p->last > p->first || next_row(a, p);
 }
 
@@ -199,17 +202,23 @@ __device__ __forceinline__ float result_lse(float m, float l)
     return m == -INFINITY ? (l == 0.0f ? -INFINITY : NAN) : kLn2 * (m + log2f(l));
 }
 
-// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row and the worker that
-// ends it; else no request.
-__device__ __forceinline__ int4 no_cut() { return make_int4(-1, 0, 0, 0); }
-
-__device__ __forceinline__ int4 cut_of(const Part& p)
+// What a worker says of its part's last row, for join_kernel: where it begins here and goes on, its request, its row and its last
+// worker; else no request.
+__device__ __forceinline__ int4 cut_of(const AttendArgs& a, const Part& p)
 {
     if (p.first != 0 || p.last == p.tiles) {
-        return no_cut();
+        return make_int4(-1, 0, 0, 0);
     }
     return make_int4(static_cast<int>(p.request), static_cast<int>(p.row),
-                     static_cast<int>(part_of(p.total, p.workers, p.row_begin + last_units(p.tiles))), 0);
+                     static_cast<int>(part_of(p.total, p.workers, p.row_begin + last_units(a.cutting, p.tiles))), 0);
+}
+
+// Called by all threads. Where the rows are few join_kernel looks at each of them instead.
+__device__ __forceinline__ void note_cut(const AttendArgs& a, const int4& cut)
+{
+    if (threadIdx.x == 0 && a.cut_by_row == 0) {
+        a.cut[blockIdx.x] = cut;
+    }
 }
 
 // ------------------------------------------------------------------ any type and head size
@@ -260,10 +269,8 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(cons
     dev::pdl_wait();
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     Part p;
-    if (!find_part(a, part_shared, &p)) {
-        if (threadIdx.x == 0) {
-            a.cut[blockIdx.x] = no_cut();
-        }
+    if (!find_part<kAttendThreads>(a, part_shared, &p)) {
+        note_cut(a, make_int4(-1, 0, 0, 0));
         return;
     }
     const bool one = a.planes[0] == a.planes[1];
@@ -421,11 +428,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(cons
                 }
             }
         }
-        const int4 cut = cut_of(p);
+        const int4 cut = cut_of(a, p);
         if (!next_row(a, &p)) {
-            if (threadIdx.x == 0) {
-                a.cut[blockIdx.x] = cut;
-            }
+            note_cut(a, cut);
             break;
         }
         __syncthreads();
@@ -555,10 +560,8 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     }
     dev::pdl_wait();
     Part p;
-    if (!find_part(a, part_shared, &p)) {
-        if (threadIdx.x == 0) {
-            a.cut[blockIdx.x] = no_cut();
-        }
+    if (!find_part<kAttendThreads>(a, part_shared, &p)) {
+        note_cut(a, make_int4(-1, 0, 0, 0));
         return;
     }
     char* const stages = memory + warp * (STAGES * Shape::kStageBytes);
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
             } else {
                 for (uint32_t k = 0; k < kWarpTokens * chunks; k += 32) {
-                    const uint32_t r = quotient(a.by_vector, k + lane);             // at most 16
+                    const uint32_t r = quotient(a.by_vector, k + lane);             // 16 and more: behind the last
                     copy_chunk(r, k + lane - r * a.by_vector.d);
                 }
             }
@@ -864,21 +867,417 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
             }
         }
-        const int4 cut = cut_of(p);
+        const int4 cut = cut_of(a, p);
         if (!next_row(a, &p)) {
-            if (threadIdx.x == 0) {
-                a.cut[blockIdx.x] = cut;
-            }
+            note_cut(a, cut);
             break;
         }
     }
     copies_wait<0>();
 }
 
+// ------------------------------------------------------------------ 16-bit types, many query heads
+//
+// Where more than 8 query heads share a key head, or a vector is long, a block's eight warps share the stages: for the scores a warp takes
+// 16 of a tile's 64 tokens and half of the row's 16 NT heads, for the results all tokens and an eighth of the values, so that the
+// accumulators stay small (a latent vector's 512 values of 32 heads are 64 registers of a thread, where a warp of its own would need
+// 512) and no sums are left to put together at a row's end. Weights and maxima go through shared memory: three
+// barriers a tile.
+
+constexpr uint32_t kWideThreads = 256;
+constexpr uint32_t kWideWarps = kWideThreads / 32;
+
+template <class T, int DP, int NT, bool ONE, int STAGES>
+struct WideShape {
+    static constexpr bool kTwoParts = std::is_same_v<T, __nv_bfloat16>;
+    static constexpr uint32_t kHeads = 16 * NT;
+    static constexpr uint32_t kRowBytes = DP * 2;
+    static constexpr uint32_t kPlaneBytes = kTile * kRowBytes;
+    static constexpr uint32_t kStageBytes = kPlaneBytes * (ONE ? 1 : 2);
+    static constexpr uint32_t kQuery = STAGES * kStageBytes;            // where the query heads start
+    static constexpr uint32_t kWeightRow = kHeads * 2 + 16;             // bytes; eight tokens' rows lie in different banks
+    static constexpr uint32_t kWeightBytes = kTile * kWeightRow;
+    static constexpr uint32_t kWeights = kQuery + kHeads * kRowBytes;
+    static constexpr uint32_t kShared = kWeights + kWeightBytes * (kTwoParts ? 2 : 1);
+    static_assert(kShared + 4096 <= 227 * 1024, "more than a block has");
+};
+
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const __grid_constant__ AttendArgs a)
+{
+    using Shape = WideShape<T, DP, NT, ONE, STAGES>;
+    constexpr bool kTwoParts = Shape::kTwoParts;
+    constexpr float kBelow = 1.0f - 0x1p-8f;
+    constexpr float kRaise = std::is_same_v<T, __half> ? 15.0f : 0.0f;
+    constexpr uint32_t GH = Shape::kHeads;
+    constexpr int KT = DP / 16;
+    constexpr int VS = KT < 8 ? KT : 8, NS = 8 / VS;         // the warps' split of the result: by values, then by heads
+    constexpr int VT = (KT + VS - 1) / VS, RT = 2 * NT / NS; // 16-value and 8-head tiles of a warp's share
+    static_assert(KT % 2 == 0 && 2 * NT % NS == 0);
+    extern __shared__ __align__(1024) char memory[];
+    __shared__ PartShared part_shared;
+    __shared__ float4 tops[GH];                              // of the four groups of 16 tokens
+    __shared__ float4 lane_sums_of[GH];
+    __shared__ uint64_t tokens_of[STAGES];                   // bit i of a stage: token i is one
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    dev::pdl_release();
+    if (a.head_dim != DP) {
+        for (uint32_t i = threadIdx.x; i < Shape::kWeights / 16; i += kWideThreads) {
+            reinterpret_cast<uint4*>(memory)[i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+    }
+    dev::pdl_wait();
+    Part p;
+    if (!find_part<kWideThreads>(a, part_shared, &p)) {
+        note_cut(a, make_int4(-1, 0, 0, 0));
+        return;
+    }
+    const uint32_t base = shared_address(memory);
+    const uint32_t chunks = a.head_dim / 8;
+    const uint32_t tiles16 = (a.head_dim + 15) / 16, value_tiles = (a.value_dim + 15) / 16;
+
+    Part ahead = p;
+    bool more_rows = true;
+    uint32_t stage_in = 0, stage_out = 0;
+    // each warp copies 8 of a tile's 64 vectors
+    const auto copy_tile = [&]() {
+        if (more_rows) {
+            const uint32_t key_head = quotient(a.by_chunks, ahead.row);
+            const int32_t* table = a.tables + ahead.request * a.table_stride;
+            const uint32_t token = ahead.span.first + ahead.first * kTile + warp * 8 + lane % 8;
+            int64_t offset = token < ahead.span.end ? token_offset(a, table, token) : -1;
+            const uint32_t there = __ballot_sync(~0u, offset >= 0) & 0xffu;
+            offset = offset >= 0 ? offset + key_head * a.page_head_stride : 0;
+            if (lane == 0) {
+                reinterpret_cast<uint8_t*>(&tokens_of[stage_in])[warp] = static_cast<uint8_t>(there);
+            }
+            const uint32_t to = base + stage_in * Shape::kStageBytes + warp * 8 * Shape::kRowBytes;
+            const auto copy_chunk = [&](uint32_t r, uint32_t c) {
+                const int64_t from = __shfl_sync(~0u, offset, r) + c * 16;
+                const uint32_t at = to + r * Shape::kRowBytes + ((c ^ r) * 16);
+                const bool is = (there >> r & 1) != 0;
+                if (r < 8) {
+                    copy_16(at, a.planes[0] + from, is);
+                    if constexpr (!ONE) {
+                        copy_16(at + Shape::kPlaneBytes, a.planes[1] + from, is);
+                    }
+                }
+            };
+            constexpr uint32_t kChunks = DP / 8;
+            if (32 % kChunks == 0 && chunks == kChunks) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8 * kChunks / 32; ++k) {
+                    copy_chunk(k * (32 / kChunks) + lane / kChunks, lane % kChunks);
+                }
+            } else {
+                for (uint32_t k = 0; k < 8 * chunks; k += 32) {
+                    const uint32_t r = quotient(a.by_vector, k + lane);             // 8 and more: behind the last
+                    copy_chunk(r, k + lane - r * a.by_vector.d);
+                }
+            }
+            if (++ahead.first == ahead.last) {
+                more_rows = next_row(a, &ahead);
+            }
+        }
+        copies_end();
+        stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    };
+    // the row's query heads, zeros for those that it does not have: read while the row before is at its last tile, laid down when
+    // all warps have that one's scores
+    constexpr uint32_t kQueryParts = (GH * DP / 8 + kWideThreads - 1) / kWideThreads;
+    uint4 query[kQueryParts];
+    const auto read_query = [&](const Part& row) {
+        const uint32_t key_head = quotient(a.by_chunks, row.row), chunk = row.row - key_head * a.by_chunks.d;
+        const uint32_t heads = min(GH, a.group - chunk * GH);
+        const char* from = a.query + row.request * a.query_stride + (key_head * a.group + chunk * GH) * a.query_head_stride;
+#pragma unroll
+        for (uint32_t k = 0; k < kQueryParts; ++k) {
+            const uint32_t i = k * kWideThreads + threadIdx.x, g = quotient(a.by_vector, i), c = i - g * a.by_vector.d;
+            query[k] = g < heads ? *reinterpret_cast<const uint4*>(from + g * a.query_head_stride + c * 16) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    const auto write_query = [&]() {
+#pragma unroll
+        for (uint32_t k = 0; k < kQueryParts; ++k) {
+            const uint32_t i = k * kWideThreads + threadIdx.x, g = quotient(a.by_vector, i), c = i - g * a.by_vector.d;
+            if (g < GH) {
+                *reinterpret_cast<uint4*>(memory + Shape::kQuery + g * Shape::kRowBytes + ((c ^ (g % 8)) * 16)) = query[k];
+            }
+        }
+    };
+    read_query(p);
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) {
+        copy_tile();
+    }
+    write_query();
+
+    const uint32_t token_group = warp % 4, head_half = warp / 4;
+    const uint32_t value_share = warp % VS, head_share = warp / VS;
+    bool more = true;
+    while (more) {
+        const uint32_t tiles = p.last - p.first;
+        const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
+        const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
+        const uint32_t heads = min(GH, a.group - chunk * GH);
+        Part next = p;
+        more = next_row(a, &next);
+        float m[2 * NT][2], l[NT][2], o[VT][RT][4];         // m of all heads, l of this warp's tokens and half
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            l[n][0] = l[n][1] = 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+#pragma unroll
+            for (int n = 0; n < RT; ++n) {
+                o[v][n][0] = o[v][n][1] = o[v][n][2] = o[v][n][3] = 0.0f;
+            }
+        }
+        bool any = false;
+        for (uint32_t t = 0; t < tiles; ++t) {
+            copies_wait<STAGES - 2>();
+            __syncthreads();
+            copy_tile();
+            const bool query_next = t + 1 == tiles && more;
+            if (query_next) {
+                read_query(next);
+            }
+            const uint64_t there = tokens_of[stage_out];
+            const uint32_t keys = base + stage_out * Shape::kStageBytes;
+            const uint32_t values = keys + (ONE ? 0 : Shape::kPlaneBytes);
+            stage_out = stage_out + 1 == STAGES ? 0 : stage_out + 1;
+            any |= there != 0;
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            }
+            {
+                const uint32_t r = token_group * 16 + lane % 16, c = lane / 16;
+                const uint32_t row = keys + r * Shape::kRowBytes;
+                // two steps of 16 values (NT 1) or two eights of heads (NT 2) in one load
+                const uint32_t g = head_half * 8 * NT + (NT == 2 ? lane / 16 * 8 : 0) + lane % 8;
+                const uint32_t qc = lane / 8 % 2 + (NT == 1 ? lane / 16 * 2 : 0);
+                const uint32_t q_row = base + Shape::kQuery + g * Shape::kRowBytes;
+#pragma unroll
+                for (int k = 0; k < KT; k += 2) {
+                    if (static_cast<uint32_t>(k) < tiles16) {
+                        uint32_t x[4], y[4], q[2][4];
+                        load_matrices(x, row + (((2 * k + c) ^ (r % 8)) * 16));
+                        load_matrices(y, row + (((2 * k + 2 + c) ^ (r % 8)) * 16));
+                        load_matrices(q[0], q_row + (((2 * k + qc) ^ (g % 8)) * 16));
+                        if constexpr (NT == 1) {
+                            multiply<T>(s[0], x, q[0][0], q[0][1]);
+                            multiply<T>(s[0], y, q[0][2], q[0][3]);
+                        } else {
+                            load_matrices(q[1], q_row + (((2 * k + 2 + qc) ^ (g % 8)) * 16));
+                            multiply<T>(s[0], x, q[0][0], q[0][1]);
+                            multiply<T>(s[1], x, q[0][2], q[0][3]);
+                            multiply<T>(s[0], y, q[1][0], q[1][1]);
+                            multiply<T>(s[1], y, q[1][2], q[1][3]);
+                        }
+                    }
+                }
+            }
+            // tokens lane / 4 and lane / 4 + 8 of the warp's 16, heads 2 (lane % 4) and the next of each eight
+            const uint32_t mine = static_cast<uint32_t>(there >> (token_group * 16)) & 0xffffu;
+            const bool first = (mine >> (lane / 4) & 1) != 0, second = (mine >> (lane / 4 + 8) & 1) != 0;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    s[n][j] = first ? s[n][j] * a.scale : -INFINITY;
+                    s[n][j + 2] = second ? s[n][j + 2] * a.scale : -INFINITY;
+                    float x = fmaxf(s[n][j], s[n][j + 2]);
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) {
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+                    }
+                    if (lane < 4) {
+                        reinterpret_cast<float*>(&tops[(head_half * NT + n) * 8 + lane * 2 + j])[token_group] = x;
+                    }
+                }
+            }
+            __syncthreads();
+            float fade[2 * NT][2];
+            bool faded = false;
+#pragma unroll
+            for (int n = 0; n < 2 * NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float4 x = tops[n * 8 + lane % 4 * 2 + j];
+                    const float top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), m[n][j]);
+                    fade[n][j] = power_of_2(m[n][j] - reference(top));
+                    faded |= top > m[n][j];
+                    m[n][j] = top;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float ref = head_half != 0 ? m[NT + n][i % 2] : m[n][i % 2];
+                    x[i] = power_of_2(s[n][i] - (reference(ref) - kRaise));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    l[n][j] = l[n][j] * (head_half != 0 ? fade[NT + n][j] : fade[n][j]) + (x[j] + x[j + 2]);
+                }
+                const uint32_t at = Shape::kWeights + (token_group * 16 + lane / 4) * Shape::kWeightRow + (head_half * NT + n) * 16 + lane % 4 * 4;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t* const to = reinterpret_cast<uint32_t*>(memory + at + h * 8 * Shape::kWeightRow);
+                    if constexpr (kTwoParts) {
+                        // the weight cut to 8 bits a little below itself, and the rest: both above 0, so that a value's infinity stays one
+                        const uint32_t lo = __float_as_uint(x[2 * h] * kBelow), hi = __float_as_uint(x[2 * h + 1] * kBelow);
+                        *to = __byte_perm(lo, hi, 0x7632);
+                        to[Shape::kWeightBytes / 4] = pack<T>(x[2 * h] - __uint_as_float(lo & 0xffff0000u),
+                                                              x[2 * h + 1] - __uint_as_float(hi & 0xffff0000u));
+                    } else {
+                        *to = pack<T>(x[2 * h], x[2 * h + 1]);
+                    }
+                }
+            }
+            if (__any_sync(~0u, faded)) {
+#pragma unroll
+                for (int n = 0; n < RT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float f = NS > 1 && head_share != 0 ? fade[(2 * NT - RT) + n][j] : fade[n][j];
+#pragma unroll
+                        for (int v = 0; v < VT; ++v) {
+                            o[v][n][j] *= f;
+                            o[v][n][j + 2] *= f;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            if (query_next) {
+                write_query();
+            }
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(kTile) / 16; ++k) {
+                uint32_t w[RT][2], rest[RT][2];
+                {
+                    const uint32_t r = k * 16 + lane % 16;
+                    const uint32_t at = base + Shape::kWeights + r * Shape::kWeightRow + head_share * RT * 16 + lane / 16 * 16;
+#pragma unroll
+                    for (int n = 0; n < RT; n += 2) {
+                        uint32_t x[4];
+                        load_matrices_across(x, at + n * 16);
+                        w[n][0] = x[0];
+                        w[n][1] = x[1];
+                        if constexpr (RT > 1) {
+                            w[n + 1][0] = x[2];
+                            w[n + 1][1] = x[3];
+                        }
+                        if constexpr (kTwoParts) {
+                            load_matrices_across(x, at + n * 16 + Shape::kWeightBytes);
+                            rest[n][0] = x[0];
+                            rest[n][1] = x[1];
+                            if constexpr (RT > 1) {
+                                rest[n + 1][0] = x[2];
+                                rest[n + 1][1] = x[3];
+                            }
+                        }
+                    }
+                }
+                const uint32_t r = k * 16 + lane % 8 + lane / 16 * 8, c = lane / 8 % 2;
+                const uint32_t row = values + r * Shape::kRowBytes;
+#pragma unroll
+                for (int v = 0; v < VT; ++v) {
+                    const uint32_t tile = value_share + v * VS;
+                    if (tile < value_tiles) {
+                        uint32_t x[4];
+                        load_matrices_across(x, row + (((2 * tile + c) ^ (r % 8)) * 16));
+#pragma unroll
+                        for (int n = 0; n < RT; ++n) {
+                            multiply<T>(o[v][n], x, w[n][0], w[n][1]);
+                            if constexpr (kTwoParts) {
+                                multiply<T>(o[v][n], x, rest[n][0], rest[n][1]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+
+        // the sums of the four groups of tokens
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {
+                    l[n][j] += __shfl_xor_sync(~0u, l[n][j], d);
+                }
+                if (lane < 4) {
+                    reinterpret_cast<float*>(&lane_sums_of[(head_half * NT + n) * 8 + lane * 2 + j])[token_group] = l[n][j];
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = tiles == p.tiles;
+        const uint32_t at_place = blockIdx.x * 2 + (p.first == 0 ? 1 : 0);
+#pragma unroll
+        for (int n = 0; n < RT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t g = (head_share * RT + n) * 8 + lane % 4 * 2 + j;
+                if (g >= heads) {
+                    continue;
+                }
+                const float4 x = lane_sums_of[g];
+                const float top = NS > 1 && head_share != 0 ? m[(2 * NT - RT) + n][j] : m[n][j];
+                float sum = ((x.x + x.y) + (x.z + x.w)) * power_of_2(-kRaise);
+                sum = top == -INFINITY && sum == 0.0f && any ? 1.0f : sum;
+                const float factor = (whole ? result_factor(top, sum) : 1.0f) * power_of_2(-kRaise);
+                T* out = reinterpret_cast<T*>(a.out + p.request * a.out_stride + (head + g) * a.out_head_stride);
+                float* partial = a.partial + (uint64_t{at_place} * GH + g) * a.value_pad;
+#pragma unroll
+                for (int v = 0; v < VT; ++v) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t d = (value_share + v * VS) * 16 + h * 8 + lane / 4;
+                        if (d < a.value_dim) {
+                            const float y = o[v][n][j + 2 * h] * factor;
+                            if (whole) {
+                                out[d] = from_float<T>(y);
+                            } else {
+                                partial[d] = y;
+                            }
+                        }
+                    }
+                }
+                if (value_share == 0 && lane < 4) {
+                    if (!whole) {
+                        a.partial_sums[at_place * GH + g] = make_float2(top, sum);
+                    } else if (a.lse != nullptr) {
+                        a.lse[p.request * a.lse_stride + head + g] = result_lse(top, sum);
+                    }
+                }
+            }
+        }
+        if (!more) {
+            note_cut(a, cut_of(a, p));
+        }
+        p = next;
+    }
+    copies_wait<0>();
+}
+
 // ------------------------------------------------------------------ joining
 //
-// Block (c, g): query head g of the row that begins in worker c's part and is cut, if there is one: worker c's place 1,
-// then place 0 of all workers up to the row's last one. A thread has four values; where a head has fewer
+// Block (x, g, z): query head g of row x, or of the cut row that begins in worker x's part, if there is one: its first worker's place 1,
+// then place 0 of the workers up to its last one. A thread has four values, of share z of them; where a share has fewer
 // than the block's threads hold, groups of threads share the pieces. The first pieces are on their way before their weights
 // are known: the kernel is a chain of a few trips to L2.
 
@@ -894,24 +1293,67 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
     dev::pdl_release();
     dev::pdl_wait();
     const uint32_t t = threadIdx.x, lane = t % 32, warp = t / 32;
-    const uint32_t c = blockIdx.x, g = blockIdx.y;
-    const int4 cut = a.cut[c];
-    if (cut.x < 0) {
-        return;
+    const uint32_t g = blockIdx.y;
+    uint32_t request, row, c, last;
+    if (a.cut_by_row != 0) {
+        request = blockIdx.x / a.rows;
+        row = blockIdx.x - request * a.rows;
+        uint64_t total = 0, begin = 0;
+        for (uint32_t r = t; r < a.requests; r += kAttendThreads) {
+            const uint64_t n = tiles_of(span_at(a, r), kTile) + kRowUnits;
+            total += n;
+            begin += r < request ? n : 0;
+        }
+        total = warp_sum(total);
+        begin = warp_sum(begin);
+        __shared__ uint64_t units[kAttendWarps][2];
+        if (lane == 0) {
+            units[warp][0] = total;
+            units[warp][1] = begin;
+        }
+        __syncthreads();
+        total = begin = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kAttendWarps; ++w) {
+            total += units[w][0];
+            begin += units[w][1];
+        }
+        const uint32_t tiles = tiles_of(span_at(a, request), kTile);
+        total *= a.rows;
+        begin = begin * a.rows + uint64_t{row} * (tiles + kRowUnits);
+        const uint32_t workers = workers_for(a.cutting, total, a.workers);
+        c = part_of(total, workers, begin + first_units(a.cutting, tiles));
+        last = part_of(total, workers, begin + last_units(a.cutting, tiles));
+        if (c == last) {
+            return;
+        }
+    } else {
+        const int4 cut = a.cut[blockIdx.x];
+        if (cut.x < 0) {
+            return;
+        }
+        request = cut.x;
+        row = cut.y;
+        c = blockIdx.x;
+        last = cut.z;
     }
-    const uint32_t row = cut.y, key_head = quotient(a.by_chunks, row), chunk = row - key_head * a.by_chunks.d;
+    const uint32_t key_head = quotient(a.by_chunks, row), chunk = row - key_head * a.by_chunks.d;
     if (chunk * gh + g >= a.group) {
         return;
     }
     const uint32_t head = key_head * a.group + chunk * gh + g;
-    const uint32_t pieces = cut.z - c + 1;
+    const uint32_t pieces = last - c + 1;
     const auto place = [&](uint32_t k) { return (uint64_t{c + k} * 2 + (k == 0 ? 1 : 0)) * gh + g; };
     // columns of four values, and the groups of threads that share the pieces of one
-    const uint32_t columns = a.value_pad / 4;
+    const uint32_t all = a.value_pad / 4, share = (all + gridDim.z - 1) / gridDim.z, from = blockIdx.z * share;
+    const uint32_t columns = from >= all ? 0 : min(share, all - from);
+    if (columns == 0) {
+        return;
+    }
     const uint32_t groups = columns >= kAttendThreads ? 1 : kAttendThreads / columns;
     const uint32_t column = columns >= kAttendThreads ? t : t % columns, group = columns >= kAttendThreads ? 0 : t / columns;
     const auto value = [&](uint32_t k, uint32_t x) {
-        return *reinterpret_cast<const float4*>(a.partial + place(k) * a.value_pad + x * 4);
+        return *reinterpret_cast<const float4*>(a.partial + place(k) * a.value_pad + (from + x) * 4);
     };
     float4 ahead[kJoinAhead];
     const bool works = group < groups && column < columns;
@@ -959,7 +1401,6 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
         sum += sums[w];
     }
     const float factor = result_factor(top, sum);
-    const uint32_t request = cut.x;
     T* out = reinterpret_cast<T*>(a.out + request * a.out_stride + head * a.out_head_stride);
     const auto fold = [](float4& s, float w, const float4& v) {
         s.x = fmaf(w, v.x, s.x);
@@ -971,8 +1412,8 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
         const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            if (x * 4 + i < a.value_dim) {
-                out[x * 4 + i] = from_float<T>(v[i] * factor);
+            if ((from + x) * 4 + i < a.value_dim) {
+                out[(from + x) * 4 + i] = from_float<T>(v[i] * factor);
             }
         }
     };
@@ -1010,7 +1451,7 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
         }
         write(x, more);
     }
-    if (t == 0 && a.lse != nullptr) {
+    if (t == 0 && blockIdx.z == 0 && a.lse != nullptr) {
         a.lse[request * a.lse_stride + head] = result_lse(top, sum);
     }
 }

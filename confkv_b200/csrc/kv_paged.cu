@@ -153,8 +153,10 @@ using JoinKernel = void (*)(const kv::AttendArgs, uint32_t);
 struct AttendPlan {
     AttendKernel kernel;
     JoinKernel join;
+    uint32_t threads;
     uint32_t heads;             // query heads of a row
     uint32_t workers;
+    kv::Cutting cutting;
     uint32_t shared;            // bytes of dynamic shared memory
     std::atomic<uint64_t>* allowed;     // devices on which the kernel may have them
 };
@@ -165,22 +167,22 @@ static_assert(4 * kSms <= kv::kMostWorkers);
 template <class T, int VEC, int R, int GH, int U, int BLOCKS>
 AttendPlan any_plan()
 {
-    return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, GH, BLOCKS * kSms, 0, nullptr};
+    return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, GH, BLOCKS * kSms, kv::Cutting{2, 1}, 0, nullptr};
 }
 
 template <class T>
 AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
 {
     if (fours) {
-        return d <= 128   ? (group == 1   ? any_plan<T, 4, 4, 1, 8, 4>()
-                             : group == 2 ? any_plan<T, 4, 4, 2, 8, 4>()
-                             : group <= 4 ? any_plan<T, 4, 4, 4, 8, 3>()
-                                          : any_plan<T, 4, 4, 8, 4, 3>())
-               : d <= 256 ? (group == 1 ? any_plan<T, 4, 8, 1, 4, 4>() : any_plan<T, 4, 8, 4, 4, 2>())
+        return d <= 128   ? (group == 1   ? any_plan<T, 4, 4, 1, 8, 3>()
+                             : group == 2 ? any_plan<T, 4, 4, 2, 8, 3>()
+                             : group <= 4 ? any_plan<T, 4, 4, 4, 8, 2>()
+                                          : any_plan<T, 4, 4, 8, 4, 2>())
+               : d <= 256 ? (group == 1 ? any_plan<T, 4, 8, 1, 4, 3>() : any_plan<T, 4, 8, 4, 4, 2>())
                           : any_plan<T, 4, 32, 1, 2, 2>();
     }
-    return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 4>() : any_plan<T, 1, 4, 8, 4, 3>())
-           : d <= 256 ? (group == 1 ? any_plan<T, 1, 8, 1, 4, 4>() : any_plan<T, 1, 8, 4, 4, 2>())
+    return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 3>() : any_plan<T, 1, 4, 8, 4, 2>())
+           : d <= 256 ? (group == 1 ? any_plan<T, 1, 8, 1, 4, 3>() : any_plan<T, 1, 8, 4, 4, 2>())
                       : any_plan<T, 1, 32, 1, 1, 2>();
 }
 
@@ -189,32 +191,51 @@ AttendPlan mma_plan()
 {
     static std::atomic<uint64_t> allowed{0};
     using Shape = kv::MmaShape<T, DP, NT, ONE, STAGES>;
-    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, Shape::kHeads, BLOCKS * kSms,
-                      Shape::kShared, &allowed};
+    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, Shape::kHeads, BLOCKS * kSms,
+                      kv::Cutting{DP <= 128 ? 8u : 4u, 2}, Shape::kShared, &allowed};
 }
 
 // Whether the 16-bit kernel takes vectors of this size, in a cache and of queries of this alignment.
 bool mma_takes(const lmcache_gpu_kv_layout& l, uint64_t cache_alignment, uint64_t query_alignment)
 {
     return l.dtype != kv::kFp32 && l.head_dim % 8 == 0 && l.head_dim <= (l.planes == 2 ? 256u : 576u) && cache_alignment >= 16 &&
-           query_alignment >= 4;
+           query_alignment >= 16;
+}
+
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+AttendPlan wide_plan()
+{
+    static std::atomic<uint64_t> allowed{0};
+    using Shape = kv::WideShape<T, DP, NT, ONE, STAGES>;
+    return AttendPlan{kv::attend_wide_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, kv::kWideThreads, Shape::kHeads,
+                      BLOCKS * kSms, kv::Cutting{2, 1}, Shape::kShared, &allowed};
 }
 
 template <class T>
 AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
 {
     const uint32_t d = l.head_dim;
-    const bool two = group > 8;
+    const bool many = group > 16;
     if (l.planes == 2) {
-        return d <= 64    ? (two ? mma_plan<T, 64, 2, false, 4, 2>() : mma_plan<T, 64, 1, false, 4, 3>())
-               : d <= 128 ? (two ? mma_plan<T, 128, 2, false, 3, 1>() : mma_plan<T, 128, 1, false, 3, 2>())
-               : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>()
-                          : mma_plan<T, 256, 1, false, 3, 1>();
+        if (group <= 8) {
+            return d <= 64    ? mma_plan<T, 64, 1, false, 4, 3>()
+                   : d <= 128 ? mma_plan<T, 128, 1, false, 3, 2>()
+                   : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>()
+                              : mma_plan<T, 256, 1, false, 3, 1>();
+        }
+        return d <= 64    ? (many ? wide_plan<T, 64, 2, false, 4, 2>() : wide_plan<T, 64, 1, false, 4, 2>())
+               : d <= 128 ? (many ? wide_plan<T, 128, 2, false, 3, 2>() : wide_plan<T, 128, 1, false, 3, 2>())
+                          : (many ? wide_plan<T, 256, 2, false, 3, 1>() : wide_plan<T, 256, 1, false, 3, 1>());
     }
-    return d <= 128   ? (two ? mma_plan<T, 128, 2, true, 5, 2>() : mma_plan<T, 128, 1, true, 5, 2>())
-           : d <= 256 ? mma_plan<T, 256, 1, true, 5, 1>()
-           : d <= 320 ? mma_plan<T, 320, 1, true, 4, 1>()
-                      : mma_plan<T, 576, 1, true, 2, 1>();
+    if (group <= 8 && d <= 320) {
+        return d <= 128   ? mma_plan<T, 128, 1, true, 5, 2>()
+               : d <= 256 ? mma_plan<T, 256, 1, true, 5, 1>()
+                          : mma_plan<T, 320, 1, true, 4, 1>();
+    }
+    return d <= 128   ? (many ? wide_plan<T, 128, 2, true, 4, 2>() : wide_plan<T, 128, 1, true, 4, 2>())
+           : d <= 256 ? (many ? wide_plan<T, 256, 2, true, 3, 1>() : wide_plan<T, 256, 1, true, 3, 1>())
+           : d <= 320 ? (many ? wide_plan<T, 320, 2, true, 3, 1>() : wide_plan<T, 320, 1, true, 4, 1>())
+                      : (many ? wide_plan<T, 576, 2, true, 2, 1>() : wide_plan<T, 576, 1, true, 2, 1>());
 }
 
 AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t cache_alignment, uint64_t query_alignment)
@@ -457,17 +478,25 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.scale = t.scale * kv::kLog2e;
     a.by_block = kv::make_fast_div(pages->block_size);
     a.by_chunks = kv::make_fast_div(a.chunks);
+    a.cutting = plan.cutting;
+    a.workers = plan.workers;
+    a.cut_by_row = uint64_t{t.requests} * a.rows * std::min(plan.heads, a.group) <= kSms ? 1 : 0;
     a.by_vector = kv::make_fast_div(std::max<uint32_t>(1, l.head_dim / 8));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = allow_shared(plan, device);
     if (e != cudaSuccess) {
         return LMCACHE_GPU_AESGCM_ERR_CUDA;
     }
-    e = launch(plan.kernel, dim3(plan.workers), kv::kAttendThreads, plan.shared, s, a);
+    e = launch(plan.kernel, dim3(plan.workers), plan.threads, plan.shared, s, a);
     // rows that no length makes long enough to be cut need no joining
     const uint32_t most = t.window != 0 ? std::min(t.window, a.limit) : a.limit;
-    if (e == cudaSuccess && kv::tiles_of(kv::Span{0, most}, kv::kTile) > kv::kWholeTiles) {
-        e = launch(plan.join, dim3(plan.workers, std::min(plan.heads, a.group)), kv::kAttendThreads, 0, s, a, plan.heads);
+    if (e == cudaSuccess && kv::tiles_of(kv::Span{0, most}, kv::kTile) > plan.cutting.whole_tiles) {
+        // few rows have many pieces each: their values are shared out among as many blocks as there are SMs, one row's among those of
+        // a worker's place where rows are many (one request, one key head, 131072 tokens: 27.9 us, and 42.0 the other way; 128 requests
+        // of one key head: 19.6, and 21.3 with blocks that look at a row each)
+        const uint32_t heads = std::min(plan.heads, a.group), rows = a.cut_by_row != 0 ? t.requests * a.rows : plan.workers;
+        const uint32_t shares = a.cut_by_row != 0 ? std::clamp(kSms / (rows * heads), 1u, (a.value_pad + 31) / 32) : 1u;
+        e = launch(plan.join, dim3(rows, heads, shares), kv::kAttendThreads, 0, s, a, plan.heads);
     }
     return cuda_rc(e);
 }

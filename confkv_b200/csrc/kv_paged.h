@@ -93,7 +93,11 @@ KV_HD uint32_t tiles_of(const Span& s, uint32_t tile)
 // part_start(c + 1)), one at least. total < 2^52, workers < 2^11.
 constexpr uint32_t kRowUnits = 3;
 
-KV_HD uint64_t part_start(uint64_t total, uint32_t workers, uint32_t c) { return total * c / workers; }
+KV_HD uint64_t part_start(uint64_t total, uint32_t workers, uint32_t c)
+{
+    // 32 bits where they hold it: the division is a good part of a small call's beginning
+    return total < (1u << 21) ? static_cast<uint32_t>(total) * c / workers : total * c / workers;
+}
 
 // The worker that has a unit: the largest c with total c / workers < unit + 1.
 KV_HD uint32_t part_of(uint64_t total, uint32_t workers, uint64_t unit)
@@ -101,35 +105,34 @@ KV_HD uint32_t part_of(uint64_t total, uint32_t workers, uint64_t unit)
     return static_cast<uint32_t>(((unit + 1) * workers - 1) / total);
 }
 
-// Few units are shared by fewer workers: cutting a row costs more than some tiles do.
-constexpr uint32_t kLeastUnits = 4;
+// How finely rows may be cut, a kernel's own: cutting costs more than some tiles do (the pieces have to be written and joined). A row of up to
+// whole_tiles tiles stays whole, and few units are shared by fewer workers, 2^least_units each.
+struct Cutting {
+    uint32_t whole_tiles, least_units;
+};
 
-KV_HD uint32_t workers_for(uint64_t total, uint32_t most)
+KV_HD uint32_t workers_for(const Cutting& k, uint64_t total, uint32_t most)
 {
-    const uint64_t n = total / kLeastUnits;
+    const uint64_t n = total >> k.least_units;
     return n == 0 ? 1u : (n < most ? static_cast<uint32_t>(n) : most);
 }
 
-// Where a part's border at `x` units behind a row's first one (or before it) cuts the row: in front of which tile. A row of few tiles stays
-// whole, and no border leaves a few tiles alone: the pieces of a cut row have to be written, counted and joined.
-constexpr uint32_t kWholeTiles = 8;
-constexpr uint32_t kLeastTiles = 2;
-
-KV_HD uint32_t first_units(uint32_t tiles)      // up to there a border lies in front of the row
+// Where a part's border at `x` units behind a row's first one (or before it) cuts the row: in front of which tile.
+KV_HD uint32_t first_units(const Cutting& k, uint32_t tiles)      // up to there a border lies in front of the row
 {
-    return tiles <= kWholeTiles ? (tiles + kRowUnits) / 2 : kRowUnits + kLeastTiles;
+    return tiles <= k.whole_tiles ? (tiles + kRowUnits) / 2 : kRowUnits;
 }
 
-KV_HD uint32_t last_units(uint32_t tiles)       // beyond there it lies behind the row
+KV_HD uint32_t last_units(const Cutting& k, uint32_t tiles)       // beyond there it lies behind the row
 {
-    return tiles <= kWholeTiles ? (tiles + kRowUnits) / 2 : kRowUnits + tiles - kLeastTiles - 1;
+    return tiles <= k.whole_tiles ? (tiles + kRowUnits) / 2 : kRowUnits + tiles - 1;
 }
 
-KV_HD uint32_t cut_at(int64_t x, uint32_t tiles)
+KV_HD uint32_t cut_at(const Cutting& k, int64_t x, uint32_t tiles)
 {
-    return x <= static_cast<int64_t>(first_units(tiles)) ? 0u
-           : x > static_cast<int64_t>(last_units(tiles)) ? tiles
-                                                         : static_cast<uint32_t>(x) - kRowUnits;
+    return x <= static_cast<int64_t>(first_units(k, tiles)) ? 0u
+           : x > static_cast<int64_t>(last_units(k, tiles)) ? tiles
+                                                            : static_cast<uint32_t>(x) - kRowUnits;
 }
 
 }  // namespace kv

@@ -44,21 +44,22 @@ void spans(const int32_t* length, int n, uint32_t limit, uint32_t window, uint32
 
 // 0 where the rows (of so many tiles each) are cut as joining takes it: every tile is one worker's; a row begins in the worker that
 // part_of names for first_units, goes on in the next ones without a gap, and ends in the one named for last_units; rows of few
-// tiles are whole, and no piece of another is shorter than kLeastTiles but between two borders.
-int check_rows(const uint32_t* tiles, int rows, uint32_t most)
+// tiles are whole.
+int check_rows(const uint32_t* tiles, int rows, uint32_t most, uint32_t whole_tiles, uint32_t least_units)
 {
+    const Cutting k{whole_tiles, least_units};
     uint64_t total = 0;
     for (int r = 0; r < rows; ++r) {
         total += tiles[r] + kRowUnits;
     }
-    const uint32_t workers = workers_for(total, most);
+    const uint32_t workers = workers_for(k, total, most);
     if (workers > total || workers > most) {
         return 1;
     }
     uint64_t row_begin = 0;
     for (int r = 0; r < rows; ++r) {
-        const uint32_t begins = part_of(total, workers, row_begin + first_units(tiles[r]));
-        const uint32_t ends = part_of(total, workers, row_begin + last_units(tiles[r]));
+        const uint32_t begins = part_of(total, workers, row_begin + first_units(k, tiles[r]));
+        const uint32_t ends = part_of(total, workers, row_begin + last_units(k, tiles[r]));
         uint32_t next = 0;
         for (uint32_t c = 0; c < workers; ++c) {
             const int64_t a = static_cast<int64_t>(part_start(total, workers, c)) - static_cast<int64_t>(row_begin);
@@ -66,7 +67,7 @@ int check_rows(const uint32_t* tiles, int rows, uint32_t most)
             if (b <= 0 || a >= static_cast<int64_t>(tiles[r] + kRowUnits)) {
                 continue;
             }
-            const uint32_t first = cut_at(a, tiles[r]), last = cut_at(b, tiles[r]);
+            const uint32_t first = cut_at(k, a, tiles[r]), last = cut_at(k, b, tiles[r]);
             if ((last > first) != (c >= begins && c <= ends)) {
                 return 2;
             }
@@ -76,15 +77,12 @@ int check_rows(const uint32_t* tiles, int rows, uint32_t most)
             if (first != next) {
                 return 3;
             }
-            if ((first == 0 || last == tiles[r]) && last - first < (tiles[r] < kLeastTiles ? tiles[r] : kLeastTiles)) {
-                return 4;
-            }
             next = last;
         }
         if (next != tiles[r]) {
             return 5;
         }
-        if (tiles[r] <= kWholeTiles && begins != ends) {
+        if (tiles[r] <= whole_tiles && begins != ends) {
             return 6;
         }
         row_begin += tiles[r] + kRowUnits;

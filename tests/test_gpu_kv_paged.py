@@ -306,7 +306,7 @@ def test_head_sizes(gpu_lib, dtype, d):
 @pytest.mark.parametrize("d,value_dim", [(16, 16), (64, 64), (128, 100), (192, 128), (256, 1), (320, 256), (320, 319), (320, 320), (576, 512), (576, 576), (100, 99), (600, 512)])
 def test_latent_vectors(gpu_lib, dtype, d, value_dim):
     for group in (1, 5, 16, 40):
-        Case(gpu_lib, dtype, 1, 1, d, group, LENGTHS, 16, value_dim=value_dim, seed=d + group).run().check()
+        Case(gpu_lib, dtype, 1, 1, d, group, LENGTHS + [3000, 0, 64], 16, value_dim=value_dim, seed=d + group).run().check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -328,8 +328,8 @@ def test_block_sizes(gpu_lib, dtype, order, size):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 64, 65, 100, 499, 500, (1 << 32) - 1])
 def test_windows(gpu_lib, dtype, window):
-    for d in (64, 100, 128):
-        Case(gpu_lib, dtype, 2, 2, d, 4, LENGTHS, 16, window=window, seed=window % 1000).run().check()
+    for d, group in ((64, 4), (100, 4), (128, 4), (128, 9)):
+        Case(gpu_lib, dtype, 2, 2, d, group, LENGTHS, 16, window=window, seed=window % 1000).run().check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -340,11 +340,11 @@ def test_alignments_of_the_cache(gpu_lib, dtype, offset, gap):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 100, 128, 256])
-def test_strides_of_queries_and_results(gpu_lib, dtype, d):
-    c = Case(gpu_lib, dtype, 2, 2, d, 4, LENGTHS, 16, layers=3, layer=2)
+@pytest.mark.parametrize("d,group", [(64, 4), (100, 4), (128, 4), (256, 4), (64, 12), (128, 12), (128, 20)])
+def test_strides_of_queries_and_results(gpu_lib, dtype, d, group):
+    c = Case(gpu_lib, dtype, 2, 2, d, group, LENGTHS, 16, layers=3, layer=2)
     want = c.want()
-    t, n, heads = c.query.dtype, len(c.lengths), 8
+    t, n, heads = c.query.dtype, len(c.lengths), 2 * group
     for off in (1, 2, 8):
         for by_heads in (False, True):
             shape = (heads, n, d + 16) if by_heads else (n, heads, d + 16)
@@ -370,11 +370,11 @@ def test_strides_of_queries_and_results(gpu_lib, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 100, 128])
+@pytest.mark.parametrize("d,group", [(64, 4), (100, 4), (128, 4), (128, 13), (64, 20)])
 @pytest.mark.parametrize("lengths", [[20000], [1, 30000, 0, 5], [4000] * 9, [0] * 50 + [9000], list(range(0, 700, 3)), [1] * 700, [0] * 300], ids=lambda x: f"{len(x)}x{max(x)}")
-def test_parts_of_rows(gpu_lib, dtype, d, lengths):
+def test_parts_of_rows(gpu_lib, dtype, d, group, lengths):
     """Few long rows, which many workers share, and many short ones; more requests than one pass of a block's threads."""
-    c = Case(gpu_lib, dtype, 2, 2, d, 4, lengths, 16, seed=len(lengths)).run()
+    c = Case(gpu_lib, dtype, 2, 2, d, group, lengths, 16, seed=len(lengths)).run()
     c.check()
     first = c.out.clone(), c.lse.clone()
     c.run()
@@ -388,10 +388,10 @@ def test_many_requests(gpu_lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 100])
-def test_blocks_that_are_none(gpu_lib, dtype, d):
+@pytest.mark.parametrize("d,group", [(64, 4), (100, 4), (64, 12)])
+def test_blocks_that_are_none(gpu_lib, dtype, d, group):
     """Tokens in blocks that are not the cache's are left out, whole rows and whole tiles of them too."""
-    c = Case(gpu_lib, dtype, 2, 2, d, 4, LENGTHS, 16, seed=9)
+    c = Case(gpu_lib, dtype, 2, 2, d, group, LENGTHS, 16, seed=9)
     blocks = c.planes[0].shape[0]
     bad = [-1, blocks, (1 << 31) - 1, -(1 << 31)]
     for r, table in enumerate(c.tables):
@@ -416,24 +416,24 @@ def test_lengths_out_of_range(gpu_lib, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 100])
+@pytest.mark.parametrize("d,group", [(64, 4), (100, 4), (64, 12)])
 @pytest.mark.parametrize("spread", [1e-3, 1.0, 60.0])
-def test_scores_of_all_sizes(gpu_lib, dtype, d, spread):
+def test_scores_of_all_sizes(gpu_lib, dtype, d, group, spread):
     """From nearly equal weights to one token that outweighs all others, at the end, the beginning and in the middle."""
-    Case(gpu_lib, dtype, 2, 2, d, 4, [700, 64, 65, 3, 1], 16, spread=spread, seed=1).run().check()
+    Case(gpu_lib, dtype, 2, 2, d, group, [700, 64, 65, 3, 1], 16, spread=spread, seed=1).run().check()
     for at in (0, 350, 699):
-        c = Case(gpu_lib, dtype, 2, 2, d, 4, [700], 16, seed=2)
-        c.planes[0][c.tables[0][at // 16], at % 16] = (c.query[0, ::4] * 8).to(c.query.dtype)
+        c = Case(gpu_lib, dtype, 2, 2, d, group, [700], 16, seed=2)
+        c.planes[0][c.tables[0][at // 16], at % 16] = (c.query[0, ::group] * 8).to(c.query.dtype)
         c.run().check()
     for scale in (0.0, -0.3, 4.0):
-        Case(gpu_lib, dtype, 2, 2, d, 4, [700, 64, 3], 16, scale=scale, seed=3).run().check()
+        Case(gpu_lib, dtype, 2, 2, d, group, [700, 64, 3], 16, scale=scale, seed=3).run().check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 128])
-def test_many_small_weights_beside_a_large_one(gpu_lib, dtype, d):
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 2), (64, 12)])
+def test_many_small_weights_beside_a_large_one(gpu_lib, dtype, d, group):
     """One token with weight 1, and 40000 with 2^-17 each, which together weigh a third of it; half's least normal number is 2^-14."""
-    c = Case(gpu_lib, dtype, 2, 1, d, 2, [40000], 16, seed=4, scale=1.0)
+    c = Case(gpu_lib, dtype, 2, 1, d, group, [40000], 16, seed=4, scale=1.0)
     c.query.zero_()
     c.query[..., 0] = 1
     c.planes[0].zero_()
@@ -443,11 +443,11 @@ def test_many_small_weights_beside_a_large_one(gpu_lib, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [64, 100])
-def test_values_that_are_not_finite(gpu_lib, dtype, d):
+@pytest.mark.parametrize("d,group", [(64, 2), (100, 2), (64, 10)])
+def test_values_that_are_not_finite(gpu_lib, dtype, d, group):
     """What is not finite among a request's own tokens shows in its rows as the formula has it, and in no other's."""
     inf = float("inf")
-    c = Case(gpu_lib, dtype, 2, 1, d, 2, [200] * 8, 16, seed=5)
+    c = Case(gpu_lib, dtype, 2, 1, d, group, [200] * 8, 16, seed=5)
     clean = c.run().out.clone()
     q, (k, v) = c.query, c.planes
     q[:, :, 0] = 1
@@ -472,7 +472,7 @@ def test_values_that_are_not_finite(gpu_lib, dtype, d):
     rest = [x for x in range(d) if x != 3]
     assert bool(torch.isfinite(c.out[4:6][:, :, rest]).all())
     # the first row again, without the token of weight 0
-    e = Case(gpu_lib, dtype, 2, 1, d, 2, [200] * 8, 16, seed=5)
+    e = Case(gpu_lib, dtype, 2, 1, d, group, [200] * 8, 16, seed=5)
     e.query.copy_(q)
     e.planes[0][row(1, 30)] = 0
     want = paged_ref.attend([torch.where(torch.isfinite(p), p, 0).cpu() for p in e.planes], q.cpu(), e.tables, e.lengths, block_size=16,

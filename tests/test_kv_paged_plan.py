@@ -90,8 +90,10 @@ def test_parts(native):
 def test_rows(native):
     rng = random.Random(2)
     rows = [[1], [2], [3], [1000], [1] * 7, [1] * 2000, [40000, 1, 1, 1, 70000], [5] * 300]
-    rows += [[max(1, int(2 ** rng.uniform(0, top))) for _ in range(rng.randrange(1, 400))] for top in (2, 5, 8, 11) for _ in range(25)]
+    rows += [[max(1, int(2 ** rng.uniform(0, top))) for _ in range(rng.randrange(1, 400))] for top in (2, 5, 8, 11) for _ in range(12)]
     for tiles in rows:
         a = np.array(tiles, dtype=np.uint32)
         for workers in (1, 2, 7, 148, 296, 592):
-            assert native.check_rows(pointer(a), len(tiles), ctypes.c_uint32(workers)) == 0, (tiles, workers)
+            for whole, least in ((1, 0), (2, 1), (4, 1), (8, 2), (16, 0)):
+                got = native.check_rows(pointer(a), len(tiles), *map(ctypes.c_uint32, (workers, whole, least)))
+                assert got == 0, (tiles, workers, whole, least)
