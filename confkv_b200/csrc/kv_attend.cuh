@@ -56,9 +56,9 @@ struct AttendArgs {
 // where the row begins in its part and into its place 0 where it goes on there, and join_kernel puts them together.
 
 struct PartShared {
-    uint64_t warp[8];
-    uint64_t found_sum;
-    uint32_t found;
+    uint32_t warp[8], rest[8];
+    uint32_t found, found_sum;
+    Span span;
 };
 
 __device__ __forceinline__ Span span_at(const AttendArgs& a, uint32_t r)
@@ -66,7 +66,7 @@ __device__ __forceinline__ Span span_at(const AttendArgs& a, uint32_t r)
     return span_of(a.lengths[r], a.limit, a.window);
 }
 
-__device__ __forceinline__ uint64_t warp_sum(uint64_t v)
+__device__ __forceinline__ uint32_t warp_sum(uint32_t v)
 {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
@@ -107,26 +107,43 @@ __device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
     return p->last != 0;
 }
 
-// Every thread gets the same; false for a worker that has no tiles.
+// Units of a row of a request.
+__device__ __forceinline__ uint32_t units_of(const Span& s) { return tiles_of(s, kTile) + kRowUnits; }
+
+// Every thread gets the same; false for a worker that has no tiles. The units of a row of each request are summed up in 32 bits;
+// the first kThreads requests are read once.
 template <uint32_t kThreads>
 __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Part* p)
 {
     const uint32_t t = threadIdx.x;
-    uint64_t sum = 0;
-    for (uint32_t r = t; r < a.requests; r += kThreads) {
-        sum += tiles_of(span_at(a, r), kTile) + kRowUnits;
+    const Span mine = t < a.requests ? span_at(a, t) : Span{};
+    uint32_t n = t < a.requests ? units_of(mine) : 0, up = n, rest = 0;
+    for (uint32_t r = t + kThreads; r < a.requests; r += kThreads) {
+        rest += units_of(span_at(a, r));
     }
-    sum = warp_sum(sum);
-    if (t % 32 == 0) {
-        s.warp[t / 32] = sum;
+    const auto scan = [&]() {
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t o = __shfl_up_sync(~0u, up, d);
+            up += t % 32 >= d ? o : 0;
+        }
+    };
+    scan();
+    rest = a.requests > kThreads ? warp_sum(rest) : 0;
+    if (t % 32 == 31) {
+        s.warp[t / 32] = up;
+        s.rest[t / 32] = rest;
     }
     __syncthreads();
-    uint64_t total = 0;
+    uint32_t before = 0, all = 0, total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kThreads / 32; ++w) {
-        total += s.warp[w];
+        before += w < t / 32 ? s.warp[w] : 0;
+        all += s.warp[w];
+        total += s.rest[w];
     }
-    p->total = total * a.rows;
+    total += all;
+    p->total = uint64_t{total} * a.rows;
     p->workers = workers_for(a.cutting, p->total, gridDim.x);
     if (blockIdx.x >= p->workers) {
         return false;
@@ -134,42 +151,40 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
     p->begin = part_start(p->total, p->workers, blockIdx.x);
     p->end = part_start(p->total, p->workers, blockIdx.x + 1);
     // the request that has unit `begin`: the one whose rows begin at or before it
-    uint64_t base = 0;
-    for (uint32_t from = 0; from < a.requests; from += kThreads) {
-        const uint32_t r = from + t;
-        const uint64_t n = r < a.requests ? uint64_t{tiles_of(span_at(a, r), kTile) + kRowUnits} * a.rows : 0;
-        uint64_t up = n;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const uint64_t o = __shfl_up_sync(~0u, up, d);
-            up += t % 32 >= d ? o : 0;
+    const auto look = [&](uint32_t r, const Span& span) {
+        if (uint64_t{before + up} * a.rows > p->begin && uint64_t{before + up - n} * a.rows <= p->begin) {
+            s.found = r;
+            s.found_sum = before + up - n;
+            s.span = span;
         }
+    };
+    look(t, mine);
+    for (uint32_t from = kThreads; uint64_t{all} * a.rows <= p->begin; from += kThreads) {
+        const uint32_t r = from + t;
+        const Span span = r < a.requests ? span_at(a, r) : Span{};
+        n = up = r < a.requests ? units_of(span) : 0;
+        scan();
         __syncthreads();
         if (t % 32 == 31) {
             s.warp[t / 32] = up;
         }
         __syncthreads();
-        uint64_t before = base, all = base;
+        before = all;
 #pragma unroll
         for (uint32_t w = 0; w < kThreads / 32; ++w) {
             before += w < t / 32 ? s.warp[w] : 0;
             all += s.warp[w];
         }
-        if (before + up > p->begin && before + up - n <= p->begin) {
-            s.found = r;
-            s.found_sum = before + up - n;
-        }
-        base = all;
-        if (all > p->begin) {
-            break;
-        }
+        look(r, span);
     }
     __syncthreads();
     p->request = s.found;
-    set_row(a, p);
-    const uint64_t in = p->begin - s.found_sum, units = p->tiles + kRowUnits;
-    p->row = in < (uint64_t{1} << 32) ? static_cast<uint32_t>(in) / static_cast<uint32_t>(units) : static_cast<uint32_t>(in / units);
-    p->row_begin = s.found_sum + p->row * units;
+    p->span = s.span;
+    p->tiles = tiles_of(p->span, kTile);
+    const uint64_t found_sum = uint64_t{s.found_sum} * a.rows, in = p->begin - found_sum;
+    const uint32_t units = p->tiles + kRowUnits;
+    p->row = in < (uint64_t{1} << 32) ? static_cast<uint32_t>(in) / units : static_cast<uint32_t>(in / units);
+    p->row_begin = found_sum + uint64_t{p->row} * units;
     p->first = cut_at(a.cutting, static_cast<int64_t>(p->begin - p->row_begin), p->tiles);
     p->last = cut_at(a.cutting, static_cast<int64_t>(p->end - p->row_begin), p->tiles);
     return p->last > p->first || next_row(a, p);
@@ -1298,25 +1313,24 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
     if (a.cut_by_row != 0) {
         request = blockIdx.x / a.rows;
         row = blockIdx.x - request * a.rows;
-        uint64_t total = 0, begin = 0;
+        uint32_t all = 0, before = 0;
         for (uint32_t r = t; r < a.requests; r += kAttendThreads) {
-            const uint64_t n = tiles_of(span_at(a, r), kTile) + kRowUnits;
-            total += n;
-            begin += r < request ? n : 0;
+            const uint32_t n = units_of(span_at(a, r));
+            all += n;
+            before += r < request ? n : 0;
         }
-        total = warp_sum(total);
-        begin = warp_sum(begin);
-        __shared__ uint64_t units[kAttendWarps][2];
+        all = warp_sum(all);
+        before = warp_sum(before);
+        __shared__ uint2 units[kAttendWarps];
         if (lane == 0) {
-            units[warp][0] = total;
-            units[warp][1] = begin;
+            units[warp] = make_uint2(all, before);
         }
         __syncthreads();
-        total = begin = 0;
+        uint64_t total = 0, begin = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kAttendWarps; ++w) {
-            total += units[w][0];
-            begin += units[w][1];
+            total += units[w].x;
+            begin += units[w].y;
         }
         const uint32_t tiles = tiles_of(span_at(a, request), kTile);
         total *= a.rows;

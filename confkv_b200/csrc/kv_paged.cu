@@ -317,7 +317,7 @@ extern "C" int lmcache_gpu_kv_resize_async(const lmcache_gpu_kv_tables* tables, 
     a.by_block = kv::make_fast_div(t.block_size);
     // the slots, and a few names a request
     const uint64_t units = std::max<uint64_t>(t.slots != nullptr ? t.capacity : 0, uint64_t{t.requests} * std::min(t.width, 32u));
-    const uint64_t grid = std::clamp<uint64_t>(units / (2 * kv::kResizeThreads), 1, kSms);
+    const uint64_t grid = std::clamp<uint64_t>((units + kv::kResizeThreads - 1) / kv::kResizeThreads, 1, kSms);
     return cuda_rc(launch(kv::resize_kernel, dim3(static_cast<uint32_t>(grid)), kv::kResizeThreads, 0,
                           reinterpret_cast<cudaStream_t>(stream), a));
 }
@@ -438,8 +438,8 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.chunks = (a.group + plan.heads - 1) / plan.heads;
     a.rows = l.heads * a.chunks;
     a.limit = kv::row_limit(t.width, pages->block_size);
-    // the units of all rows have to be countable
-    if (uint64_t{t.requests} * a.rows >= (uint64_t{1} << 51) / (a.limit / kv::kTile + 1 + kv::kRowUnits)) {
+    // the units of all requests, a row of each, are counted in 32 bits
+    if (t.requests >= (1u << 31) / (a.limit / kv::kTile + 1 + kv::kRowUnits)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     DeviceGuard guard(device);

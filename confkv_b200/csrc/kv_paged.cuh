@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_con
     __syncthreads();
     const uint32_t given = min(s.given, a.ring - cursor.count);
 
-    if (blockIdx.x == 0) {
+    // what requests keep, shared out by warps
+    if (warp % gridDim.x == blockIdx.x) {
         uint32_t start = s.tokens[t];
         for (uint32_t r = first; r < last; ++r) {
             const Change c = change_at(a, r);
@@ -166,63 +167,63 @@ __global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_con
             }
             start += stays ? 0 : c.tokens;
         }
-        if (t == 0) {
-            if (a.starts != nullptr) {
-                a.starts[a.requests] = total.tokens;
-            }
-            a.cursor_after[0] = static_cast<int32_t>(a.ring != 0 ? ring_place(cursor.first, total.take, a.ring) : 0);
-            a.cursor_after[1] = static_cast<int32_t>(cursor.count - total.take + given);
+    }
+    if (blockIdx.x == 0 && t == 0) {
+        if (a.starts != nullptr) {
+            a.starts[a.requests] = total.tokens;
         }
+        a.cursor_after[0] = static_cast<int32_t>(a.ring != 0 ? ring_place(cursor.first, total.take, a.ring) : 0);
+        a.cursor_after[1] = static_cast<int32_t>(cursor.count - total.take + given);
     }
 
-    const uint32_t step = gridDim.x * kResizeThreads;
-    const uint32_t me = blockIdx.x * kResizeThreads + t;
-    // names taken: the ring's front goes behind the blocks that requests have
-    for (uint64_t i = me; i < total.take; i += step) {
-        const uint32_t n = static_cast<uint32_t>(i), bucket = thread_of(s.take, n);
-        uint32_t r = bucket * a.per, in = s.take[bucket];
-        Change c = change_at(a, r);
-        while (n - in >= c.take) {
-            in += c.take;
-            c = change_at(a, ++r);
-        }
-        a.tables[r * a.table_stride + c.before + (n - in)] = a.free[ring_place(cursor.first, n, a.ring)];
-    }
-    // names given back, behind the ring's end
-    const uint32_t end = a.ring != 0 ? ring_place(cursor.first, cursor.count, a.ring) : 0;
-    for (uint64_t i = me; i < given; i += step) {
-        const uint32_t n = static_cast<uint32_t>(i), bucket = thread_of(s.give, n);
-        uint32_t r = bucket * a.per, in = s.give[bucket];
-        Change c = change_at(a, r);
-        while (n - in >= c.give) {
-            in += c.give;
-            c = change_at(a, ++r);
-        }
-        a.free[ring_place(end, n, a.ring)] = a.tables[r * a.table_stride + (c.before - c.give) + (n - in)];
-    }
-    // slots of new tokens; a block that was taken just now is read from the ring
+    // slots, names taken and names given back in one row, so that their trips to memory do not follow one another in a thread
     const uint32_t listed = a.slots != nullptr ? a.capacity : 0;
-    for (uint64_t i = me; i < listed; i += step) {
-        const uint32_t n = static_cast<uint32_t>(i);
-        int64_t slot = -1;
-        if (n < total.tokens) {
-            const uint32_t bucket = thread_of(s.tokens, n);
-            uint32_t r = bucket * a.per, in = s.tokens[bucket], taken = s.take[bucket];
+    const uint32_t end = a.ring != 0 ? ring_place(cursor.first, cursor.count, a.ring) : 0;
+    const uint64_t all = uint64_t{listed} + total.take + given;
+    for (uint64_t i = blockIdx.x * kResizeThreads + t; i < all; i += gridDim.x * kResizeThreads) {
+        if (i < listed) {
+            // the slot of a new token; a block that is taken just now is read from the ring
+            const uint32_t n = static_cast<uint32_t>(i);
+            int64_t slot = -1;
+            if (n < total.tokens) {
+                const uint32_t bucket = thread_of(s.tokens, n);
+                uint32_t r = bucket * a.per, in = s.tokens[bucket], taken = s.take[bucket];
+                Change c = change_at(a, r);
+                while (n - in >= c.tokens) {
+                    in += c.tokens;
+                    taken += c.take;
+                    c = change_at(a, ++r);
+                }
+                const uint32_t token = c.held + (n - in);
+                const uint32_t block = quotient(a.by_block, token);
+                const int32_t name = block < c.before ? a.tables[r * a.table_stride + block]
+                                                      : a.free[ring_place(cursor.first, taken + (block - c.before), a.ring)];
+                if (name >= 0 && static_cast<uint32_t>(name) < a.blocks) {
+                    slot = int64_t{name} * a.by_block.d + (token - block * a.by_block.d);
+                }
+            }
+            a.slots[n] = slot;
+        } else if (i < uint64_t{listed} + total.take) {
+            // the ring's front goes behind the blocks that requests have
+            const uint32_t n = static_cast<uint32_t>(i - listed), bucket = thread_of(s.take, n);
+            uint32_t r = bucket * a.per, in = s.take[bucket];
             Change c = change_at(a, r);
-            while (n - in >= c.tokens) {
-                in += c.tokens;
-                taken += c.take;
+            while (n - in >= c.take) {
+                in += c.take;
                 c = change_at(a, ++r);
             }
-            const uint32_t token = c.held + (n - in);
-            const uint32_t block = quotient(a.by_block, token);
-            const int32_t name = block < c.before ? a.tables[r * a.table_stride + block]
-                                                  : a.free[ring_place(cursor.first, taken + (block - c.before), a.ring)];
-            if (name >= 0 && static_cast<uint32_t>(name) < a.blocks) {
-                slot = int64_t{name} * a.by_block.d + (token - block * a.by_block.d);
+            a.tables[r * a.table_stride + c.before + (n - in)] = a.free[ring_place(cursor.first, n, a.ring)];
+        } else {
+            // behind the ring's end
+            const uint32_t n = static_cast<uint32_t>(i - listed - total.take), bucket = thread_of(s.give, n);
+            uint32_t r = bucket * a.per, in = s.give[bucket];
+            Change c = change_at(a, r);
+            while (n - in >= c.give) {
+                in += c.give;
+                c = change_at(a, ++r);
             }
+            a.free[ring_place(end, n, a.ring)] = a.tables[r * a.table_stride + (c.before - c.give) + (n - in)];
         }
-        a.slots[n] = slot;
     }
 }
 

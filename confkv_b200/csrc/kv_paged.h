@@ -61,8 +61,11 @@ KV_HD Cursor cursor_of(int32_t first, int32_t count, uint32_t ring)
 {
     Cursor c{};
     if (ring != 0) {
-        const int64_t f = first % static_cast<int64_t>(ring);
-        c.first = static_cast<uint32_t>(f < 0 ? f + ring : f);
+        c.first = static_cast<uint32_t>(first);
+        if (c.first >= ring) {
+            const int64_t f = first % static_cast<int64_t>(ring);
+            c.first = static_cast<uint32_t>(f < 0 ? f + ring : f);
+        }
         c.count = count < 0 ? 0 : (static_cast<uint32_t>(count) < ring ? static_cast<uint32_t>(count) : ring);
     }
     return c;
