@@ -551,7 +551,42 @@ struct MmaShape {
     static_assert(kShared + 4096 <= 227 * 1024, "more than a block has");
 };
 
-template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+// A warp's way through its block's part, 16 tokens at a step. Of a long row each warp takes a quarter of every tile. With ALONE, where the part
+// is long enough for four of them, whole rows of few tiles go to one warp each, in turns, and there is nothing to put together at their
+// ends: 1000 requests of up to 100 tokens of 8 key heads take 49 us, and 83 with all rows shared by the warps. The code for it costs
+// others 2 to 9 % (64 requests of up to 4096 tokens 32.3 us and 31.1, one of 256 tokens 7.6 and 7.0), so there are two kernels, and calls with rows enough
+// for parts of four rows take this one.
+template <bool ALONE>
+struct Walk {
+    Part p;
+    uint32_t whole;             // rows met that go to one warp
+    uint32_t token, step, left; // the next 16 tokens, those behind them, how many steps are left in the row
+
+    __device__ __forceinline__ bool alone(const AttendArgs& a) const
+    {
+        return ALONE && p.first == 0 && p.last == p.tiles && p.tiles <= a.cutting.whole_tiles &&
+               kAttendWarps * (p.tiles + kRowUnits) <= p.end - p.begin;
+    }
+
+    // At the row that p has, if it is one of this warp's, or the next one that is; false where there is none.
+    __device__ __forceinline__ bool enter(const AttendArgs& a, uint32_t warp)
+    {
+        while (alone(a) && whole++ % kAttendWarps != warp) {
+            if (!next_row(a, &p)) {
+                return false;
+            }
+        }
+        const bool one = alone(a);
+        token = p.span.first + (one ? 0 : p.first * kTile + warp * kWarpTokens);
+        step = one ? kWarpTokens : kTile;
+        left = one ? max(1u, (p.span.end - p.span.first + kWarpTokens - 1) / kWarpTokens) : p.last - p.first;
+        return true;
+    }
+
+    __device__ __forceinline__ bool next(const AttendArgs& a, uint32_t warp) { return next_row(a, &p) && enter(a, warp); }
+};
+
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE>
 __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(const __grid_constant__ AttendArgs a)
 {
     using Shape = MmaShape<T, DP, NT, ONE, STAGES>;
@@ -586,17 +621,19 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     const uint32_t tiles16 = (a.head_dim + 15) / 16, value_tiles = (a.value_dim + 15) / 16;
 
     // what is copied runs ahead of what is computed: the next tile to copy, and the tokens that each tile under way has
-    Part ahead = p;
-    bool more_rows = true;
+    Walk<ALONE> ahead{p, 0, 0, 0, 0};
+    bool more_rows = ahead.enter(a, warp);
+    Walk<ALONE> now = ahead;
+    bool more = more_rows;
     uint32_t tokens_of[STAGES];                 // bit i: token i of this warp's 16 is one
     uint32_t stage_in = 0, stage_out = 0;
     const auto copy_tile = [&]() -> uint32_t {
         uint32_t there = 0;
         if (more_rows) {
-            const uint32_t key_head = quotient(a.by_chunks, ahead.row);
-            const int32_t* table = a.tables + ahead.request * a.table_stride;
-            const uint32_t token = ahead.span.first + ahead.first * kTile + warp * kWarpTokens + lane % kWarpTokens;
-            int64_t offset = token < ahead.span.end ? token_offset(a, table, token) : -1;
+            const uint32_t key_head = quotient(a.by_chunks, ahead.p.row);
+            const int32_t* table = a.tables + ahead.p.request * a.table_stride;
+            const uint32_t token = ahead.token + lane % kWarpTokens;
+            int64_t offset = token < ahead.p.span.end ? token_offset(a, table, token) : -1;
             there = __ballot_sync(~0u, offset >= 0) & 0xffffu;
             offset = offset >= 0 ? offset + key_head * a.page_head_stride : 0;
             const uint32_t to = stage_base + stage_in * Shape::kStageBytes;
@@ -623,8 +660,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                     copy_chunk(r, k + lane - r * a.by_vector.d);
                 }
             }
-            if (++ahead.first == ahead.last) {
-                more_rows = next_row(a, &ahead);
+            ahead.token += ahead.step;
+            if (--ahead.left == 0) {
+                more_rows = ahead.next(a, warp);
             }
         }
         copies_end();
@@ -637,8 +675,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     }
 
     uint32_t turn = 0;
-    for (;;) {
-        const uint32_t tiles = p.last - p.first;
+    while (more) {
+        p = now.p;
+        const bool alone = ALONE && now.step == kWarpTokens;
         const uint32_t key_head = quotient(a.by_chunks, p.row), chunk = p.row - key_head * a.by_chunks.d;
         const uint32_t head = key_head * a.group + chunk * GH;              // the row's first query head
         const uint32_t heads = min(GH, a.group - chunk * GH);
@@ -671,7 +710,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
             }
         }
         bool any = false;
-        for (uint32_t t = 0; t < tiles; ++t) {
+        for (; now.left != 0; --now.left) {
             copies_wait<STAGES - 2>();
             __syncwarp();
             tokens_of[STAGES - 1] = copy_tile();
@@ -785,9 +824,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
             }
         }
 
-        // the four warps' sums together
-        float2 (&sums)[kAttendWarps][GH] = merge_sums[turn];
-        turn ^= 1;
+        const bool whole = p.last - p.first == p.tiles;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -797,98 +834,131 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                     l[n][j] += __shfl_xor_sync(~0u, l[n][j], d);
                 }
                 l[n][j] = m[n][j] == -INFINITY && l[n][j] == 0.0f && any ? 1.0f : l[n][j] * power_of_2(-kRaise);
-                if (lane < 4) {
-                    sums[warp][n * 8 + lane * 2 + j] = make_float2(m[n][j], l[n][j]);
-                }
             }
         }
-        __syncthreads();
+        if (alone) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t g = n * 8 + lane % 4 * 2 + j;
-                float top_of_all = -INFINITY;
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t g = n * 8 + lane % 4 * 2 + j;
+                    if (g < heads) {
+                        const float factor = result_factor(m[n][j], l[n][j]) * power_of_2(-kRaise);
+                        T* out = reinterpret_cast<T*>(a.out + p.request * a.out_stride + (head + g) * a.out_head_stride);
 #pragma unroll
-                for (uint32_t v = 0; v < kAttendWarps; ++v) {
-                    top_of_all = fmaxf(top_of_all, sums[v][g].x);
+                        for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t d = k * 16 + h * 8 + lane / 4;
+                                if (d < a.value_dim) {
+                                    out[d] = from_float<T>(o[k][n][j + 2 * h] * factor);
+                                }
+                            }
+                        }
+                        if (lane < 4 && a.lse != nullptr) {
+                            a.lse[p.request * a.lse_stride + head + g] = result_lse(m[n][j], l[n][j]);
+                        }
+                    }
                 }
-                const float f = top_of_all == -INFINITY ? 1.0f : power_of_2(m[n][j] - top_of_all - kRaise);
+            }
+        } else {
+            // the four warps' sums together
+            float2 (&sums)[kAttendWarps][GH] = merge_sums[turn];
+            turn ^= 1;
+            if (lane < 4) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        sums[warp][n * 8 + lane * 2 + j] = make_float2(m[n][j], l[n][j]);
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t g = n * 8 + lane % 4 * 2 + j;
+                    float top_of_all = -INFINITY;
+#pragma unroll
+                    for (uint32_t v = 0; v < kAttendWarps; ++v) {
+                        top_of_all = fmaxf(top_of_all, sums[v][g].x);
+                    }
+                    const float f = top_of_all == -INFINITY ? 1.0f : power_of_2(m[n][j] - top_of_all - kRaise);
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) {
+                        o[k][n][j] *= f;
+                        o[k][n][j + 2] *= f;
+                    }
+                }
+            }
+            // value lane / 4 (and 8 further on) of each 16, heads as above
+            float* const mine = merge + warp % 2 * (GH * kRow) + lane % 4 * 2 * kRow + lane / 4;
+            if (warp >= 2) {
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    o[k][n][j] *= f;
-                    o[k][n][j + 2] *= f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] = o[k][n][i];
+                        }
+                    }
                 }
             }
-        }
-        // value lane / 4 (and 8 further on) of each 16, heads as above
-        float* const mine = merge + warp % 2 * (GH * kRow) + lane % 4 * 2 * kRow + lane / 4;
-        if (warp >= 2) {
+            __syncthreads();
+            if (warp < 2) {
 #pragma unroll
-            for (int k = 0; k < KT; ++k) {
+                for (int k = 0; k < KT; ++k) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] = o[k][n][i];
+                        for (int i = 0; i < 4; ++i) {
+                            mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] += o[k][n][i];
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            const uint32_t at_place = blockIdx.x * 2 + (p.first == 0 ? 1 : 0);
+            for (uint32_t g = warp; g < heads; g += kAttendWarps) {
+                float2 part[kAttendWarps];
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kAttendWarps; ++w) {
+                    part[w] = sums[w][g];
+                    top = fmaxf(top, part[w].x);
+                }
+#pragma unroll
+                for (uint32_t w = 0; w < kAttendWarps; ++w) {
+                    sum += part[w].y * (top == -INFINITY ? 1.0f : power_of_2(part[w].x - top));
+                }
+                const float factor = whole ? result_factor(top, sum) : 1.0f;
+                T* out = reinterpret_cast<T*>(a.out + p.request * a.out_stride + (head + g) * a.out_head_stride);
+                float* partial = a.partial + (uint64_t{at_place} * GH + g) * a.value_pad;
+                for (uint32_t d = lane; d < a.value_dim; d += 32) {
+                    const float x = merge[g * kRow + d] + merge[(GH + g) * kRow + d];
+                    if (whole) {
+                        out[d] = from_float<T>(x * factor);
+                    } else {
+                        partial[d] = x;
+                    }
+                }
+                if (lane == 0) {
+                    if (!whole) {
+                        a.partial_sums[at_place * GH + g] = make_float2(top, sum);
+                    } else if (a.lse != nullptr) {
+                        a.lse[p.request * a.lse_stride + head + g] = result_lse(top, sum);
                     }
                 }
             }
         }
-        __syncthreads();
-        if (warp < 2) {
-#pragma unroll
-            for (int k = 0; k < KT; ++k) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mine[(n * 8 + i % 2) * kRow + k * 16 + i / 2 * 8] += o[k][n][i];
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        const bool whole = tiles == p.tiles;
-        const uint32_t at_place = blockIdx.x * 2 + (p.first == 0 ? 1 : 0);
-        for (uint32_t g = warp; g < heads; g += kAttendWarps) {
-            float2 part[kAttendWarps];
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kAttendWarps; ++w) {
-                part[w] = sums[w][g];
-                top = fmaxf(top, part[w].x);
-            }
-#pragma unroll
-            for (uint32_t w = 0; w < kAttendWarps; ++w) {
-                sum += part[w].y * (top == -INFINITY ? 1.0f : power_of_2(part[w].x - top));
-            }
-            const float factor = whole ? result_factor(top, sum) : 1.0f;
-            T* out = reinterpret_cast<T*>(a.out + p.request * a.out_stride + (head + g) * a.out_head_stride);
-            float* partial = a.partial + (uint64_t{at_place} * GH + g) * a.value_pad;
-            for (uint32_t d = lane; d < a.value_dim; d += 32) {
-                const float x = merge[g * kRow + d] + merge[(GH + g) * kRow + d];
-                if (whole) {
-                    out[d] = from_float<T>(x * factor);
-                } else {
-                    partial[d] = x;
-                }
-            }
-            if (lane == 0) {
-                if (!whole) {
-                    a.partial_sums[at_place * GH + g] = make_float2(top, sum);
-                } else if (a.lse != nullptr) {
-                    a.lse[p.request * a.lse_stride + head + g] = result_lse(top, sum);
-                }
-            }
-        }
-        const int4 cut = cut_of(a, p);
-        if (!next_row(a, &p)) {
-            note_cut(a, cut);
-            break;
-        }
+        more = now.next(a, warp);
     }
     copies_wait<0>();
+    // a row that is cut was the last one of every warp
+    note_cut(a, cut_of(a, p));
 }
 
 // ------------------------------------------------------------------ 16-bit types, many query heads

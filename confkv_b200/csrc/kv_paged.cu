@@ -186,13 +186,20 @@ AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
                       : any_plan<T, 1, 32, 1, 1, 2>();
 }
 
-template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE>
 AttendPlan mma_plan()
 {
     static std::atomic<uint64_t> allowed{0};
     using Shape = kv::MmaShape<T, DP, NT, ONE, STAGES>;
-    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, Shape::kHeads, BLOCKS * kSms,
+    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS, ALONE>, kv::join_kernel<T>, kv::kAttendThreads, Shape::kHeads, BLOCKS * kSms,
                       kv::Cutting{DP <= 128 ? 8u : 4u, 2}, Shape::kShared, &allowed};
+}
+
+// `rows`: of all requests; with four a worker whole rows may go to a warp each.
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
+AttendPlan mma_plan(uint64_t rows)
+{
+    return rows >= 4 * BLOCKS * kSms ? mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, true>() : mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, false>();
 }
 
 // Whether the 16-bit kernel takes vectors of this size, in a cache and of queries of this alignment.
@@ -212,25 +219,26 @@ AttendPlan wide_plan()
 }
 
 template <class T>
-AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
+AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t requests)
 {
     const uint32_t d = l.head_dim;
+    const uint64_t rows = requests * l.heads;       // with groups of up to 8
     const bool many = group > 16;
     if (l.planes == 2) {
         if (group <= 8) {
-            return d <= 64    ? mma_plan<T, 64, 1, false, 4, 3>()
-                   : d <= 128 ? mma_plan<T, 128, 1, false, 3, 2>()
-                   : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>()
-                              : mma_plan<T, 256, 1, false, 3, 1>();
+            return d <= 64    ? mma_plan<T, 64, 1, false, 4, 3>(rows)
+                   : d <= 128 ? mma_plan<T, 128, 1, false, 3, 2>(rows)
+                   : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>(rows)
+                              : mma_plan<T, 256, 1, false, 3, 1>(rows);
         }
         return d <= 64    ? (many ? wide_plan<T, 64, 2, false, 4, 2>() : wide_plan<T, 64, 1, false, 4, 2>())
                : d <= 128 ? (many ? wide_plan<T, 128, 2, false, 3, 2>() : wide_plan<T, 128, 1, false, 3, 2>())
                           : (many ? wide_plan<T, 256, 2, false, 3, 1>() : wide_plan<T, 256, 1, false, 3, 1>());
     }
     if (group <= 8 && d <= 320) {
-        return d <= 128   ? mma_plan<T, 128, 1, true, 5, 2>()
-               : d <= 256 ? mma_plan<T, 256, 1, true, 5, 1>()
-                          : mma_plan<T, 320, 1, true, 4, 1>();
+        return d <= 128   ? mma_plan<T, 128, 1, true, 5, 2>(rows)
+               : d <= 256 ? mma_plan<T, 256, 1, true, 5, 1>(rows)
+                          : mma_plan<T, 320, 1, true, 4, 1>(rows);
     }
     return d <= 128   ? (many ? wide_plan<T, 128, 2, true, 4, 2>() : wide_plan<T, 128, 1, true, 4, 2>())
            : d <= 256 ? (many ? wide_plan<T, 256, 2, true, 3, 1>() : wide_plan<T, 256, 1, true, 3, 1>())
@@ -238,10 +246,11 @@ AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group)
                       : (many ? wide_plan<T, 576, 2, true, 2, 1>() : wide_plan<T, 576, 1, true, 2, 1>());
 }
 
-AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t cache_alignment, uint64_t query_alignment)
+AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t cache_alignment, uint64_t query_alignment,
+                       uint64_t requests)
 {
     if (mma_takes(l, cache_alignment, query_alignment)) {
-        return l.dtype == kv::kBf16 ? mma_plan<__nv_bfloat16>(l, group) : mma_plan<__half>(l, group);
+        return l.dtype == kv::kBf16 ? mma_plan<__nv_bfloat16>(l, group, requests) : mma_plan<__half>(l, group, requests);
     }
     const bool fours = l.head_dim % 4 == 0 && cache_alignment >= 4 * kv::element_bytes(l.dtype);
     return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group, fours)
@@ -313,12 +322,14 @@ extern "C" int lmcache_gpu_kv_resize_async(const lmcache_gpu_kv_tables* tables, 
     a.limit = kv::row_limit(t.width, t.block_size);
     a.blocks = t.blocks;
     a.ring = t.ring;
-    a.per = (t.requests + kv::kResizeThreads - 1) / kv::kResizeThreads;
+    // a thread a request or two: 256 requests take 3.3 us with 256 threads and 4.3 with 1024, 2000 take 14.6 and 7.1
+    const uint32_t threads = t.requests <= 512 ? 256 : 1024;
+    a.per = (t.requests + threads - 1) / threads;
     a.by_block = kv::make_fast_div(t.block_size);
     // the slots, and a few names a request
     const uint64_t units = std::max<uint64_t>(t.slots != nullptr ? t.capacity : 0, uint64_t{t.requests} * std::min(t.width, 32u));
-    const uint64_t grid = std::clamp<uint64_t>((units + kv::kResizeThreads - 1) / kv::kResizeThreads, 1, kSms);
-    return cuda_rc(launch(kv::resize_kernel, dim3(static_cast<uint32_t>(grid)), kv::kResizeThreads, 0,
+    const uint64_t grid = std::clamp<uint64_t>((units + threads - 1) / threads, 1, kSms);
+    return cuda_rc(launch(threads == 256 ? kv::resize_kernel<256> : kv::resize_kernel<1024>, dim3(static_cast<uint32_t>(grid)), threads, 0,
                           reinterpret_cast<cudaStream_t>(stream), a));
 }
 
@@ -398,7 +409,7 @@ extern "C" size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layo
     const uint32_t group = query_heads / layout->heads;
     uint64_t most = 0;
     for (uint64_t alignment = 1; alignment <= 16; alignment *= 2) {
-        most = std::max(most, workspace_of(attend_plan(*layout, group, alignment, alignment), value_dim).size);
+        most = std::max(most, workspace_of(attend_plan(*layout, group, alignment, alignment, 0), value_dim).size);
     }
     return most;
 }
@@ -420,7 +431,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     const uint64_t query_bits = reinterpret_cast<uintptr_t>(t.query) | (t.requests > 1 ? t.query_stride * element : 0) |
                                 (t.query_heads > 1 ? t.query_head_stride * element : 0);
     const AttendPlan plan = attend_plan(l, t.query_heads / l.heads, alignment_of(layer_bits(l, *pages, layer, element)),
-                                        alignment_of(query_bits));
+                                        alignment_of(query_bits), t.requests);
     const Workspace w = workspace_of(plan, t.value_dim);
     if (!array_ok(t.workspace, 16) ||
         t.workspace_bytes < lmcache_gpu_kv_attend_workspace_size(layout, t.query_heads, t.value_dim)) {

@@ -18,7 +18,6 @@ namespace kv {
 // the first block), so that it knows where any name or slot belongs, and then writes its share of them. The sums saturate at
 // 2^31 - 1, which is more than any ring or list of slots holds.
 
-constexpr uint32_t kResizeThreads = 512;
 constexpr uint32_t kMost = 0x7fffffffu;   // rings and lists of slots are shorter
 
 struct ResizeArgs {
@@ -50,21 +49,23 @@ __device__ __forceinline__ Sums add(const Sums& a, const Sums& b)
 
 __device__ __forceinline__ Sums of_change(const Change& c) { return Sums{c.take, c.tokens, c.give}; }
 
+template <uint32_t THREADS>
 struct ResizeShared {
     // exclusive sums in front of each thread's requests, refused ones left out
-    uint32_t take[kResizeThreads], tokens[kResizeThreads], give[kResizeThreads];
-    Sums warp[kResizeThreads / 32];
+    uint32_t take[THREADS], tokens[THREADS], give[THREADS];
+    Sums warp[THREADS / 32];
     Sums before_refused;        // taken and listed in all
     uint32_t refused;           // the first request that is refused
     uint32_t given;
 };
 
 // The last of the threads' sums that is not above i.
-__device__ __forceinline__ uint32_t thread_of(const uint32_t* sums, uint32_t i)
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t thread_of(const uint32_t (&sums)[THREADS], uint32_t i)
 {
     uint32_t t = 0;
 #pragma unroll
-    for (uint32_t step = kResizeThreads / 2; step != 0; step /= 2) {
+    for (uint32_t step = THREADS / 2; step != 0; step /= 2) {
         if (sums[t + step] <= i) {
             t += step;
         }
@@ -83,9 +84,10 @@ __device__ __forceinline__ uint32_t ring_place(uint32_t first, uint32_t n, uint3
     return at >= ring ? at - ring : at;
 }
 
-__global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_constant__ ResizeArgs a)
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) resize_kernel(const __grid_constant__ ResizeArgs a)
 {
-    __shared__ ResizeShared s;
+    __shared__ ResizeShared<THREADS> s;
     dev::pdl_release();
     dev::pdl_wait();
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t / 32;
@@ -141,10 +143,10 @@ __global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_con
     const uint32_t stop = s.refused;
     if (refused == stop && stop < a.requests) {
         s.before_refused = at;                      // the thread that has it
-    } else if (stop == a.requests && t == kResizeThreads - 1) {
+    } else if (stop == a.requests && t == THREADS - 1) {
         s.before_refused = at;                      // the sums of all
     }
-    if (t == kResizeThreads - 1) {
+    if (t == THREADS - 1) {
         s.given = add(sum, mine).give;
     }
     __syncthreads();
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(kResizeThreads) resize_kernel(const __grid_con
     const uint32_t listed = a.slots != nullptr ? a.capacity : 0;
     const uint32_t end = a.ring != 0 ? ring_place(cursor.first, cursor.count, a.ring) : 0;
     const uint64_t all = uint64_t{listed} + total.take + given;
-    for (uint64_t i = blockIdx.x * kResizeThreads + t; i < all; i += gridDim.x * kResizeThreads) {
+    for (uint64_t i = blockIdx.x * THREADS + t; i < all; i += gridDim.x * THREADS) {
         if (i < listed) {
             // the slot of a new token; a block that is taken just now is read from the ring
             const uint32_t n = static_cast<uint32_t>(i);

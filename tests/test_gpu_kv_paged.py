@@ -381,10 +381,13 @@ def test_parts_of_rows(gpu_lib, dtype, d, group, lengths):
     assert torch.equal(c.out, first[0]) and torch.equal(c.lse, first[1])            # equal calls, equal bits
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-def test_many_requests(gpu_lib, dtype):
-    rng = random.Random(3)
-    Case(gpu_lib, dtype, 2, 1, 64, 2, [rng.choice([0, 1, 5, 70, 130]) for _ in range(5000)], 16).run().check()
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,planes,window", [(64, 2, 0), (72, 2, 100), (128, 2, 0), (256, 2, 0), (128, 1, 0), (320, 1, 70)])
+def test_many_requests(gpu_lib, dtype, d, planes, window):
+    """Rows enough that whole ones go to a warp each, empty and long ones among them."""
+    rng = random.Random(d)
+    lengths = [rng.choice([0, 1, 5, 16, 70, 130, 400]) if k % 300 else rng.choice([600, 5000]) for k in range(3000 if d < 256 else 1500)]
+    Case(gpu_lib, dtype, planes, 1, d, 2, lengths, 16, window=window, value_dim=d - 3 if planes == 1 else None).run().check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
