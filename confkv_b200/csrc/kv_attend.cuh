@@ -1446,11 +1446,14 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
         const uint32_t k = group + i * groups;
         ahead[i] = works && k < pieces ? value(k, column) : make_float4(0, 0, 0, 0);
     }
+    constexpr uint32_t kMine = (kMostWorkers + kAttendThreads - 1) / kAttendThreads;
+    float2 x[kMine];
     float top = -INFINITY;
-    for (uint32_t k = t; k < pieces; k += kAttendThreads) {
-        const float2 x = a.partial_sums[place(k)];
-        weights[k] = x.x;
-        top = fmaxf(top, x.x);
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+        const uint32_t k = t + i * kAttendThreads;
+        x[i] = k < pieces ? a.partial_sums[place(k)] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, x[i].x);
     }
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
@@ -1466,10 +1469,15 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
     }
     const float base = reference(top);
     float sum = 0.0f;
-    for (uint32_t k = t; k < pieces; k += kAttendThreads) {
-        const float w = top == -INFINITY ? 1.0f : exp2f(weights[k] - base);
-        weights[k] = w;
-        sum += a.partial_sums[place(k)].y * w;
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+        const uint32_t k = t + i * kAttendThreads;
+        if (k < pieces) {
+            // where no piece has a finite maximum, the sums say whether there were tokens
+            const float w = top == -INFINITY ? 1.0f : exp2f(x[i].x - base);
+            weights[k] = w;
+            sum += x[i].y * w;
+        }
     }
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {

@@ -506,7 +506,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
         // a worker's place where rows are many (one request, one key head, 131072 tokens: 27.9 us, and 42.0 the other way; 128 requests
         // of one key head: 19.6, and 21.3 with blocks that look at a row each)
         const uint32_t heads = std::min(plan.heads, a.group), rows = a.cut_by_row != 0 ? t.requests * a.rows : plan.workers;
-        const uint32_t shares = a.cut_by_row != 0 ? std::clamp(kSms / (rows * heads), 1u, (a.value_pad + 31) / 32) : 1u;
+        const uint32_t shares = a.cut_by_row != 0 ? std::clamp(kSms / (rows * heads), 1u, (a.value_pad + 15) / 16) : 1u;
         e = launch(plan.join, dim3(rows, heads, shares), kv::kAttendThreads, 0, s, a, plan.heads);
     }
     return cuda_rc(e);

@@ -81,7 +81,7 @@ class _Calls:
         """The address of a contiguous [count] tensor."""
         if t.dtype is not dtype or t.get_device() != self._index or t.shape != (count,):
             raise ValueError(f"kv paged: {name} is a {dtype} tensor of {count} values on {self.device}")
-        if count > 1 and t.stride(0) != 1:
+        if not t.is_contiguous():
             raise ValueError(f"kv paged: the values of {name} have to follow one another")
         return t.data_ptr()
 
@@ -118,10 +118,10 @@ class KvBlockTables(_Calls):
         handle = self._stream(stream)
         ptr, stride, width = self._rows(tables, n)
         row, i32 = self._row, torch.int32
-        ring = free.shape[0] if free.dim() == 1 else -1
+        ring = free.numel()
         slots_ptr = starts_ptr = capacity = 0
         if slots is not None:
-            capacity = slots.shape[0] if slots.dim() == 1 else -1
+            capacity = slots.numel()
             # an empty tensor has no address; any other than null says that there is a list, of no places
             slots_ptr = row("slots", slots, torch.int64, capacity) or 8
             if starts is not None:
