@@ -22,6 +22,11 @@ seal_batch_async / open_batch_async per rank).
 record (kv_codec) in the place of its bytes: quantise -> seal, and open ->
 dequantise. GB/s then counts the objects' bytes.
 
+--decode N (with --kv-format) goes on from there as a server does: the opened records are read back into a paged
+cache as the prompts of up to 4 requests, and N tokens are decoded over them: a step takes blocks and slots for one
+token of each request, and for every layer writes its keys and values and attends to the cache, 4 query heads a
+key head (kv_paged). The last layer's results are checked against plain attention.
+
 One process per GPU, each with its own key handle and stream; no data crosses
 GPUs. Every timed iteration starts after a barrier and runs INNER back-to-back
 calls; each rank times its own work with CUDA events on its stream and the
@@ -44,7 +49,8 @@ from . import hostmem, multigpu, workloads
 from .batch import DeviceBatch
 from .clocks import ClockSampler
 from .gpu_aesgcm import GpuAes128GcmKey, GpuAesGcmLibrary
-from .kv_codec import FORMATS, MX_BLOCK, KvCodec
+from .kv_codec import FORMATS, MX_BLOCK, KvCodec, PagedKvCache
+from .kv_paged import KvAttention, KvBlockTables
 
 ALIGN = 256
 INNER = 4  # calls per timed iteration
@@ -259,6 +265,117 @@ class QuantisedWork(RankWork):
                 all(within_format(x, y, self.codec.format) for x, y in zip(self.objects, self.restored)))
 
 
+def attended_within(out, query, keys, values, scale: float) -> bool:
+    """Whether out [heads, d] is softmax(scale query keys) values over keys, values [tokens, key heads, d] as the type goes: half a
+    step of it, and 2^-10 of the weighted sizes of the values for all roundings before (the weights' 2^-15 or 2^-11, and
+    those of the scores: head_dim 2^-23 of scale sum |q k| each)."""
+    q, k, v, got = query.double(), keys.double(), values.double(), out.double()
+    group = q.shape[0] // k.shape[1]
+    k, v = (x.repeat_interleave(group, 1) for x in (k, v))
+    p = torch.softmax(scale * torch.einsum("hd,thd->ht", q, k), -1)
+    want, size = torch.einsum("ht,thd->hd", p, v), torch.einsum("ht,thd->hd", p, v.abs())
+    return bool(((got - want).abs() <= want.abs() * torch.finfo(out.dtype).eps / 2 + size * 2.0 ** -10).all())
+
+
+class DecodeWork:
+    """The objects of a QuantisedWork as the prompts of up to 4 requests in a paged cache, read back from its opened
+    records, and decoding steps over them."""
+
+    BLOCK, GROUP = 16, 4
+
+    def __init__(self, lib, work: QuantisedWork, steps: int):
+        self.work, self.steps, codec = work, steps, work.codec
+        n, _, _, chunk, heads, d = work.objects.shape
+        dev, dtype = work.objects.device, work.objects.dtype
+        self.requests = min(4, n)
+        # as many objects a request as there are for all; those that are left over are not read back
+        self.chunks = n // self.requests
+        self.prompt = self.chunks * chunk
+        self.width = -(-(self.prompt + steps) // self.BLOCK)
+        blocks = self.requests * self.width
+        self.layers = [torch.zeros((codec.planes, blocks, self.BLOCK, heads, d), dtype=dtype, device=dev) for _ in range(codec.layers)]
+        cache = PagedKvCache(codec, self.layers)
+        self.cache = cache
+        self.tables = KvBlockTables(lib, blocks=blocks, block_size=self.BLOCK, device=dev)
+        self.attention = KvAttention(lib, cache, query_heads=self.GROUP * heads)
+        self.workspace = self.attention.workspace()
+
+        def ints(count, value=0, dtype=torch.int32):
+            return torch.full((count,), value, dtype=dtype, device=dev)
+
+        r = self.requests
+        g = torch.Generator(device=dev).manual_seed(7)
+        self.free = torch.randperm(blocks, generator=g, device=dev).to(torch.int32)
+        self.names = torch.zeros((r, self.width), dtype=torch.int32, device=dev)
+        self.none, self.prompts = ints(r), ints(r, self.prompt)
+        self.held, self.lengths, self.kept = ints(r), ints(r), ints(r)
+        self.cursor, self.after = ints(2), ints(2)
+        self.slots, self.new_slots = ints(r * self.prompt, dtype=torch.int64), ints(r, dtype=torch.int64)
+        self.ok = ints(r * self.chunks)
+        self.keys, self.values, self.query = (
+            torch.randn((r, h, d), generator=g, device=dev).to(dtype) for h in (heads, heads, self.GROUP * heads))
+        self.out = torch.zeros_like(self.query)
+
+    def restore(self):
+        """Blocks and slots for the prompts, and their records read back into them."""
+        w = self.work
+        self.cursor.copy_(torch.tensor([0, self.free.numel()], dtype=torch.int32), non_blocking=True)
+        self.tables.resize(self.names, self.none, self.prompts, self.free, self.cursor, kept=self.held, cursor_after=self.after,
+                           slots=self.slots, stream=w.stream)
+        self.cursor.copy_(self.after)
+        n = self.requests * self.chunks
+        w.codec.dequantise_paged(w.opened[:n], self.cache, self.slots.view(n, -1), ok=self.ok, stream=w.stream)
+
+    def step(self):
+        """One token of each request, through all layers."""
+        s, a = self.work.stream, self.attention
+        torch.add(self.held, 1, out=self.lengths)
+        self.tables.resize(self.names, self.held, self.lengths, self.free, self.cursor, kept=self.kept, cursor_after=self.after,
+                           slots=self.new_slots, stream=s)
+        for layer in range(len(self.layers)):
+            a.append(layer, self.new_slots, self.keys, self.values if self.work.codec.planes == 2 else None, stream=s)
+            a.attend(layer, self.query, self.names, self.kept, self.out, workspace=self.workspace, stream=s)
+        self.held.copy_(self.kept)
+        self.cursor.copy_(self.after)
+
+    def run(self) -> dict:
+        """Device times of reading the prompts back and of the steps, captured once and replayed, and whether what came out is right."""
+        w = self.work
+        with torch.cuda.stream(w.stream):
+            self.restore()                          # once before any is timed
+            self.step()
+            a, b, c = (torch.cuda.Event(enable_timing=True) for _ in range(3))
+            a.record(w.stream)
+            self.restore()
+            b.record(w.stream)
+            b.synchronize()
+        replay = w.graphed(self.step)
+        b2 = torch.cuda.Event(enable_timing=True)
+        b2.record(w.stream)
+        for _ in range(self.steps):
+            replay()
+        c.record(w.stream)
+        c.synchronize()
+        return {"requests": self.requests, "prompt_tokens": self.prompt, "decode_steps": self.steps,
+                "restore_ms": round(a.elapsed_time(b), 4), "decode_ms_per_step": round(b2.elapsed_time(c) / self.steps, 4),
+                "decode_ok": self.check()}
+
+    def check(self) -> bool:
+        """All records were the codec's, every request holds its prompt and the decoded tokens, and the last layer's results are those of
+        plain attention over what its slots should hold."""
+        if not bool((self.ok == 1).all()) or self.held.tolist() != [self.prompt + self.steps] * self.requests:
+            return False
+        last = len(self.layers) - 1
+        n = self.requests * self.chunks
+        prompt = self.work.restored[:n, :, last].unflatten(0, (self.requests, self.chunks))   # [r, chunks, planes, chunk, heads, d]
+        for r in range(self.requests):
+            planes = [torch.cat((prompt[r, :, p].flatten(0, 1), x[r].expand(self.steps, -1, -1)))
+                      for p, x in zip(range(self.work.codec.planes), (self.keys, self.values))]
+            if not attended_within(self.out[r], self.query[r], planes[0], planes[-1], self.attention.scale):
+                return False
+        return True
+
+
 def barrier(world, dev):
     if world > 1:
         torch.distributed.barrier()
@@ -367,6 +484,7 @@ def main():
     ap.add_argument("--api", default="both", choices=["both", "all", "per_object", "per_object_graph", "batched"],
                     help="both = per_object + batched; all adds per-object calls replayed from a CUDA graph")
     ap.add_argument("--kv-format", choices=FORMATS, help="seal the objects' records (kv_small, kv_llama8b, tp8)")
+    ap.add_argument("--decode", type=int, default=0, metavar="N", help="with --kv-format: N tokens decoded over the records read back")
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--iters", type=int, default=30)
     ap.add_argument("--min-log2", type=int, default=12)
@@ -374,6 +492,8 @@ def main():
     args = ap.parse_args()
     if args.kv_format and args.config not in ("kv_small", "kv_llama8b", "tp8"):
         ap.error("--kv-format takes the configurations of KV objects: kv_small, kv_llama8b, tp8")
+    if args.decode < 0 or args.decode and not args.kv_format:
+        ap.error("--decode takes a number of tokens, and --kv-format")
     rank, world, local = multigpu.rank_env()
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
@@ -413,6 +533,9 @@ def main():
                 work = QuantisedWork(lib, key, objects, args.kv_format, stream, workloads.make_ivs(1000 + rank, len(mine)))
                 emit({**extra, "kv_format": args.kv_format, "record_bytes": work.lens[0] if work.lens else 0},
                      measure(work, apis, args.warmup, args.iters, world, dev))
+                if args.decode and work.lens:
+                    result = DecodeWork(lib, work, args.decode).run()
+                    emit({**extra, "kv_format": args.kv_format}, [result])
             else:
                 plain, offs, lens = bf16_plain(shape, len(mine), seed=50 + rank, dev=dev)
                 run(lens, plain, offs, extra)

@@ -425,7 +425,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     const int64_t element = kv::element_bytes(l.dtype);
     if (!heads_ok(l, t.query_heads, t.value_dim) || t.requests >= kv::kMaxRequests || t.width >= kv::kMost ||
         t.query_stride < 0 || t.query_head_stride < 0 || t.out_stride < 0 || t.out_head_stride < 0 || t.lse_stride < 0 ||
-        t.table_stride < 0 || !std::isfinite(t.scale)) {
+        t.table_stride < 0 || !std::isfinite(t.scale * kv::kLog2e)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     const uint64_t query_bits = reinterpret_cast<uintptr_t>(t.query) | (t.requests > 1 ? t.query_stride * element : 0) |

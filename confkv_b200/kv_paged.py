@@ -18,7 +18,6 @@ and synchronises.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 
 import torch
@@ -155,8 +154,8 @@ class KvAttention(_Calls):
             raise ValueError("kv paged: attention takes vectors of 1024 values at most")
         if not 1 <= self.value_dim <= self.head_dim or self.planes == 2 and self.value_dim != self.head_dim:
             raise ValueError("kv paged: value_dim is head_dim, or with one plane 1 to head_dim")
-        if not math.isfinite(self.scale) or not 0 <= self.window < 1 << 32:
-            raise ValueError("kv paged: scale has to be finite, window 0 to 2^32 - 1")
+        if not abs(self.scale) < 2.0 ** 127 or not 0 <= self.window < 1 << 32:
+            raise ValueError("kv paged: scale has to be finite and below 2^127, window 0 to 2^32 - 1")
         self._layout = KvLayout(0, DTYPES.index(self.dtype), self.planes, self.layers, self.heads, self.head_dim)
         self._layout_ptr = ctypes.addressof(self._layout)
         lib = library.lib
@@ -200,7 +199,8 @@ class KvAttention(_Calls):
         """out[r] = softmax(scale query[r] keys) values over the `lengths[r]` tokens (int32) that row r of `tables` (int32 [requests,
         width]) names, the last `window` of them; zeros where there are none. query [requests, query_heads, head_dim], out
         [requests, query_heads, value_dim]; lse (float32 [requests, query_heads]): the log of the sum of exponents.
-        Without a workspace the call takes one of its own from torch's allocator."""
+        Without a workspace the call takes one of its own from torch's allocator. out, lse and the workspace share no memory with
+        one another or with what is read."""
         n = lengths.shape[0]
         query_at = self._vectors("query", query, (n, self.query_heads, self.head_dim))
         out_at = self._vectors("out", out, (n, self.query_heads, self.value_dim))

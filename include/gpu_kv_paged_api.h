@@ -36,10 +36,10 @@ typedef struct lmcache_gpu_kv_tables {
     int64_t* starts;         /* out, or null: requests + 1 places in `slots`, where each request's begin */
     uint64_t capacity;       /* places of `slots`, below 2^31 - 1 */
     uint32_t requests;       /* below 2^24 */
-    uint32_t width;
+    uint32_t width;          /* below 2^31 - 1 */
     uint32_t blocks;         /* of the cache; blocks * block_size < 2^31 */
     uint32_t block_size;
-    uint32_t ring;           /* below 2^31 */
+    uint32_t ring;           /* below 2^31 - 1 */
     uint32_t reserved;       /* set to 0 */
 } lmcache_gpu_kv_tables;
 
@@ -61,7 +61,7 @@ typedef struct lmcache_gpu_kv_tables {
  *
  * ERR_ARGUMENT before any launch: a null pointer (but slots and starts; free where ring is 0; any but
  * cursor and cursor_after where requests is 0), pointers that are not aligned to their
- * element, values out of the ranges above; kept, cursor_after, slots, starts, the ring or the rows sharing
+ * element, starts without slots, values out of the ranges above; kept, cursor_after, slots, starts, the ring or the rows sharing
  * memory with one another or with an input.
  */
 int lmcache_gpu_kv_resize_async(const lmcache_gpu_kv_tables* tables, int device, void* stream);
@@ -108,7 +108,7 @@ typedef struct lmcache_gpu_kv_attention {
     uint32_t requests;       /* below 2^24 */
     uint32_t query_heads;    /* a multiple of the cache's heads; query head j reads head j / (query_heads / heads) */
     uint32_t value_dim;      /* two planes: head_dim; one: 1 .. head_dim */
-    uint32_t width;
+    uint32_t width;          /* below 2^31 - 1 */
     uint32_t window;         /* 0: all tokens; else the last `window` */
     float scale;
 } lmcache_gpu_kv_attention;
@@ -123,10 +123,12 @@ size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layout* layout,
  * and lengths over width * block_size are that. Where no token is left, out is 0 and lse -infinity. What lies in the cache
  * beside the tokens is not read. Scores, sums and products are held in 32 bits; with 16-bit types the weights exp(s_i - m)
  * enter the products in that type (bfloat16: as the sum of two).
- * The order of the sums depends on the lengths and on the shapes alone: equal calls give equal bits.
+ * The order of the sums depends on the lengths, the shapes and the alignment alone: equal calls give equal bits.
+ * out, lse and the workspace share no memory with one another or with anything that is read, and the rows of out and lse not with one another.
  *
  * ERR_ARGUMENT before any launch: null or misaligned pointers, a layer that is none, head_dim above 1024, query_heads above 65535, a workspace
- * that is too small, a scale that is not finite, values out of the ranges above or of the codec's.
+ * that is too small, a scale that is not finite (times log2 e, in 32 bits), requests * (width * block_size / 64 + 4) of 2^31 or more, values out of the ranges
+ * above or of the codec's.
  */
 int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
                                 const lmcache_gpu_kv_attention* attention, int device, void* stream);

@@ -601,6 +601,60 @@ def test_a_captured_step(gpu_lib, dtype, d):
     del graph
 
 
+FIRST_CALL = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+from confkv_b200.gpu_aesgcm import GpuAesGcmLibrary
+from test_gpu_kv_paged import Case, assert_near, ints
+c = Case(GpuAesGcmLibrary(), {dtype!r}, 2, 2, {d}, {group}, [3000, 0, 17], 16)
+tables, lengths = ints(c.tables), ints(c.lengths)
+workspace = c.attention.workspace() if {own} else None
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c.attention.attend(0, c.query, tables, lengths, c.out, lse=c.lse, workspace=workspace)
+c.out.zero_()
+g.replay()
+torch.cuda.synchronize()
+c.check()
+"""
+
+
+@pytest.mark.parametrize("dtype,d,group,own", [("bf16", 128, 4, True), ("fp16", 64, 12, False), ("fp32", 100, 2, False)])
+def test_a_process_whose_first_call_is_captured(gpu_lib, dtype, d, group, own):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    tests = Path(__file__).resolve().parent
+    code = FIRST_CALL.format(paths=[str(tests), str(tests.parent)], dtype=dtype, d=d, group=group, own=own)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_two_graphs_with_one_workspace(gpu_lib):
+    """Replayed in turns on one stream."""
+    cases = [Case(gpu_lib, dtype, 2, 2, d, group, [5000, 70, 0, 400], 16, seed=d) for dtype, d, group in (("bf16", 128, 4), ("fp16", 64, 12), ("fp32", 100, 2))]
+    want = [c.want() for c in cases]
+    shared = torch.empty(max(c.attention.workspace().numel() for c in cases), dtype=torch.uint8, device="cuda")
+    at = [(ints(c.tables), ints(c.lengths)) for c in cases]
+    torch.cuda.synchronize()
+    graphs = []
+    for c, (tables, lengths) in zip(cases, at):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.attention.attend(0, c.query, tables, lengths, c.out, lse=c.lse, workspace=shared)
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for c, w in zip(cases, want):
+        assert_near(c.out, c.lse, *w)
+    del graphs
+
+
 @pytest.mark.parametrize("fmt", ["int8", "mxfp4"])
 def test_records_read_back_are_attended_to(gpu_lib, fmt):
     """A stored prompt: blocks for its tokens, its records read back into their slots, one more token, attention."""
