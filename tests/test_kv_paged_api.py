@@ -185,7 +185,7 @@ BAD_ATTENTION = [
     dict(query_stride=-1), dict(query_head_stride=-1), dict(out_stride=-1), dict(out_head_stride=-1), dict(lse_stride=-1),
     dict(table_stride=-1), dict(requests=1 << 24), dict(query_heads=0), dict(query_heads=12), dict(query_heads=1 << 17),
     dict(value_dim=0), dict(value_dim=63), dict(value_dim=65), dict(width=(1 << 31) - 1), dict(scale=float("nan")),
-    dict(scale=float("inf")), dict(scale=3e38), dict(requests=100, width=1 << 27), dict(requests=1 << 23, width=1000),
+    dict(scale=float("inf")), dict(scale=3e38), dict(requests=100, width=1 << 27), dict(requests=1 << 23, width=1024),
     # 2^24 requests of 32 heads of 2^31 tokens: more tiles than are counted
     dict(requests=(1 << 24) - 1, query_heads=65528, width=1 << 27),
 ]
