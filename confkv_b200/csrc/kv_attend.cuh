@@ -42,7 +42,8 @@ struct AttendArgs {
     uint32_t head_dim, value_dim, value_pad;
     float scale;                                // times log2 e: exponents are of base 2
     FastDiv by_block, by_chunks;
-    FastDiv by_vector;                          // chunks of 16 bytes of a vector
+    FastDiv by_vector;                          // granules of a vector
+    uint32_t granule;                           // bytes of a copy: 16, where SMALL 8 or 4
     Cutting cutting;
     uint32_t cut_by_row;                        // the rows are few
     uint32_t workers;                           // at most
@@ -297,13 +298,14 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(cons
         const int32_t* table = a.tables + p.request * a.table_stride;
         const uint32_t from = p.span.first + p.first * kTile;
         const uint32_t to = min(p.span.end, from + tiles * kTile);
-        // where the warp's next U tokens lie; the table is read one turn ahead
-        int64_t offset[U];
+        // where the warp's next 32 tokens lie, a token a lane, which is that of the turns to come
+        constexpr uint32_t kTurns = 32 / U;
+        int64_t offsets = -1;
+        uint32_t turn = kTurns;
         const auto find_tokens = [&](uint32_t at) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                offset[u] = at + u < to ? token_offset(a, table, at + u) : -1;
-            }
+            const uint32_t token = at + lane / U * (kAttendWarps * U) + lane % U;
+            offsets = token < to ? token_offset(a, table, token) : -1;
+            turn = 0;
         };
         find_tokens(from + warp * U);
         float q[GH][R], o[GH][R];
@@ -324,9 +326,10 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(cons
             uint32_t there = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const bool is = offset[u] >= 0;
+                const int64_t offset = __shfl_sync(~0u, offsets, turn * U + u);
+                const bool is = offset >= 0;
                 there |= is ? 1u << u : 0u;
-                const int64_t where = offset[u] + key_head * a.page_head_stride;
+                const int64_t where = offset + key_head * a.page_head_stride;
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
                     const uint32_t d = (lane + i * 32) * VEC;
@@ -343,7 +346,9 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_any_kernel(cons
                 }
             }
             any |= there != 0;
-            find_tokens(at + kAttendWarps * U);
+            if (++turn == kTurns) {
+                find_tokens(at + kAttendWarps * U);
+            }
             float s[N];
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
@@ -470,6 +475,16 @@ __device__ __forceinline__ void copy_16(uint32_t to, const char* from, bool ther
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
+// 4 or 8 bytes likewise.
+__device__ __forceinline__ void copy_small(uint32_t to, const char* from, bool there, uint32_t bytes)
+{
+    if (bytes == 8) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(there ? 8 : 0) : "memory");
+    } else {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+    }
+}
+
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <int N>
@@ -586,7 +601,7 @@ struct Walk {
     __device__ __forceinline__ bool next(const AttendArgs& a, uint32_t warp) { return next_row(a, &p) && enter(a, warp); }
 };
 
-template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE>
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE, bool SMALL>
 __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(const __grid_constant__ AttendArgs a)
 {
     using Shape = MmaShape<T, DP, NT, ONE, STAGES>;
@@ -649,7 +664,21 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
             };
             constexpr uint32_t kChunks = DP / 8;
-            if (32 % kChunks == 0 && chunks == kChunks) {
+            if constexpr (SMALL) {
+                const uint32_t size = a.granule;
+                for (uint32_t k = 0; k < kWarpTokens * a.by_vector.d; k += 32) {
+                    const uint32_t r = quotient(a.by_vector, k + lane), at = (k + lane - r * a.by_vector.d) * size;
+                    const int64_t from = __shfl_sync(~0u, offset, r) + at;
+                    const uint32_t where = to + r * Shape::kRowBytes + (((at / 16) ^ (r % 8)) * 16) + at % 16;
+                    const bool is = (there >> r & 1) != 0;
+                    if (r < kWarpTokens) {
+                        copy_small(where, a.planes[0] + from, is, size);
+                        if constexpr (!ONE) {
+                            copy_small(where + Shape::kPlaneBytes, a.planes[1] + from, is, size);
+                        }
+                    }
+                }
+            } else if (32 % kChunks == 0 && chunks == kChunks) {
 #pragma unroll
                 for (uint32_t k = 0; k < kWarpTokens * kChunks / 32; ++k) {
                     copy_chunk(k * (32 / kChunks) + lane / kChunks, lane % kChunks);
@@ -691,7 +720,8 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
             for (int k = 0; k < KT; ++k) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    q[k][n][j] = g < heads && static_cast<uint32_t>(k * 2 + j) < chunks
+                    const bool is = SMALL ? k * 16 + j * 8 + lane % 4 * 2 < a.head_dim : static_cast<uint32_t>(k * 2 + j) < chunks;
+                    q[k][n][j] = g < heads && is
                                      ? *reinterpret_cast<const uint32_t*>(from + k * 32 + j * 16) : 0u;
                 }
             }

@@ -157,6 +157,7 @@ struct AttendPlan {
     uint32_t heads;             // query heads of a row
     uint32_t workers;
     kv::Cutting cutting;
+    bool small;                 // copies of 4 or 8 bytes
     uint32_t shared;            // bytes of dynamic shared memory
     std::atomic<uint64_t>* allowed;     // devices on which the kernel may have them
 };
@@ -167,39 +168,47 @@ static_assert(4 * kSms <= kv::kMostWorkers);
 template <class T, int VEC, int R, int GH, int U, int BLOCKS>
 AttendPlan any_plan()
 {
-    return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, GH, BLOCKS * kSms, kv::Cutting{2, 1}, 0, nullptr};
+    return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, GH, BLOCKS * kSms, kv::Cutting{2, 1}, false, 0, nullptr};
 }
 
+// Steps of four values (float32, and what is too long for the 16-bit kernels) or single ones; as many query heads in a row as registers hold,
+// and no more than there are. Fewer blocks an SM than these spill less and hide less; measured, us: 17 requests of up to 3001 tokens, 3 key heads of
+// 100 float32, 2 query heads each, 3 blocks 16.6, 4 blocks 18.2; 16 requests of up to 2048, 8 heads of 128, 8 query heads
+// each, 2 blocks 46.1, 3 blocks 37.2, 4 blocks with half the tokens a turn 55.4.
 template <class T>
 AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
 {
-    if (fours) {
-        return d <= 128   ? (group == 1   ? any_plan<T, 4, 4, 1, 8, 3>()
-                             : group == 2 ? any_plan<T, 4, 4, 2, 8, 3>()
-                             : group <= 4 ? any_plan<T, 4, 4, 4, 8, 2>()
-                                          : any_plan<T, 4, 4, 8, 4, 2>())
-               : d <= 256 ? (group == 1 ? any_plan<T, 4, 8, 1, 4, 3>() : any_plan<T, 4, 8, 4, 4, 2>())
-                          : any_plan<T, 4, 32, 1, 2, 2>();
+    if constexpr (sizeof(T) == 4) {
+        if (fours && d <= 256) {
+            return d <= 128   ? (group == 1   ? any_plan<T, 4, 4, 1, 8, 3>()
+                                 : group == 2 ? any_plan<T, 4, 4, 2, 8, 3>()
+                                 : group <= 4 ? any_plan<T, 4, 4, 4, 4, 4>()
+                                              : any_plan<T, 4, 4, 8, 4, 3>())
+                   : group == 1 ? any_plan<T, 4, 8, 1, 4, 3>()
+                                : any_plan<T, 4, 8, 4, 4, 2>();
+        }
     }
-    return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 3>() : any_plan<T, 1, 4, 8, 4, 2>())
+    return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 3>() : any_plan<T, 1, 4, 8, 4, 3>())
            : d <= 256 ? (group == 1 ? any_plan<T, 1, 8, 1, 4, 3>() : any_plan<T, 1, 8, 4, 4, 2>())
+           : fours    ? any_plan<T, 4, 32, 1, 2, 2>()
                       : any_plan<T, 1, 32, 1, 1, 2>();
 }
 
-template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE>
+template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS, bool ALONE, bool SMALL>
 AttendPlan mma_plan()
 {
     static std::atomic<uint64_t> allowed{0};
     using Shape = kv::MmaShape<T, DP, NT, ONE, STAGES>;
-    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS, ALONE>, kv::join_kernel<T>, kv::kAttendThreads, Shape::kHeads, BLOCKS * kSms,
-                      kv::Cutting{DP <= 128 ? 8u : 4u, 2}, Shape::kShared, &allowed};
+    return AttendPlan{kv::attend_mma_kernel<T, DP, NT, ONE, STAGES, BLOCKS, ALONE, SMALL>, kv::join_kernel<T>, kv::kAttendThreads, Shape::kHeads, BLOCKS * kSms,
+                      kv::Cutting{DP <= 128 ? 8u : 4u, 2}, SMALL, Shape::kShared, &allowed};
 }
 
 // `rows`: of all requests; with four a worker whole rows may go to a warp each.
 template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
 AttendPlan mma_plan(uint64_t rows)
 {
-    return rows >= 4 * BLOCKS * kSms ? mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, true>() : mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, false>();
+    return rows >= 4 * BLOCKS * kSms ? mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, true, false>()
+                                     : mma_plan<T, DP, NT, ONE, STAGES, BLOCKS, false, false>();
 }
 
 // Whether the 16-bit kernel takes vectors of this size, in a cache and of queries of this alignment.
@@ -215,9 +224,13 @@ AttendPlan wide_plan()
     static std::atomic<uint64_t> allowed{0};
     using Shape = kv::WideShape<T, DP, NT, ONE, STAGES>;
     return AttendPlan{kv::attend_wide_kernel<T, DP, NT, ONE, STAGES, BLOCKS>, kv::join_kernel<T>, kv::kWideThreads, Shape::kHeads,
-                      BLOCKS * kSms, kv::Cutting{2, 1}, Shape::kShared, &allowed};
+                      BLOCKS * kSms, kv::Cutting{2, 1}, false, Shape::kShared, &allowed};
 }
 
+// Up to 8 query heads a key head: warps of their own; more, or long vectors: warps that share a tile. Measured, us: 64 requests of up to
+// 8192 tokens, one latent vector of 576, 16 query heads 134 with warps of their own and 44, 128 query heads 524 and 126; 32
+// requests of up to 4096, 8 key heads of 128, 16 query heads each 41 and 35 (of 64: 25 and 28, the one size where sharing loses). Stages and
+// blocks: what fills shared memory.
 template <class T>
 AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t requests)
 {
@@ -246,11 +259,34 @@ AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t req
                       : (many ? wide_plan<T, 576, 2, true, 2, 1>() : wide_plan<T, 576, 1, true, 2, 1>());
 }
 
+// Whether it takes them in copies of 4 or 8 bytes (32 requests of up to 2048 tokens, 8 key heads of 100, 4 query heads each: 26 us, 53 with
+// attend_any_kernel): even head sizes that are no multiple of 8, or addresses of less than 16 bytes.
+bool mma_takes_small(const lmcache_gpu_kv_layout& l, uint64_t cache_alignment, uint64_t query_alignment)
+{
+    return l.dtype != kv::kFp32 && l.head_dim % 2 == 0 && l.head_dim <= (l.planes == 2 ? 256u : 320u) && cache_alignment >= 4 &&
+           query_alignment >= 4;
+}
+
+template <class T>
+AttendPlan small_plan(const lmcache_gpu_kv_layout& l)
+{
+    const uint32_t d = l.head_dim;
+    if (l.planes == 1) {
+        return mma_plan<T, 320, 1, true, 4, 1, false, true>();
+    }
+    return d <= 64    ? mma_plan<T, 64, 1, false, 4, 3, false, true>()
+           : d <= 128 ? mma_plan<T, 128, 1, false, 3, 2, false, true>()
+                      : mma_plan<T, 256, 1, false, 3, 1, false, true>();
+}
+
 AttendPlan attend_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t cache_alignment, uint64_t query_alignment,
                        uint64_t requests)
 {
     if (mma_takes(l, cache_alignment, query_alignment)) {
         return l.dtype == kv::kBf16 ? mma_plan<__nv_bfloat16>(l, group, requests) : mma_plan<__half>(l, group, requests);
+    }
+    if (mma_takes_small(l, cache_alignment, query_alignment)) {
+        return l.dtype == kv::kBf16 ? small_plan<__nv_bfloat16>(l) : small_plan<__half>(l);
     }
     const bool fours = l.head_dim % 4 == 0 && cache_alignment >= 4 * kv::element_bytes(l.dtype);
     return l.dtype == kv::kBf16   ? any_plan<__nv_bfloat16>(l.head_dim, group, fours)
@@ -430,8 +466,8 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     }
     const uint64_t query_bits = reinterpret_cast<uintptr_t>(t.query) | (t.requests > 1 ? t.query_stride * element : 0) |
                                 (t.query_heads > 1 ? t.query_head_stride * element : 0);
-    const AttendPlan plan = attend_plan(l, t.query_heads / l.heads, alignment_of(layer_bits(l, *pages, layer, element)),
-                                        alignment_of(query_bits), t.requests);
+    const uint64_t cache_alignment = alignment_of(layer_bits(l, *pages, layer, element));
+    const AttendPlan plan = attend_plan(l, t.query_heads / l.heads, cache_alignment, alignment_of(query_bits), t.requests);
     const Workspace w = workspace_of(plan, t.value_dim);
     if (!array_ok(t.workspace, 16) ||
         t.workspace_bytes < lmcache_gpu_kv_attend_workspace_size(layout, t.query_heads, t.value_dim)) {
@@ -492,7 +528,8 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.cutting = plan.cutting;
     a.workers = plan.workers;
     a.cut_by_row = uint64_t{t.requests} * a.rows * std::min(plan.heads, a.group) <= kSms ? 1 : 0;
-    a.by_vector = kv::make_fast_div(std::max<uint32_t>(1, l.head_dim / 8));
+    a.granule = !plan.small ? 16 : std::min(cache_alignment, alignment_of(l.head_dim * element)) >= 8 ? 8 : 4;
+    a.by_vector = kv::make_fast_div(std::max(1u, static_cast<uint32_t>(l.head_dim * element / a.granule)));
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = allow_shared(plan, device);
     if (e != cudaSuccess) {
