@@ -229,13 +229,13 @@ AttendPlan wide_plan()
 
 // Up to 8 query heads a key head: warps of their own; more, or long vectors: warps that share a tile. Measured, us: 64 requests of up to
 // 8192 tokens, one latent vector of 576, 16 query heads 134 with warps of their own and 44, 128 query heads 524 and 126; 32
-// requests of up to 4096, 8 key heads of 128, 16 query heads each 41 and 35 (of 64: 25 and 28, the one size where sharing loses). Stages and
+// requests of up to 4096, 8 key heads of 128, 16 query heads each 41 and 35, but of 64 values 25 and 28. Stages and
 // blocks: what fills shared memory.
 template <class T>
 AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t requests)
 {
     const uint32_t d = l.head_dim;
-    const uint64_t rows = requests * l.heads;       // with groups of up to 8
+    const uint64_t rows = requests * l.heads;       // where a group is one row
     const bool many = group > 16;
     if (l.planes == 2) {
         if (group <= 8) {
@@ -244,7 +244,7 @@ AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t req
                    : d <= 192 ? mma_plan<T, 192, 1, false, 4, 1>(rows)
                               : mma_plan<T, 256, 1, false, 3, 1>(rows);
         }
-        return d <= 64    ? (many ? wide_plan<T, 64, 2, false, 4, 2>() : wide_plan<T, 64, 1, false, 4, 2>())
+        return d <= 64    ? (many ? wide_plan<T, 64, 2, false, 4, 2>() : mma_plan<T, 64, 2, false, 4, 2>(rows))
                : d <= 128 ? (many ? wide_plan<T, 128, 2, false, 3, 2>() : wide_plan<T, 128, 1, false, 3, 2>())
                           : (many ? wide_plan<T, 256, 2, false, 3, 1>() : wide_plan<T, 256, 1, false, 3, 1>());
     }

@@ -93,7 +93,8 @@ KV_HD uint32_t tiles_of(const Span& s, uint32_t tile)
 
 // Attention's work is counted in units: a row's tiles, and kRowUnits in front of them for its beginning and its end. The units of all rows, one row
 // behind the other, are cut into equal parts for `workers` <= total workers: worker c has the units [part_start(c),
-// part_start(c + 1)), one at least. total < 2^52, workers < 2^11.
+// part_start(c + 1)), one at least. total < 2^52, workers < 2^11. With one, two, three and five units in front of a row 64 ragged
+// requests take 34.9, 31.4, 31.7 and 33.3 us, and 128 of one key head 22.6, 21.0, 19.2 and 18.8.
 constexpr uint32_t kRowUnits = 3;
 
 KV_HD uint64_t part_start(uint64_t total, uint32_t workers, uint32_t c)
