@@ -122,7 +122,10 @@ __device__ __forceinline__ bool next_row(const AttendArgs& a, Part* p)
     }
     if (++p->row == a.rows) {
         p->row = 0;
-        ++p->request;
+        // lengths that something else changes meanwhile cost the results, not an address
+        if (++p->request >= a.requests) {
+            return false;
+        }
         set_row(a, p);
     }
     p->first = 0;
@@ -157,6 +160,10 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
         s.warp[t / 32] = up;
         s.rest[t / 32] = rest;
     }
+    if (t == 0) {
+        s.found = s.found_sum = 0;
+        s.span = mine;
+    }
     __syncthreads();
     uint32_t before = 0, all = 0, total = 0;
 #pragma unroll
@@ -182,7 +189,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, PartShared& s, Pa
         }
     };
     look(t, mine);
-    for (uint32_t from = kThreads; uint64_t{all} * a.rows <= p->begin; from += kThreads) {
+    for (uint32_t from = kThreads; from < a.requests && uint64_t{all} * a.rows <= p->begin; from += kThreads) {
         const uint32_t r = from + t;
         const Span span = r < a.requests ? span_at(a, r) : Span{};
         n = up = r < a.requests ? units_of(span) : 0;
@@ -1482,6 +1489,10 @@ __global__ void __launch_bounds__(kAttendThreads) join_kernel(const __grid_const
         return;
     }
     const uint32_t head = key_head * a.group + chunk * gh + g;
+    last = min(last, a.workers - 1);
+    if (last < c) {
+        return;
+    }
     const uint32_t pieces = last - c + 1;
     const auto place = [&](uint32_t k) { return (uint64_t{c + k} * 2 + (k == 0 ? 1 : 0)) * gh + g; };
     // columns of four values, and the groups of threads that share the pieces of one

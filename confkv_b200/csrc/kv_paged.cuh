@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(THREADS) resize_kernel(const __grid_constant__
         a.cursor_after[1] = static_cast<int32_t>(cursor.count - total.take + given);
     }
 
+    // (the bounds in the three searches hold by the sums; they keep every address in its array where something else changes the
+    // inputs while the call runs)
     // slots, names taken and names given back in one row, so that their trips to memory do not follow one another in a thread
     const uint32_t listed = a.slots != nullptr ? a.capacity : 0;
     const uint32_t end = a.ring != 0 ? ring_place(cursor.first, cursor.count, a.ring) : 0;
@@ -196,17 +198,19 @@ __global__ void __launch_bounds__(THREADS) resize_kernel(const __grid_constant__
                 const uint32_t bucket = thread_of(s.tokens, n);
                 uint32_t r = bucket * a.per, in = s.tokens[bucket], taken = s.take[bucket];
                 Change c = change_at(a, r);
-                while (n - in >= c.tokens) {
+                while (n - in >= c.tokens && r + 1 < a.requests) {
                     in += c.tokens;
                     taken += c.take;
                     c = change_at(a, ++r);
                 }
-                const uint32_t token = c.held + (n - in);
-                const uint32_t block = quotient(a.by_block, token);
-                const int32_t name = block < c.before ? a.tables[r * a.table_stride + block]
-                                                      : a.free[ring_place(cursor.first, taken + (block - c.before), a.ring)];
-                if (name >= 0 && static_cast<uint32_t>(name) < a.blocks) {
-                    slot = int64_t{name} * a.by_block.d + (token - block * a.by_block.d);
+                if (n - in < c.tokens) {
+                    const uint32_t token = c.held + (n - in);
+                    const uint32_t block = quotient(a.by_block, token), place = taken + (block - c.before);
+                    const int32_t name = block < c.before ? a.tables[r * a.table_stride + block]
+                                         : place < a.ring ? a.free[ring_place(cursor.first, place, a.ring)] : -1;
+                    if (name >= 0 && static_cast<uint32_t>(name) < a.blocks) {
+                        slot = int64_t{name} * a.by_block.d + (token - block * a.by_block.d);
+                    }
                 }
             }
             a.slots[n] = slot;
@@ -215,21 +219,25 @@ __global__ void __launch_bounds__(THREADS) resize_kernel(const __grid_constant__
             const uint32_t n = static_cast<uint32_t>(i - listed), bucket = thread_of(s.take, n);
             uint32_t r = bucket * a.per, in = s.take[bucket];
             Change c = change_at(a, r);
-            while (n - in >= c.take) {
+            while (n - in >= c.take && r + 1 < a.requests) {
                 in += c.take;
                 c = change_at(a, ++r);
             }
-            a.tables[r * a.table_stride + c.before + (n - in)] = a.free[ring_place(cursor.first, n, a.ring)];
+            if (n - in < c.take) {
+                a.tables[r * a.table_stride + c.before + (n - in)] = a.free[ring_place(cursor.first, n, a.ring)];
+            }
         } else {
             // behind the ring's end
             const uint32_t n = static_cast<uint32_t>(i - listed - total.take), bucket = thread_of(s.give, n);
             uint32_t r = bucket * a.per, in = s.give[bucket];
             Change c = change_at(a, r);
-            while (n - in >= c.give) {
+            while (n - in >= c.give && r + 1 < a.requests) {
                 in += c.give;
                 c = change_at(a, ++r);
             }
-            a.free[ring_place(end, n, a.ring)] = a.tables[r * a.table_stride + (c.before - c.give) + (n - in)];
+            if (n - in < c.give) {
+                a.free[ring_place(end, n, a.ring)] = a.tables[r * a.table_stride + (c.before - c.give) + (n - in)];
+            }
         }
     }
 }
