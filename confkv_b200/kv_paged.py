@@ -113,23 +113,30 @@ class KvBlockTables(_Calls):
         `kept` (int32 [requests]): what each holds then, `held` where it grows and there was no room; `cursor_after`: the
         cursor of the next call; `slots` (int64): the slots of all new tokens, -1 behind the last; `starts`
         (int64 [requests + 1]): where in it each request's begin. Outputs share no memory with inputs."""
-        n = held.shape[0]
+        shape = held.shape
+        n = shape[0]
         handle = self._stream(stream)
         ptr, stride, width = self._rows(tables, n)
-        row, i32 = self._row, torch.int32
-        ring = free.numel()
+        ring, i32, index = free.numel(), torch.int32, self._index
+        # all at once; where something is wrong, one by one to say what
+        good = len(shape) == 1 and lengths.shape == shape and kept.shape == shape and cursor.shape == cursor_after.shape == (2,)
+        for t in (held, lengths, kept, cursor, cursor_after):
+            good = good and t.dtype is i32 and t.get_device() == index and t.is_contiguous()
+        if not good:
+            for name, t, count in (("held", held, n), ("lengths", lengths, n), ("kept", kept, n), ("cursor", cursor, 2), ("cursor_after", cursor_after, 2)):
+                self._row(name, t, i32, count)
         slots_ptr = starts_ptr = capacity = 0
         if slots is not None:
             capacity = slots.numel()
             # an empty tensor has no address; any other than null says that there is a list, of no places
-            slots_ptr = row("slots", slots, torch.int64, capacity) or 8
+            slots_ptr = self._row("slots", slots, torch.int64, capacity) or 8
             if starts is not None:
-                starts_ptr = row("starts", starts, torch.int64, n + 1)
+                starts_ptr = self._row("starts", starts, torch.int64, n + 1)
         elif starts is not None:
             raise ValueError("kv paged: starts are places in slots")
-        raw = TABLES.pack(ptr, stride, row("held", held, i32, n), row("lengths", lengths, i32, n), row("free", free, i32, ring),
-                          row("cursor", cursor, i32, 2), row("kept", kept, i32, n), row("cursor_after", cursor_after, i32, 2),
-                          slots_ptr, starts_ptr, capacity, n, width, self.blocks, self.block_size, ring, 0)
+        raw = TABLES.pack(ptr, stride, held.data_ptr(), lengths.data_ptr(), self._row("free", free, i32, ring), cursor.data_ptr(),
+                          kept.data_ptr(), cursor_after.data_ptr(), slots_ptr, starts_ptr, capacity, n, width, self.blocks,
+                          self.block_size, ring, 0)
         rc = self._resize(raw, self._index, handle)
         if rc != 0:
             self.library.check(rc, "kv_resize")
