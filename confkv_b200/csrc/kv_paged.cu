@@ -174,7 +174,8 @@ AttendPlan any_plan()
 // Steps of four values (float32, and what is too long for the 16-bit kernels) or single ones; as many query heads in a row as registers hold,
 // and no more than there are. Fewer blocks an SM than these spill less and hide less; measured, us: 17 requests of up to 3001 tokens, 3 key heads of
 // 100 float32, 2 query heads each, 3 blocks 16.6, 4 blocks 18.2; 16 requests of up to 2048, 8 heads of 128, 8 query heads
-// each, 2 blocks 46.1, 3 blocks 37.2, 4 blocks with half the tokens a turn 55.4.
+// each, 2 blocks 46.1, 3 blocks 37.2, 4 blocks with half the tokens a turn 55.4; 32 requests of up to 4000 tokens, 16 query heads on a latent
+// vector of 320 float32, four heads in a row 51, one 154; of 576, two in a row 91, one 165.
 template <class T>
 AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
 {
@@ -187,6 +188,9 @@ AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
                    : group == 1 ? any_plan<T, 4, 8, 1, 4, 3>()
                                 : any_plan<T, 4, 8, 4, 4, 2>();
         }
+    }
+    if (fours && group > 1 && d > 256 && d <= 640) {
+        return d <= 384 ? any_plan<T, 4, 12, 4, 2, 2>() : any_plan<T, 4, 20, 2, 2, 2>();
     }
     return d <= 128   ? (group == 1 ? any_plan<T, 1, 4, 1, 8, 3>() : any_plan<T, 1, 4, 8, 4, 3>())
            : d <= 256 ? (group == 1 ? any_plan<T, 1, 8, 1, 4, 3>() : any_plan<T, 1, 8, 4, 4, 2>())

@@ -318,6 +318,13 @@ def test_groups(gpu_lib, dtype, d, group):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [260, 320, 384, 388, 576, 640, 644])
+def test_groups_of_long_vectors(gpu_lib, dtype, d):
+    for group in (1, 2, 3, 4, 5, 9):
+        Case(gpu_lib, dtype, 2, 2, d, group, [0, 1, 40, 130, 1000], 16, seed=group).run().check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("order", ["NHD", "HND"])
 @pytest.mark.parametrize("size", [1, 3, 5, 8, 16, 48, 64, 100, 256])
 def test_block_sizes(gpu_lib, dtype, order, size):
