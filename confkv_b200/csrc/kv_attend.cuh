@@ -12,7 +12,7 @@
 // where the wide kernel below is bound by its instructions.
 //
 // Measured on B200, us of the GPU a call with cold L2 (calls back to back in a graph; TB/s of the cache's bytes and the results):
-//   1 request of 131072 tokens, 8 key heads of 128, 4 query heads each, bfloat16        85.5   6.28
+//   1 request of 131072 tokens, 8 key heads of 128, 4 query heads each, bfloat16        86     6.24   (89.5 in a run of seconds)
 //   64 requests of up to 4096 tokens, as above                                          31.2   4.44
 //   64 requests of 2048 tokens, as above                                                89     6.04
 //   1000 requests of up to 100 tokens, as above                                         48.7   2.16
