@@ -445,11 +445,14 @@ extern "C" size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layo
     if (layout == nullptr || !heads_ok(*layout, query_heads, value_dim)) {
         return 0;
     }
-    // the most that any alignment's kernel takes
+    // the most that the kernel of any alignment takes; the cache's and the query's need not be the same
     const uint32_t group = query_heads / layout->heads;
+    const uint64_t element = kv::element_bytes(layout->dtype);
     uint64_t most = 0;
-    for (uint64_t alignment = 1; alignment <= 16; alignment *= 2) {
-        most = std::max(most, workspace_of(attend_plan(*layout, group, alignment, alignment, 0), value_dim).size);
+    for (uint64_t cache = element; cache <= 16; cache *= 2) {
+        for (uint64_t query = element; query <= 16; query *= 2) {
+            most = std::max(most, workspace_of(attend_plan(*layout, group, cache, query, 0), value_dim).size);
+        }
     }
     return most;
 }
@@ -474,7 +477,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     const AttendPlan plan = attend_plan(l, t.query_heads / l.heads, cache_alignment, alignment_of(query_bits), t.requests);
     const Workspace w = workspace_of(plan, t.value_dim);
     if (!array_ok(t.workspace, 16) ||
-        t.workspace_bytes < lmcache_gpu_kv_attend_workspace_size(layout, t.query_heads, t.value_dim)) {
+        t.workspace_bytes < std::max<uint64_t>(w.size, lmcache_gpu_kv_attend_workspace_size(layout, t.query_heads, t.value_dim))) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     if (t.requests == 0) {

@@ -721,3 +721,18 @@ def test_another_current_device(gpu_lib):
         c.attention.attend(0, c.query, tables, lengths, c.out, lse=c.lse)
     torch.cuda.synchronize(0)
     c.check()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d,value_dim,group", [(260, 1, 2), (300, 16, 4), (320, 64, 4), (320, 128, 8), (260, 16, 9), (320, 320, 3), (576, 64, 4)])
+def test_a_query_less_aligned_than_the_cache(gpu_lib, dtype, d, value_dim, group):
+    """Queries at an odd element over an aligned cache of latent vectors, with a workspace of exactly the bytes asked for."""
+    c = Case(gpu_lib, dtype, 1, 1, d, group, [20000, 0, 3000, 70], 16, value_dim=value_dim, seed=d + group)
+    raw = torch.zeros(c.query.numel() + 1, dtype=c.query.dtype, device="cuda")
+    query = raw[1:].view(c.query.shape)
+    query.copy_(c.query)
+    c.query = query
+    size = c.attention.workspace().numel()
+    space = torch.full((size + 8192,), 0x5a, dtype=torch.uint8, device="cuda")
+    c.run(workspace=space[:size]).check()
+    assert bool((space[size:] == 0x5a).all()), "wrote behind the workspace"

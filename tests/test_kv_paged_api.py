@@ -214,6 +214,35 @@ def test_workspace_size_is_what_the_call_takes(lib):
     assert lib.lmcache_gpu_kv_attend_workspace_size(ctypes.byref(layout(head_dim=1025)), 32, 1025) == 0
     assert lib.lmcache_gpu_kv_attend_workspace_size(None, 32, 64) == 0
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("d", range(260, 321, 4))
+def test_workspace_size_counts_a_query_less_aligned_than_the_cache(lib, dtype, d):
+    """16-bit latent vectors that only the kernel of any type takes with a query at an odd element: 2 blocks on each of 148 SMs, 4 query
+    heads in a row. A block has 16 bytes for its cut, and 2 places of 4 heads of 8 bytes and of value_dim floats, in fours."""
+    for group in range(2, 9):
+        for v in (1, 16, 64, 128, d):
+            b = layout(dtype, 1, 4, 1, d)
+            need = 296 * (16 + 2 * 4 * (8 + 4 * -(-v // 4) * 4))
+            assert lib.lmcache_gpu_kv_attend_workspace_size(ctypes.byref(b), group, v) >= need
+
+
+@pytest.mark.parametrize("dtype", range(3))
+@pytest.mark.parametrize("planes,d", [(2, 6), (2, 64), (2, 66), (2, 100), (2, 128), (2, 192), (2, 260), (2, 321), (2, 576), (2, 644), (1, 64), (1, 65), (1, 100),
+                                      (1, 128), (1, 256), (1, 260), (1, 300), (1, 320), (1, 384), (1, 576), (1, 640), (1, 1024)])
+def test_workspace_size_is_enough_for_every_alignment(lib, dtype, planes, d):
+    """A call refuses less than its own kernel takes, whatever the size function says."""
+    element = 4 if dtype == 2 else 2
+    for group in (1, 2, 4, 5, 8, 9, 16, 17, 64):
+        b = layout(dtype, planes, 4, 1, d)
+        v = d if planes == 2 else max(1, d - 3)
+        size = lib.lmcache_gpu_kv_attend_workspace_size(ctypes.byref(b), group, v)
+        for at in (element, 2 * element, 4 * element, 8 * element):
+            # one block of one token of one head: no stride counts, the addresses alone
+            p = pages(bases=[0x100000 + 0x10000 * k + at for k in range(8)], blocks=1, block_size=1)
+            for off in (element, 2 * element, 4 * element, 8 * element):
+                what = attention(workspace_bytes=size, query=0x800000 + off, query_heads=group, value_dim=v, requests=0)
+                assert lib.lmcache_gpu_kv_attend_async(ctypes.byref(b), ctypes.byref(p), 1, what, 0, None) == OK, (group, at, off)
+
 
 # ------------------------------------------------------------------ the binding
 
