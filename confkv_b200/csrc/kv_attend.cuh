@@ -566,6 +566,23 @@ __device__ __forceinline__ float power_of_2(float x)
     return r;
 }
 
+// Half has no normal numbers below 2^-14: weights of its kernels are held times 2^15, which is as far as the largest, 1, can be raised.
+template <class T>
+constexpr float kRaised = std::is_same_v<T, __half> ? 15.0f : 0.0f;
+
+// The weight of a score, raised. The maximum goes off first: where floats lie further than 1 apart there (2^24 and more), it raised by
+// itself would be rounded to another one, and its own weight to 2^16, more than half holds.
+template <class T>
+__device__ __forceinline__ float raised_weight(float s, float m)
+{
+    const float x = s - reference(m);
+    if constexpr (std::is_same_v<T, __half>) {
+        return power_of_2(x + kRaised<T>);
+    } else {
+        return power_of_2(x);
+    }
+}
+
 // Two values in one register, `lo` in the low half.
 template <class T>
 __device__ __forceinline__ uint32_t pack(float lo, float hi)
@@ -637,7 +654,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
     constexpr int KT = DP / 16;
     constexpr bool kTwoParts = std::is_same_v<T, __nv_bfloat16>;
     constexpr float kBelow = 1.0f - 0x1p-8f;
-    constexpr float kRaise = std::is_same_v<T, __half> ? 15.0f : 0.0f;
+    constexpr float kRaise = kRaised<T>;
     constexpr uint32_t GH = Shape::kHeads;
     extern __shared__ __align__(1024) char memory[];
     __shared__ PartShared part_shared;
@@ -843,11 +860,10 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
             uint32_t w[NT][2], rest[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float base[2] = {reference(m[n][0]) - kRaise, reference(m[n][1]) - kRaise};
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[i] = power_of_2(s[n][i] - base[i % 2]);
+                    x[i] = raised_weight<T>(s[n][i], m[n][i % 2]);
                     l[n][i % 2] += x[i];
                 }
 #pragma unroll
@@ -1052,7 +1068,7 @@ __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const
     using Shape = WideShape<T, DP, NT, ONE, STAGES>;
     constexpr bool kTwoParts = Shape::kTwoParts;
     constexpr float kBelow = 1.0f - 0x1p-8f;
-    constexpr float kRaise = std::is_same_v<T, __half> ? 15.0f : 0.0f;
+    constexpr float kRaise = kRaised<T>;
     constexpr uint32_t GH = Shape::kHeads;
     constexpr int KT = DP / 16;
     constexpr int VS = KT < 8 ? KT : 8, NS = 8 / VS;         // the warps' split of the result: by values, then by heads
@@ -1268,7 +1284,7 @@ __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float ref = head_half != 0 ? m[NT + n][i % 2] : m[n][i % 2];
-                    x[i] = power_of_2(s[n][i] - (reference(ref) - kRaise));
+                    x[i] = raised_weight<T>(s[n][i], ref);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {

@@ -736,3 +736,36 @@ def test_a_query_less_aligned_than_the_cache(gpu_lib, dtype, d, value_dim, group
     space = torch.full((size + 8192,), 0x5a, dtype=torch.uint8, device="cuda")
     c.run(workspace=space[:size]).check()
     assert bool((space[size:] == 0x5a).all()), "wrote behind the workspace"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("planes,d,group", [(2, 64, 4), (2, 64, 12), (2, 128, 12), (2, 100, 2), (1, 128, 4), (1, 320, 16), (1, 576, 20)])
+@pytest.mark.parametrize("size", [12000.0, 16384.0, 24000.0, 40000.0, 65504.0])
+def test_scores_of_millions(gpu_lib, dtype, planes, d, group, size):
+    """One channel of queries and keys so large that floats lie 2 to 32 apart at the scores. It alone makes the scores, so that they
+    are equal or far apart: a mean of the values of the tokens that have it, which errs by the rounding of its n sums, 2^-23 n of the values'
+    sizes, and its own to the type; and the score itself, rounded a few times."""
+    c = Case(gpu_lib, dtype, planes, 1, d, group, [200, 1, 64, 5000, 0], 16, seed=8)
+    channel = c.query.new_tensor(size)
+    c.query.zero_()
+    c.query[..., 0] = channel
+    tops = [[7], [0], list(range(64)), list(range(0, 5000, 3)), []]
+    for plane in c.planes:
+        plane.copy_(torch.nan_to_num(plane))
+    for table, x, top in zip(c.tables, c.lengths, tops):
+        for i in range(x):
+            c.planes[0][table[i // 16], i % 16, 0, 0] = channel if i in top else 0
+    c.run()
+    score = float(channel) ** 2 * c.scale
+    values = c.planes[-1].double().cpu()
+    for r, top in enumerate(tops):
+        if not top:
+            assert not c.out[r].any() and bool(torch.isneginf(c.lse[r]).all())
+            continue
+        v = torch.stack([values[c.tables[r][i // 16], i % 16, 0] for i in top])
+        want, n = v.mean(0), len(top)
+        got = c.out[r].double().cpu()
+        far = v.abs().mean(0) * (n + 8) * 2.0 ** -23 + want.abs() * torch.finfo(c.out.dtype).eps / 2 * 1.001 + 2.0 ** -25
+        assert bool(torch.isfinite(got).all()) and bool(((got - want).abs() <= far).all()), (r, (got - want).abs().max())
+        lse = score + float(np.log(n))
+        assert bool(((c.lse[r].double() - lse).abs() <= lse * 2.0 ** -21).all())
