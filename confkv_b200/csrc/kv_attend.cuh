@@ -596,6 +596,32 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi)
     return r;
 }
 
+// Two weights as the sums of two of T, so that the products have more of them than T's 8 or 11 bits: each cut to T's bits a little
+// below itself, and the rest. Neither is 0 where the weight is not, so that a value's infinity stays one. bfloat16: 2^-15 of the weight is lost. Half: 2^-20,
+// or 2^-23 (2^-38 before it was raised) where that is more: both are held at half's least number, 2^-24.
+template <class T>
+__device__ __forceinline__ void split(float lo, float hi, uint32_t& cut, uint32_t& rest)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        constexpr float kBelow = 1.0f - 0x1p-12f;
+        float c[2], r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x = i == 0 ? lo : hi, least = fminf(x * 0x1p102f, 0x1p-24f);
+            const float y = __uint_as_float(__float_as_uint(x * kBelow) & 0xffffe000u);
+            c[i] = fmaxf(y, least);
+            r[i] = fmaxf(x - y, least);
+        }
+        cut = pack<T>(c[0], c[1]);
+        rest = pack<T>(r[0], r[1]);
+    } else {
+        constexpr float kBelow = 1.0f - 0x1p-8f;
+        const uint32_t x = __float_as_uint(lo * kBelow), y = __float_as_uint(hi * kBelow);
+        cut = __byte_perm(x, y, 0x7632);
+        rest = pack<T>(lo - __uint_as_float(x & 0xffff0000u), hi - __uint_as_float(y & 0xffff0000u));
+    }
+}
+
 // DP: values of a vector in shared memory, a multiple of 64, zeros behind head_dim. NT: eights of query heads of a row. ONE: keys
 // and values are the same vectors. Vectors are whole chunks of 16 bytes; chunk c of token r lies at place c ^ (r % 8), so
 // that eight tokens' chunks of one column lie in different banks.
@@ -652,8 +678,6 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
 {
     using Shape = MmaShape<T, DP, NT, ONE, STAGES>;
     constexpr int KT = DP / 16;
-    constexpr bool kTwoParts = std::is_same_v<T, __nv_bfloat16>;
-    constexpr float kBelow = 1.0f - 0x1p-8f;
     constexpr float kRaise = kRaised<T>;
     constexpr uint32_t GH = Shape::kHeads;
     extern __shared__ __align__(1024) char memory[];
@@ -868,15 +892,10 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if constexpr (kTwoParts) {
-                        // the weight cut to 8 bits a little below itself, and the rest: both above 0, so that a value's infinity stays one
-                        const uint32_t lo = __float_as_uint(x[2 * h] * kBelow), hi = __float_as_uint(x[2 * h + 1] * kBelow);
-                        w[n][h] = across(__byte_perm(lo, hi, 0x7632));
-                        rest[n][h] = across(pack<T>(x[2 * h] - __uint_as_float(lo & 0xffff0000u),
-                                                    x[2 * h + 1] - __uint_as_float(hi & 0xffff0000u)));
-                    } else {
-                        w[n][h] = across(pack<T>(x[2 * h], x[2 * h + 1]));
-                    }
+                    uint32_t cut, more_of_it;
+                    split<T>(x[2 * h], x[2 * h + 1], cut, more_of_it);
+                    w[n][h] = across(cut);
+                    rest[n][h] = across(more_of_it);
                 }
             }
             {
@@ -890,9 +909,7 @@ __global__ void __launch_bounds__(kAttendThreads, BLOCKS) attend_mma_kernel(cons
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             multiply<T>(o[k][n], x, w[n][0], w[n][1]);
-                            if constexpr (kTwoParts) {
-                                multiply<T>(o[k][n], x, rest[n][0], rest[n][1]);
-                            }
+                            multiply<T>(o[k][n], x, rest[n][0], rest[n][1]);
                         }
                     }
                 }
@@ -1049,7 +1066,6 @@ constexpr uint32_t kWideWarps = kWideThreads / 32;
 
 template <class T, int DP, int NT, bool ONE, int STAGES>
 struct WideShape {
-    static constexpr bool kTwoParts = std::is_same_v<T, __nv_bfloat16>;
     static constexpr uint32_t kHeads = 16 * NT;
     static constexpr uint32_t kRowBytes = DP * 2;
     static constexpr uint32_t kPlaneBytes = kTile * kRowBytes;
@@ -1058,7 +1074,7 @@ struct WideShape {
     static constexpr uint32_t kWeightRow = kHeads * 2 + 16;             // bytes; eight tokens' rows lie in different banks
     static constexpr uint32_t kWeightBytes = kTile * kWeightRow;
     static constexpr uint32_t kWeights = kQuery + kHeads * kRowBytes;
-    static constexpr uint32_t kShared = kWeights + kWeightBytes * (kTwoParts ? 2 : 1);
+    static constexpr uint32_t kShared = kWeights + 2 * kWeightBytes;
     static_assert(kShared + 4096 <= 227 * 1024, "more than a block has");
 };
 
@@ -1066,8 +1082,6 @@ template <class T, int DP, int NT, bool ONE, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const __grid_constant__ AttendArgs a)
 {
     using Shape = WideShape<T, DP, NT, ONE, STAGES>;
-    constexpr bool kTwoParts = Shape::kTwoParts;
-    constexpr float kBelow = 1.0f - 0x1p-8f;
     constexpr float kRaise = kRaised<T>;
     constexpr uint32_t GH = Shape::kHeads;
     constexpr int KT = DP / 16;
@@ -1294,15 +1308,7 @@ __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t* const to = reinterpret_cast<uint32_t*>(memory + at + h * 8 * Shape::kWeightRow);
-                    if constexpr (kTwoParts) {
-                        // the weight cut to 8 bits a little below itself, and the rest: both above 0, so that a value's infinity stays one
-                        const uint32_t lo = __float_as_uint(x[2 * h] * kBelow), hi = __float_as_uint(x[2 * h + 1] * kBelow);
-                        *to = __byte_perm(lo, hi, 0x7632);
-                        to[Shape::kWeightBytes / 4] = pack<T>(x[2 * h] - __uint_as_float(lo & 0xffff0000u),
-                                                              x[2 * h + 1] - __uint_as_float(hi & 0xffff0000u));
-                    } else {
-                        *to = pack<T>(x[2 * h], x[2 * h + 1]);
-                    }
+                    split<T>(x[2 * h], x[2 * h + 1], *to, to[Shape::kWeightBytes / 4]);
                 }
             }
             if (__any_sync(~0u, faded)) {
@@ -1339,14 +1345,12 @@ __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const
                             w[n + 1][0] = x[2];
                             w[n + 1][1] = x[3];
                         }
-                        if constexpr (kTwoParts) {
-                            load_matrices_across(x, at + n * 16 + Shape::kWeightBytes);
-                            rest[n][0] = x[0];
-                            rest[n][1] = x[1];
-                            if constexpr (RT > 1) {
-                                rest[n + 1][0] = x[2];
-                                rest[n + 1][1] = x[3];
-                            }
+                        load_matrices_across(x, at + n * 16 + Shape::kWeightBytes);
+                        rest[n][0] = x[0];
+                        rest[n][1] = x[1];
+                        if constexpr (RT > 1) {
+                            rest[n + 1][0] = x[2];
+                            rest[n + 1][1] = x[3];
                         }
                     }
                 }
@@ -1361,9 +1365,7 @@ __global__ void __launch_bounds__(kWideThreads, BLOCKS) attend_wide_kernel(const
 #pragma unroll
                         for (int n = 0; n < RT; ++n) {
                             multiply<T>(o[v][n], x, w[n][0], w[n][1]);
-                            if constexpr (kTwoParts) {
-                                multiply<T>(o[v][n], x, rest[n][0], rest[n][1]);
-                            }
+                            multiply<T>(o[v][n], x, rest[n][0], rest[n][1]);
                         }
                     }
                 }

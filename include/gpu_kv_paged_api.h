@@ -121,8 +121,9 @@ size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layout* layout,
  * over the request's tokens (the last `window` of them). k is the layer's first plane, v its second; with one plane
  * v_i is the first value_dim values of k_i. Tokens whose block is not one of the cache's are left out, lengths below 0 are 0,
  * and lengths over width * block_size are that. Where no token is left, out is 0 and lse -infinity. What lies in the cache
- * beside the tokens is not read. Scores, sums and products are held in 32 bits; with 16-bit types the weights exp(s_i - m)
- * enter the products in that type (bfloat16: as the sum of two).
+ * beside the tokens is not read. Scores, sums and products are held in 32 bits; with 16-bit types the weights exp(s_i - m), m the
+ * largest score, may enter the products as the sum of two values of that type (off by 2^-15 of a weight in bfloat16; by 2^-20
+ * of it in half, or by 2^-38 where that is more).
  * The order of the sums depends on the lengths, the shapes and the alignment alone: equal calls give equal bits.
  * out, lse and the workspace share no memory with one another or with anything that is read, and the rows of out and lse not with one another.
  *

@@ -769,3 +769,72 @@ def test_scores_of_millions(gpu_lib, dtype, planes, d, group, size):
         assert bool(torch.isfinite(got).all()) and bool(((got - want).abs() <= far).all()), (r, (got - want).abs().max())
         lse = score + float(np.log(n))
         assert bool(((c.lse[r].double() - lse).abs() <= lse * 2.0 ** -21).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("planes,d,group", [(2, 64, 2), (2, 64, 12), (2, 100, 4), (2, 128, 4), (2, 128, 12), (2, 192, 20), (1, 128, 4), (1, 320, 16), (1, 576, 20)])
+def test_weights_have_more_bits_than_the_type(gpu_lib, dtype, planes, d, group):
+    """Values that cancel: what is left shows the weights' own roundings. Scores are of one product, exact, and times the scale; they err by
+    3 2^-24 of their size, their difference from the maximum and its power by 2^-22; weights enter the products with 2^-15 (bfloat16) or
+    2^-20 (half) of theirs; sums of n by n 2^-23. The result's own rounding is that of a small number."""
+    lengths = [2, 3, 5, 9, 16, 17, 40] * 3
+    c = Case(gpu_lib, dtype, planes, 1, d, group, lengths, 16, seed=11, scale=0.7)
+    t = c.query.dtype
+    g = torch.Generator(device="cuda").manual_seed(12)
+    c.query.zero_()
+    c.query[..., 0] = 1
+    for plane in c.planes:
+        plane.copy_(torch.nan_to_num(plane))
+    step = {"bf16": 2.0 ** -15, "fp16": 2.0 ** -20}[dtype]
+    for r, x in enumerate(lengths):
+        at = [(c.tables[r][i // 16], i % 16) for i in range(x)]
+        s = -4 * torch.rand(x, generator=g, device="cuda")
+        s[int(torch.randint(x, (1,), generator=g, device="cuda"))] = 0
+        for (b, row), y in zip(at, s.to(t)):
+            c.planes[0][b, row, 0, 0] = y
+        keys = torch.stack([c.planes[0][b, row, 0, 0] for b, row in at]).double()
+        v = torch.stack([c.planes[-1][b, row, 0] for b, row in at]).double()
+        p = torch.softmax(0.7 * keys, 0)
+        last = (-(p[:-1, None] * v[:-1]).sum(0) / p[-1]).clamp(-60000, 60000)
+        if planes == 1:
+            last[0] = keys[-1]
+        c.planes[-1][at[-1]] = last[None].to(t)
+    c.run()
+    got = c.out.double()
+    worst = 0.0
+    for r, x in enumerate(lengths):
+        at = [(c.tables[r][i // 16], i % 16) for i in range(x)]
+        keys = torch.stack([c.planes[0][b, row, 0, 0] for b, row in at]).double()
+        v = torch.stack([c.planes[-1][b, row, 0] for b, row in at]).double()
+        p = torch.softmax(0.7 * keys, 0)
+        want, sizes = p @ v, p @ v.abs()
+        far = sizes * (step + 4 * 0.7 * 4 * 2.0 ** -24 + 2.0 ** -22 + (x + 4) * 2.0 ** -23) + want.abs() * torch.finfo(t).eps / 2 * 1.01 + 2.0 ** -24
+        off = (got[r] - want).abs() / far
+        worst = max(worst, float(off.max()))
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,group", [(64, 2), (64, 12), (100, 4), (128, 12), (192, 20), (256, 3)])
+def test_infinite_values_of_small_weights(gpu_lib, dtype, d, group):
+    """A value's infinity stays one as far down as floats have the weight, and a thousand finite values beside it are as they were."""
+    c = Case(gpu_lib, dtype, 2, 1, d, group, [3, 100, 1000, 5000], 16, seed=13, scale=1.0)
+    c.query.zero_()
+    c.query[..., 0] = 1
+    for plane in c.planes:
+        plane.copy_(torch.nan_to_num(plane))
+    for k, score in enumerate((-8.0, -20.0, -31.0, -60.0)):
+        for r, x in enumerate(c.lengths):
+            for i in range(x):
+                c.planes[0][c.tables[r][i // 16], i % 16, 0, 0] = score if i else 0
+        c.run().check()
+        clean = c.out.clone()
+        at = [(c.tables[r][(x - 1) // 16], (x - 1) % 16, 0, 5 + k) for r, x in enumerate(c.lengths)]
+        for r, place in enumerate(at):
+            c.planes[-1][place] = float("inf") if r % 2 else float("-inf")
+        c.run()
+        for r, place in enumerate(at):
+            assert bool((c.out[r, :, 5 + k] == (float("inf") if r % 2 else float("-inf"))).all())
+            c.planes[-1][place] = 0.5
+        rest = [i for i in range(d) if i != 5 + k]
+        assert torch.equal(c.out[:, :, rest], clean[:, :, rest])
