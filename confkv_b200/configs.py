@@ -79,6 +79,8 @@ class RankWork:
         self.open_entries = [(fb + self.fr_off[i], ob + self.pt_off[i], n, n + 29, ab + 4 * i)
                              for i, n in enumerate(self.lens)]
         self.bseal = self.bopen = None
+        # `stream` need not wait for the current one by itself, which still fills the buffers above and the plaintext
+        stream.wait_stream(torch.cuda.current_stream(dev))
         if self.lens:
             self.bseal = DeviceBatch(lib, len(self.lens), dev)
             self.bopen = DeviceBatch(lib, len(self.lens), dev)
@@ -341,6 +343,7 @@ class DecodeWork:
     def run(self) -> dict:
         """Device times of reading the prompts back and of the steps, captured once and replayed, and whether what came out is right."""
         w = self.work
+        w.stream.wait_stream(torch.cuda.current_stream(w.stream.device))       # which still fills the tensors that __init__ made
         with torch.cuda.stream(w.stream):
             self.restore()                          # once before any is timed
             self.step()

@@ -1,7 +1,9 @@
 """The config runner's verdict on attention, and its arguments."""
 
+import contextlib
 import subprocess
 import sys
+import types
 
 import pytest
 import torch
@@ -30,3 +32,56 @@ def test_right_results_pass_and_wrong_ones_do_not(dtype):
 def test_arguments(more):
     r = subprocess.run([sys.executable, "-m", "confkv_b200.configs", "--config", "kv_small", *more], capture_output=True, text=True, timeout=120)
     assert r.returncode == 2 and "--decode" in r.stderr
+
+
+class Order:
+    """A stream that notes what waits for it or uses it, in turn."""
+
+    device = torch.device("cuda", 0)
+
+    def __init__(self):
+        self.notes = []
+
+    def wait_stream(self, other):
+        self.notes.append(("wait", other))
+
+
+class Stop(Exception):
+    pass
+
+
+def test_decoding_waits_for_the_stream_that_filled_its_tensors(monkeypatch):
+    stream = Order()
+    d = object.__new__(configs.DecodeWork)
+    d.work = types.SimpleNamespace(stream=stream)
+
+    def restore():
+        stream.notes.append("restore")
+        raise Stop
+
+    d.restore = restore
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: f"current of {device}")
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    with pytest.raises(Stop):
+        d.run()
+    assert stream.notes == [("wait", "current of cuda:0"), "restore"]
+
+
+def test_sealing_waits_for_the_stream_that_filled_its_buffers(monkeypatch):
+    stream = Order()
+
+    class Batch:
+        def __init__(self, lib, count, device):
+            self.workspace_bytes = 0
+
+        def seal(self, key, entries, stream):
+            stream.notes.append("seal")
+
+        def open(self, key, entries, stream):
+            stream.notes.append("open")
+
+    monkeypatch.setattr(configs, "DeviceBatch", Batch)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: f"current of {device}")
+    plain = torch.zeros(64, dtype=torch.uint8)
+    configs.RankWork(None, None, [5, 20], plain, [0, 16], stream, [b"0" * 12] * 2)
+    assert stream.notes == [("wait", "current of cpu"), "seal", "open"]

@@ -46,3 +46,20 @@ def test_the_command(gpu_lib):
     assert r.returncode == 0, r.stderr[-2000:]
     lines = [json.loads(x) for x in r.stdout.splitlines()]
     assert lines[0]["round_trip_ok"] and lines[1]["decode_ok"] and lines[1]["decode_ms_per_step"] > 0
+
+
+def test_decode_behind_a_busy_stream(gpu_lib):
+    """The constructors' fills still wait behind other work of the current stream when the work's own stream starts."""
+    objects = workloads.bf16_batch((2, 2, 48, 2, 40), 8, seed=4, device="cuda")
+    stream = torch.cuda.Stream()
+    with GpuAes128GcmKey(gpu_lib, workloads.make_key(1)) as key:
+        torch.cuda.synchronize()
+        torch.cuda._sleep(200_000_000)          # a tenth of a second
+        work = configs.QuantisedWork(gpu_lib, key, objects, "int8", stream, workloads.make_ivs(2, 8))
+        work.seal_batched()
+        work.open_batched()
+        torch.cuda._sleep(200_000_000)
+        got = configs.DecodeWork(gpu_lib, work, 6).run()
+        torch.cuda.synchronize()
+        assert got["decode_ok"] and work.round_trip_ok()
+        del work
