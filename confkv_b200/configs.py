@@ -379,6 +379,15 @@ class DecodeWork:
         return True
 
 
+def decoded_by_all(result: dict | None, dev) -> dict | None:
+    """This rank's DecodeWork.run() with the verdict of all ranks and the times of the slowest. Called by every rank, with None by one
+    that has no objects."""
+    times = ("restore_ms", "decode_ms_per_step")
+    ok = multigpu.all_ok(result is None or result["decode_ok"], device=dev)
+    slowest = multigpu.reduce_max([result[t] if result else 0.0 for t in times], device=dev)
+    return result and {**result, **dict(zip(times, slowest)), "decode_ok": ok}
+
+
 def barrier(world, dev):
     if world > 1:
         torch.distributed.barrier()
@@ -536,9 +545,9 @@ def main():
                 work = QuantisedWork(lib, key, objects, args.kv_format, stream, workloads.make_ivs(1000 + rank, len(mine)))
                 emit({**extra, "kv_format": args.kv_format, "record_bytes": work.lens[0] if work.lens else 0},
                      measure(work, apis, args.warmup, args.iters, world, dev))
-                if args.decode and work.lens:
-                    result = DecodeWork(lib, work, args.decode).run()
-                    emit({**extra, "kv_format": args.kv_format}, [result])
+                if args.decode:
+                    result = decoded_by_all(DecodeWork(lib, work, args.decode).run() if work.lens else None, dev)
+                    emit({**extra, "kv_format": args.kv_format}, [result] if result else [])
             else:
                 plain, offs, lens = bf16_plain(shape, len(mine), seed=50 + rank, dev=dev)
                 run(lens, plain, offs, extra)

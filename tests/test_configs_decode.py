@@ -1,6 +1,9 @@
 """The config runner's verdict on attention, and its arguments."""
 
 import contextlib
+import datetime
+import multiprocessing
+import socket
 import subprocess
 import sys
 import types
@@ -85,3 +88,45 @@ def test_sealing_waits_for_the_stream_that_filled_its_buffers(monkeypatch):
     plain = torch.zeros(64, dtype=torch.uint8)
     configs.RankWork(None, None, [5, 20], plain, [0, 16], stream, [b"0" * 12] * 2)
     assert stream.notes == [("wait", "current of cpu"), "seal", "open"]
+
+
+def _decoding_rank(rank, world, port, q):
+    import os
+
+    import torch.distributed as dist
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=60))
+    try:
+        def result(ms, ok):
+            return {"requests": 4, "restore_ms": ms, "decode_ms_per_step": 10 - ms, "decode_ok": ok}
+
+        q.put((rank, [configs.decoded_by_all(result(1.0 + rank, True), None), configs.decoded_by_all(result(1.0 + rank, rank == 0), None),
+                      configs.decoded_by_all(result(2.0, True) if rank == 0 else None, None)]))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_the_verdict_on_decoding_is_that_of_all_ranks():
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = multiprocessing.get_context("spawn")
+    q = ctx.Queue()
+    ranks = [ctx.Process(target=_decoding_rank, args=(r, 2, port, q)) for r in range(2)]
+    for p in ranks:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in ranks)
+    for p in ranks:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    right = {"requests": 4, "restore_ms": 2.0, "decode_ms_per_step": 9.0, "decode_ok": True}
+    for rank in range(2):
+        assert got[rank][:2] == [right, {**right, "decode_ok": False}]
+    assert got[0][2] == {**right, "decode_ms_per_step": 8.0} and got[1][2] is None
+
+
+def test_the_verdict_on_decoding_of_one_process():
+    result = {"requests": 4, "restore_ms": 1.5, "decode_ms_per_step": 2.5, "decode_ok": False}
+    assert configs.decoded_by_all(result, None) == result
+    assert configs.decoded_by_all(None, None) is None
