@@ -493,7 +493,7 @@ extern "C" int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, 
     a.rows = l.heads * a.chunks;
     a.limit = kv::row_limit(t.width, pages->block_size);
     // the units of all requests, a row of each, are counted in 32 bits
-    if (t.requests >= (1u << 31) / (a.limit / kv::kTile + 1 + kv::kRowUnits)) {
+    if (uint64_t{t.requests} * (a.limit / kv::kTile + 1 + kv::kRowUnits) >= (uint64_t{1} << 31)) {
         return LMCACHE_GPU_AESGCM_ERR_ARGUMENT;
     }
     DeviceGuard guard(device);

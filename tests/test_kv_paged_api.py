@@ -244,6 +244,19 @@ def test_workspace_size_is_enough_for_every_alignment(lib, dtype, planes, d):
                 assert lib.lmcache_gpu_kv_attend_async(ctypes.byref(b), ctypes.byref(p), 1, what, 0, None) == OK, (group, at, off)
 
 
+NO_DEVICE = 1 << 20         # what passes all checks gets as far as this device, and no further
+
+
+@pytest.mark.parametrize("width", [1024, 1025, 5000, 1 << 20])
+def test_the_most_requests_for_a_width(lib, width):
+    """As many as the header says: requests * (width * block_size / 64 + 4) below 2^31."""
+    most = ((1 << 31) - 1) // (width * 16 // 64 + 4)
+    for requests, refused in ((most, False), (most + 1, True)):
+        what = attention(requests=requests, width=width, table_stride=width)
+        rc = lib.lmcache_gpu_kv_attend_async(ctypes.byref(layout()), ctypes.byref(pages()), 1, what, NO_DEVICE, None)
+        assert (rc == ERR_ARG) == refused and rc != OK
+
+
 # ------------------------------------------------------------------ the binding
 
 def cache(cpu_lib, planes=2, head_dim=64, dtype=BF16, layers=2, overlap=False):
