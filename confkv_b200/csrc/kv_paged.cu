@@ -65,6 +65,20 @@ bool meet(const Range& a, const Range& b)
     return a.begin < a.end && b.begin < b.end && a.begin < b.end && b.begin < a.end;
 }
 
+// Whether any of n rows of `width` bytes, `stride` bytes apart, shares memory with a range; what lies between rows is not theirs.
+bool rows_meet(const void* rows, uint64_t n, uint64_t stride, uint64_t width, const Range& r)
+{
+    const Range all = range_of(rows, n != 0 && width != 0 ? (n - 1) * stride + width : 0);
+    if (!meet(all, r)) {
+        return false;
+    }
+    if (n == 1 || r.begin <= all.begin) {
+        return true;
+    }
+    const uint64_t row = (r.begin - all.begin) / stride, first = all.begin + row * stride;      // the last that begins at or before the range
+    return r.begin < first + width || r.end > first + stride;
+}
+
 bool tables_ok(const lmcache_gpu_kv_tables& t)
 {
     if (t.requests >= kv::kMaxRequests || t.width >= kv::kMost || t.ring >= kv::kMost || t.block_size == 0 ||
@@ -88,10 +102,20 @@ bool tables_ok(const lmcache_gpu_kv_tables& t)
                          range_of(t.cursor_after, 8),
                          range_of(t.slots, 8 * t.capacity),
                          range_of(t.starts, 8 * (n + 1)),
-                         range_of(t.free, 4 * uint64_t{t.ring}),
-                         range_of(n != 0 && t.width != 0 ? t.tables : nullptr, 4 * ((n != 0 ? n - 1 : 0) * static_cast<uint64_t>(t.table_stride) + t.width))};
+                         range_of(t.free, 4 * uint64_t{t.ring})};
     const Range in[] = {range_of(t.held, 4 * n), range_of(t.lengths, 4 * n), range_of(t.cursor, 8)};
+    const auto in_tables = [&](const Range& r) {
+        return rows_meet(t.tables, n, 4 * static_cast<uint64_t>(t.table_stride), 4 * uint64_t{t.width}, r);
+    };
+    for (const Range& r : in) {
+        if (in_tables(r)) {
+            return false;
+        }
+    }
     for (size_t i = 0; i < std::size(out); ++i) {
+        if (in_tables(out[i])) {
+            return false;
+        }
         for (size_t k = i + 1; k < std::size(out); ++k) {
             if (meet(out[i], out[k])) {
                 return false;

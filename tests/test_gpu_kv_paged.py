@@ -838,3 +838,27 @@ def test_infinite_values_of_small_weights(gpu_lib, dtype, d, group):
             c.planes[-1][place] = 0.5
         rest = [i for i in range(d) if i != 5 + k]
         assert torch.equal(c.out[:, :, rest], clean[:, :, rest])
+
+
+def test_resize_of_arrays_between_the_rows(gpu_lib):
+    """Whatever the call reads and writes beside the tables lies between their rows."""
+    rng = random.Random(14)
+    w, new = world(rng, 12, 9, 16, 40, 0.2, 1.2)
+    want = paged_ref.resize(**w, capacity=20)
+    gap, width = 64, 9
+    big = torch.full((12, width + gap), -77, dtype=I32, device="cuda")
+    rows = big[:, :width]
+    rows.copy_(ints(w["tables"]))
+    names = {"held": w["held"], "lengths": w["lengths"], "cursor": w["cursor"], "kept": [0] * 12, "cursor_after": [0, 0]}
+    at = {}
+    for k, (name, values) in enumerate(names.items()):
+        at[name] = big[2 * k, width + 3:width + 3 + len(values)]
+        at[name].copy_(ints(values))
+    free = ints(w["ring"])
+    slots = big.view(-1)[width + (width + gap) + 10:][:40].view(I64)        # 8-byte aligned: (9 + 73 + 10) names
+    KvBlockTables(gpu_lib, blocks=w["blocks"], block_size=16).resize(rows, at["held"], at["lengths"], free, at["cursor"], kept=at["kept"],
+                                                                     cursor_after=at["cursor_after"], slots=slots)
+    torch.cuda.synchronize()
+    assert rows.tolist() == want["tables"] and at["kept"].tolist() == want["kept"] and at["cursor_after"].tolist() == want["cursor"]
+    assert slots.tolist() == want["slots"] and free.tolist() == want["free"]
+    assert at["held"].tolist() == w["held"] and at["lengths"].tolist() == w["lengths"] and at["cursor"].tolist() == w["cursor"]

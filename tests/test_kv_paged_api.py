@@ -257,6 +257,19 @@ def test_the_most_requests_for_a_width(lib, width):
         assert (rc == ERR_ARG) == refused and rc != OK
 
 
+@pytest.mark.parametrize("name,size", [("held", 32), ("lengths", 32), ("kept", 32), ("cursor", 8), ("cursor_after", 8), ("starts", 72), ("free", 40)])
+def test_what_lies_between_the_rows_of_tables(lib, name, size):
+    """8 rows of 64 names, 100 apart: other arrays may lie between two of them and behind the last, and nowhere in one."""
+    at, row, stride = P["tables"], 4 * 64, 4 * 100
+    between = [(k, o) for k in (0, 3, 6) for o in (row, row + (stride - row - size) // 16 * 8, stride - size)] + [(7, row), (7, row + 200), (0, -size)]
+    within = [(k, o) for k in (0, 3, 7) for o in (0, 8, row - 8, 8 - size)]
+    for refused, places in ((False, between), (True, within)):
+        for k, o in places:
+            what = tables(**{name: at + k * stride + o, "table_stride": 100, "ring": 10})
+            rc = lib.lmcache_gpu_kv_resize_async(what, NO_DEVICE, None)
+            assert (rc == ERR_ARG) == refused and rc != OK, (k, o)
+
+
 # ------------------------------------------------------------------ the binding
 
 def cache(cpu_lib, planes=2, head_dim=64, dtype=BF16, layers=2, overlap=False):
