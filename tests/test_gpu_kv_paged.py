@@ -862,3 +862,44 @@ def test_resize_of_arrays_between_the_rows(gpu_lib):
     assert rows.tolist() == want["tables"] and at["kept"].tolist() == want["kept"] and at["cursor_after"].tolist() == want["cursor"]
     assert slots.tolist() == want["slots"] and free.tolist() == want["free"]
     assert at["held"].tolist() == w["held"] and at["lengths"].tolist() == w["lengths"] and at["cursor"].tolist() == w["cursor"]
+
+
+@pytest.mark.parametrize("n,new", [(100_003, 20), ((1 << 20) + 3, 1), ((1 << 22) + 1, 2)])
+def test_resize_of_very_many_requests(gpu_lib, n, new):
+    """Thousands of requests a thread: every one grows, the odd thousandth ends, and all that is written is compared."""
+    size, width = 16, 4
+    g = torch.Generator(device="cuda").manual_seed(n)
+    held = torch.randint(0, 33, (n,), generator=g, device="cuda", dtype=I32)
+    lengths = torch.where(torch.arange(n, device="cuda") % 1000 == 999, 0, held + new).to(I32)
+    before, behind = (held + size - 1) // size, (lengths + size - 1) // size
+    take, give = (behind - before).clamp(min=0), (before - behind).clamp(min=0)
+    taken, given = int(take.sum()), int(give.sum())
+    owned = int(before.sum())
+    blocks = owned + taken + 7
+    names = torch.randperm(blocks, generator=g, device="cuda").to(I32)
+    col = torch.arange(width, device="cuda")
+    first = before.cumsum(0) - before
+    tables = torch.where(col < before[:, None], names[(first[:, None] + col).clamp(max=blocks - 1)], -9).to(I32).contiguous()
+    ring = torch.full((blocks,), -7, dtype=I32, device="cuda")
+    start = blocks - 5                                                  # the free names go over the ring's end
+    ring[(start + torch.arange(taken + 7, device="cuda")) % blocks] = names[owned:]
+    was, was_ring = tables.clone(), ring.clone()
+    tokens = torch.where(lengths > held, lengths - held, 0)
+    total = int(tokens.sum())
+    kept, after = torch.full_like(held, -1), ints([0, 0])
+    slots, starts = torch.zeros(total + 5, dtype=I64, device="cuda"), torch.zeros(n + 1, dtype=I64, device="cuda")
+    KvBlockTables(gpu_lib, blocks=blocks, block_size=size).resize(tables, held, lengths, ring, ints([start, taken + 7]), kept=kept, cursor_after=after,
+                                                                  slots=slots, starts=starts)
+    torch.cuda.synchronize()
+    assert torch.equal(kept, lengths) and after.tolist() == [(start + taken) % blocks, 7 + given]
+    assert torch.equal(starts[1:], tokens.cumsum(0)) and int(starts[0]) == 0
+    at = ((take.cumsum(0) - take)[:, None] + col - before[:, None]).clamp(0, blocks - 1)
+    grown = (col >= before[:, None]) & (col < (before + take)[:, None])
+    assert torch.equal(tables, torch.where(grown, was_ring[(start + at) % blocks], was))
+    returned = was[(col >= behind[:, None]) & (col < before[:, None])]
+    want = was_ring.clone()
+    want[(start + taken + 7 + torch.arange(given, device="cuda")) % blocks] = returned
+    assert torch.equal(ring, want)
+    r = torch.repeat_interleave(torch.arange(n, device="cuda"), tokens.long())
+    token = held[r] + torch.arange(total, device="cuda") - starts[r]
+    assert torch.equal(slots[:total], tables[r, token // size].long() * size + token % size) and bool((slots[total:] == -1).all())
