@@ -12,15 +12,15 @@
 // where the wide kernel below is bound by its instructions.
 //
 // Measured on B200, us of the GPU a call with cold L2 (calls back to back in a graph; TB/s of the cache's bytes and the results):
-//   1 request of 131072 tokens, 8 key heads of 128, 4 query heads each, bfloat16        86     6.24   (89.5 in a run of seconds)
-//   64 requests of up to 4096 tokens, as above                                          31.2   4.44
-//   64 requests of 2048 tokens, as above                                                89     6.04
-//   1000 requests of up to 100 tokens, as above                                         48.7   2.16
-//   1 request of 256 tokens, as above                                                    7.0   0.15   a chain of trips to memory
-//   128 requests of up to 8192 tokens, 1 key head of 128, 8 query heads, half           19.3   2.81
-//   32 requests of up to 4000 tokens, a latent vector of 320, 16 query heads            18.2   0.46
+//   1 request of 131072 tokens, 8 key heads of 128, 4 query heads each, bfloat16        86.7   6.19   (90 in a run of seconds)
+//   64 requests of up to 4096 tokens, as above                                          31.8   4.36
+//   64 requests of 2048 tokens, as above                                                91     5.88
+//   1000 requests of up to 100 tokens, as above                                         49.0   2.14
+//   1 request of 256 tokens, as above                                                    7.1   0.15   a chain of trips to memory
+//   128 requests of up to 8192 tokens, 1 key head of 128, 8 query heads, half           19.8   2.74
+//   32 requests of up to 4000 tokens, a latent vector of 320, 16 query heads            18.5   0.46
 //   64 requests of up to 8192 tokens, a latent vector of 576, 16 query heads            43.8   1.81
-//   17 requests of up to 3001 tokens, 3 key heads of 100, 2 query heads each, float32   16.6   1.98
+//   17 requests of up to 3001 tokens, 3 key heads of 100, 2 query heads each, float32   16.4   2.01
 #pragma once
 
 #include <cuda_runtime.h>

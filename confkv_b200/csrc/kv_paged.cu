@@ -195,11 +195,13 @@ AttendPlan any_plan()
     return AttendPlan{kv::attend_any_kernel<T, VEC, R, GH, U, BLOCKS>, kv::join_kernel<T>, kv::kAttendThreads, GH, BLOCKS * kSms, kv::Cutting{2, 1}, false, 0, nullptr};
 }
 
-// Steps of four values (float32, and what is too long for the 16-bit kernels) or single ones; as many query heads in a row as registers hold,
-// and no more than there are. Fewer blocks an SM than these spill less and hide less; measured, us: 17 requests of up to 3001 tokens, 3 key heads of
-// 100 float32, 2 query heads each, 3 blocks 16.6, 4 blocks 18.2; 16 requests of up to 2048, 8 heads of 128, 8 query heads
+// Steps of four values (float32, and what is too long or too little aligned for the 16-bit kernels) or single ones; as many query heads in a row as
+// registers hold, and no more than there are. Fewer blocks an SM than these spill less and hide less; measured, us: 17 requests of up to 3001 tokens, 3 key
+// heads of 100 float32, 2 query heads each, 3 blocks 16.6, 4 blocks 18.2; 16 requests of up to 2048, 8 heads of 128, 8 query heads
 // each, 2 blocks 46.1, 3 blocks 37.2, 4 blocks with half the tokens a turn 55.4; 32 requests of up to 4000 tokens, 16 query heads on a latent
-// vector of 320 float32, four heads in a row 51, one 154; of 576, two in a row 91, one 165.
+// vector of 320 float32, four heads in a row 51, one 154; of 576, two in a row 91, one 165. In 16 bits, with queries at an odd element, on a latent
+// vector of 320 four in a row 37, 52, 83 and 271 for 4, 8, 16 and 64 heads, one in a row 106, 189, 357 and 1329; of 576 two in a row 48 and 206 for 2 and 16, one 94
+// and 475; 32 requests of up to 2048, 4 key heads of 320, 2 and 8 query heads each, 121 and 202, and 243 and 669; of 640, 2 each, 163 and 358.
 template <class T>
 AttendPlan any_plan(uint32_t d, uint32_t group, bool fours)
 {
@@ -255,10 +257,11 @@ AttendPlan wide_plan()
                       BLOCKS * kSms, kv::Cutting{2, 1}, false, Shape::kShared, &allowed};
 }
 
-// Up to 8 query heads a key head: warps of their own; more, or long vectors: warps that share a tile. Measured, us: 64 requests of up to
-// 8192 tokens, one latent vector of 576, 16 query heads 134 with warps of their own and 44, 128 query heads 524 and 126; 32
-// requests of up to 4096, 8 key heads of 128, 16 query heads each 41 and 35, but of 64 values 25 and 28. Stages and
-// blocks: what fills shared memory.
+// Up to 8 query heads a key head, which fill a product's columns: warps of their own; more, or long vectors: warps that share a tile. Measured, us, own and
+// shared: 32 requests of up to 4096 tokens, 8 key heads of 64 with 5, 8 and 16 query heads each 20.2 and 22.2, 19.7 and 23.2, 25 and 28 (so up to 16 there);
+// of 128 with 5, 8 and 16 25.2 and 34.0, 26.3 and 34.6, 41 and 35; of 256 (up to 2048 tokens) with 5 and 8 30.2 and 39.7, 31.0 and 39.6; one latent vector of 128, 256
+// and 320, 8 query heads, 64 requests of up to 8192 15.5 and 18.5, 23.1 and 26.5, 27.5 and 32.0; of 576, 16 query heads 134 and 44, 64 requests of up to 4096 with 128
+// query heads 524 and 126. Stages and blocks: what fills shared memory.
 template <class T>
 AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t requests)
 {
@@ -287,8 +290,11 @@ AttendPlan mma_plan(const lmcache_gpu_kv_layout& l, uint32_t group, uint64_t req
                       : (many ? wide_plan<T, 576, 2, true, 2, 1>() : wide_plan<T, 576, 1, true, 2, 1>());
 }
 
-// Whether it takes them in copies of 4 or 8 bytes (32 requests of up to 2048 tokens, 8 key heads of 100, 4 query heads each: 26 us, 53 with
-// attend_any_kernel): even head sizes that are no multiple of 8, or addresses of less than 16 bytes.
+// Whether it takes them in copies of 4 or 8 bytes: even head sizes that are no multiple of 8, or addresses of less than 16 bytes. Measured, us, and in brackets with
+// attend_any_kernel: 32 requests of up to 2048 tokens, 8 key heads of 36 with 4 query heads each 17 (53), of 64 with 1, 16 and 64 22 (29), 38 (98) and 112 (323),
+// of 100 with 1, 4 and 64 29 (33), 26 (53) and 132 (341), of 130 and 250 with 4 64 (93) and 99 (101). 32 requests of up to 4000 tokens on a latent vector, all sizes in
+// stages of 320 values: of 2, 36 and 100 with 4 heads 16 (23), 16 (22) and 19 (24), of 64 with 1, 4, 16 and 64 19 (15), 20 (22), 25 (28) and 70 (69), of 128 with 128 131 (125), of
+// 300 with 1, 8 and 64 27 (38), 28 (50) and 110 (269).
 bool mma_takes_small(const lmcache_gpu_kv_layout& l, uint64_t cache_alignment, uint64_t query_alignment)
 {
     return l.dtype != kv::kFp32 && l.head_dim % 2 == 0 && l.head_dim <= (l.planes == 2 ? 256u : 320u) && cache_alignment >= 4 &&
@@ -386,7 +392,8 @@ extern "C" int lmcache_gpu_kv_resize_async(const lmcache_gpu_kv_tables* tables, 
     a.limit = kv::row_limit(t.width, t.block_size);
     a.blocks = t.blocks;
     a.ring = t.ring;
-    // a thread a request or two: 256 requests take 3.3 us with 256 threads and 4.3 with 1024, 2000 take 14.6 and 7.1
+    // a thread a request or two: a token each for 256, 512 and 1024 requests takes 3.2, 3.9 and 5.5 us with 256 threads and 4.3, 4.7 and 5.6 with 1024,
+    // 100 tokens each 3.6, 4.1 and 6.3 and 4.7, 5.2 and 5.4
     const uint32_t threads = t.requests <= 512 ? 256 : 1024;
     a.per = (t.requests + threads - 1) / threads;
     a.by_block = kv::make_fast_div(t.block_size);

@@ -128,8 +128,8 @@ size_t lmcache_gpu_kv_attend_workspace_size(const lmcache_gpu_kv_layout* layout,
  * out, lse and the workspace share no memory with one another or with anything that is read, and the rows of out and lse not with one another.
  *
  * ERR_ARGUMENT before any launch: null or misaligned pointers, a layer that is none, head_dim above 1024, query_heads above 65535, a workspace
- * that is too small, a scale that is not finite (times log2 e, in 32 bits), requests * (width * block_size / 64 + 4) of 2^31 or more, values out of the ranges
- * above or of the codec's.
+ * that is too small, a scale that is not finite (times log2 e, in 32 bits), requests * (width * block_size / 64 + 4) of 2^31 or more (width *
+ * block_size up to 2^31 - 1, which is all that a length counts), values out of the ranges above or of the codec's.
  */
 int lmcache_gpu_kv_attend_async(const lmcache_gpu_kv_layout* layout, const lmcache_gpu_kv_pages* pages, uint32_t layer,
                                 const lmcache_gpu_kv_attention* attention, int device, void* stream);
